@@ -18,6 +18,8 @@ __all__ = [
     "lib", "SGEntry", "HostBuffer", "DeviceBuffer", "CpuPollingThread", "StagingPool",
     "DescriptorQueue", "zero_copy_gather_tokens", "zero_copy_gather", "GfdError",
     "HOST_DEFAULT", "HOST_COHERENT", "HOST_NONCOHERENT", "HOST_NUMA_USER", "QUEUE_SIZE",
+    "BF16", "FP16", "E4M3", "KVCache", "KVRows", "Attention", "kv_append", "paged_attention",
+    "shared_prefix_attention", "attention_workspace_bytes",
 ]
 
 HOST_DEFAULT, HOST_COHERENT, HOST_NONCOHERENT, HOST_NUMA_USER = 0, 1, 2, 4
@@ -67,6 +69,43 @@ class DeviceSGEntry(ctypes.Structure):
 
     _fields_ = [("src", ctypes.c_uint64), ("dst", ctypes.c_uint64), ("size", ctypes.c_uint32),
                 ("tag", ctypes.c_uint32)]
+
+
+# Element types of the paged cache's operators, and the bits of their error word.
+BF16, FP16, E4M3 = 0, 1, 2
+KV_ERR_PAGE, KV_ERR_LENGTH = 1, 2
+
+
+class KVCache(ctypes.Structure):
+    """gfd_kv_cache: keys and values in pages (device pointers, strides in
+    elements).  Made once with the pages; see include/gfd_capi.h."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("num_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
+class KVRows(ctypes.Structure):
+    """gfd_kv_rows: the tokens that kv_append() rotates and stores."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("q_out_stride", ctypes.c_int64), ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("inv_freq", ctypes.c_void_p), ("num_tokens", ctypes.c_int), ("num_q_heads", ctypes.c_int),
+                ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class Attention(ctypes.Structure):
+    """gfd_attention: a batch's queries, lengths, pages and masks."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("doc_start", ctypes.c_void_p), ("prefix_end", ctypes.c_void_p), ("slopes", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int),
+                ("batch", ctypes.c_int), ("num_tokens", ctypes.c_int), ("max_q_len", ctypes.c_int),
+                ("max_kv_len", ctypes.c_int), ("num_q_heads", ctypes.c_int), ("dtype", ctypes.c_int)]
 
 
 DEVICE_SG_ENTRY_DTYPE = np.dtype([("src", np.uint64), ("dst", np.uint64), ("size", np.uint32), ("tag", np.uint32)])
@@ -221,6 +260,12 @@ def _declare(L):
         "gfd_sg_session_enable_trace": ([vp, c_u32], c_int),
         "gfd_sg_session_read_trace": ([vp, vp, c_u32, vp, c_u32, ctypes.POINTER(c_u32), ctypes.POINTER(c_u32)],
                                       c_int),
+        "gfd_kv_append": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), vp, vp], c_int),
+        "gfd_attention_workspace_bytes": ([ctypes.POINTER(KVCache), ctypes.POINTER(Attention), c_int],
+                                          ctypes.c_int64),
+        "gfd_paged_attention": ([ctypes.POINTER(KVCache), ctypes.POINTER(Attention), vp, c_sz, vp, vp], c_int),
+        "gfd_shared_prefix_attention": ([ctypes.POINTER(KVCache), ctypes.POINTER(Attention), vp, c_int, vp, c_sz, vp,
+                                         vp], c_int),
         "gfd_bench_sg_session": ([vp, vp, c_u32, c_u32, c_int, c_int, pd], c_int),
     }
     for name, (args, res) in sig.items():
@@ -812,6 +857,43 @@ class SGWarpSpecSession:
 
 
 SgWarpSpecSession = SGWarpSpecSession
+
+
+# ------------------------------------------------ operators on the paged cache
+
+def kv_append(cache, rows, error_flag=None, stream=None):
+    """Rotate the queries and keys of `rows` (KVRows) to their positions and
+    append the keys and values to `cache` (KVCache).  error_flag: device int
+    that takes KV_ERR_* bits.  See gfd_kv_append in include/gfd_capi.h."""
+    rc = lib().gfd_kv_append(cache, rows, error_flag, stream)
+    if rc:
+        _check(rc, "gfd_kv_append")
+
+
+def attention_workspace_bytes(cache, call, prefix_len=0):
+    """Device bytes that paged_attention() (prefix_len 0) or
+    shared_prefix_attention() needs for `call` (Attention)."""
+    n = lib().gfd_attention_workspace_bytes(cache, call, prefix_len)
+    if n < 0:
+        _check(-1, "gfd_attention_workspace_bytes")
+    return n
+
+
+def paged_attention(cache, call, workspace=None, workspace_bytes=0, error_flag=None, stream=None):
+    """Attention of `call` (Attention) over `cache` (KVCache); see gfd_paged_attention in include/gfd_capi.h."""
+    rc = lib().gfd_paged_attention(cache, call, workspace, workspace_bytes, error_flag, stream)
+    if rc:
+        _check(rc, "gfd_paged_attention")
+
+
+def shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace=None, workspace_bytes=0, error_flag=None,
+                            stream=None):
+    """paged_attention() of sequences whose first prefix_len keys are the same
+    ones, in the pages of prefix_table; they are read once for all."""
+    rc = lib().gfd_shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace, workspace_bytes,
+                                           error_flag, stream)
+    if rc:
+        _check(rc, "gfd_shared_prefix_attention")
 
 
 def build(verbose=False):

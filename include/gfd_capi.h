@@ -512,6 +512,111 @@ int gfd_sg_poller_run(void* queue, void* sg_queue, const gfd_device_sg_entry* d_
                       const uint32_t* d_list_offsets, int num_lists, uint32_t total_entries,
                       uint64_t timeout_us, unsigned long long* list_sums, int* status, void* stream);
 
+/* ---- the paged KV cache's operators; no counterpart in the reference, which
+ * moves a cache's tokens and does not compute on them.  The gather entry
+ * points fill pages; these append a step's keys and values to them and read
+ * them by attention.  Every pointer is device memory.  Calls run on `stream`
+ * (NULL: the default stream) of the current device, allocate nothing, do not
+ * synchronise, and can be captured into a graph.  A refused call launches
+ * nothing, and gfd_last_error() says why. ---- */
+enum { GFD_BF16 = 0, GFD_FP16 = 1, GFD_E4M3 = 2 };  /* element types; E4M3: 8-bit floats (OCP e4m3fn) */
+
+/* Keys and values in pages.  Slot s of page p, head h starts at element
+ * p * page_stride + s * slot_stride + h * head_stride of k and of v; its
+ * head_dim elements are contiguous.  So one 64 KiB page of 16 tokens (keys,
+ * then values) and one 4 KiB token a page are both expressed.  k, v and the
+ * strides (in bytes) are multiples of 16.  head_dim: 64, 128 or 256;
+ * page_size: 1 to 65536.  E4M3: the value is the stored number times k_scale / v_scale
+ * (other types: the scales are not read). */
+typedef struct gfd_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride, slot_stride, head_stride;  /* elements */
+    int num_pages, page_size, num_heads, head_dim;
+    int dtype;
+    float k_scale, v_scale;
+} gfd_kv_cache;
+
+/* Bits of *error_flag (device int, zeroed by the caller; NULL: not reported). */
+enum {
+    GFD_KV_ERR_PAGE = 1,   /* a slot or page outside the cache: not written, read as nothing */
+    GFD_KV_ERR_LENGTH = 2  /* a length past the maximum that the call stated: cut there */
+};
+
+/* The tokens of one step: rows of num_q_heads (k, v: the cache's num_heads)
+ * heads of head_dim elements, heads contiguous, row t at t * its stride.  All
+ * of dtype (GFD_BF16 or GFD_FP16); pointers 16-byte aligned, strides multiples of 8.
+ * Token t goes to slots[t] = page * page_size + slot; a negative one is
+ * skipped (padding; its q is rotated all the same).  Two tokens of one call
+ * must not share a slot. */
+typedef struct gfd_kv_rows {
+    const void* q;     /* NULL: no queries */
+    const void* k;
+    const void* v;
+    void* q_out;       /* the rotated queries; may be q itself */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;  /* elements */
+    const int* positions;
+    const int64_t* slots;
+    const float* inv_freq;  /* rotary_dim / 2 */
+    int num_tokens, num_q_heads;
+    int rotary_dim;    /* even, at most head_dim; 0: no rotation (positions and inv_freq are not read) */
+    int interleaved;   /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+    int dtype;
+} gfd_kv_rows;
+
+/* Rotate q and k to their positions (angle i = position * inv_freq[i], its
+ * turns taken in 64 bits) and append k and v to the cache, converted to its
+ * type: cache = round(x / scale) for E4M3, saturated at +-448 (NaN stays). */
+int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows, int* error_flag, void* stream);
+
+/* Attention of a batch's tokens over the cache.  Sequence b has the tokens
+ * q_start[b] .. q_start[b + 1] of q (any number, also none), which are the
+ * last of its kv_len[b] keys; key j is slot j % page_size of page
+ * block_table[b * table_stride + j / page_size].  Query head h reads head
+ * h / (num_q_heads / num_heads).  Token i of sequence b, at position p =
+ * kv_len[b] - q_len + i, sees the keys lo <= j < hi:
+ *   lo = max(0, doc_start[token], p - window + 1)   (doc_start NULL, window 0: none)
+ *   hi = min(kv_len[b], max(p + 1, prefix_end[token]))   (prefix_end NULL: p + 1)
+ * with the score
+ *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[head] |p - j| if slopes
+ * out = sum of softmax(s) v (zeros where nothing is visible), lse = the
+ * natural logarithm of the sum of exp(s) (-inf there; NULL: not wanted).
+ * Values of slots that no token of the sequence sees are never used. */
+typedef struct gfd_attention {
+    const void* q;     /* rows as in gfd_kv_rows */
+    void* out;
+    float* lse;        /* [num_tokens][num_q_heads] */
+    int64_t q_stride, out_stride;  /* elements */
+    const int* q_start;      /* [batch + 1] */
+    const int* kv_len;       /* [batch] */
+    const int* block_table;  /* [batch][table_stride] */
+    int64_t table_stride;
+    const int* doc_start;    /* [num_tokens] */
+    const int* prefix_end;   /* [num_tokens] */
+    const float* slopes;     /* [num_q_heads] */
+    float scale, softcap;
+    int window;
+    int batch, num_tokens;
+    int max_q_len, max_kv_len;  /* at least the batch's largest */
+    int num_q_heads;
+    int dtype;               /* of q and out: GFD_BF16 or GFD_FP16; the cache's type is the same or E4M3 */
+} gfd_attention;
+
+/* Workspace that the next two need for such a call (prefix_len 0: the first);
+ * -1: the call would be refused.  It grows with num_tokens, max_kv_len and
+ * batch, so that of a program's largest call is enough for all. */
+int64_t gfd_attention_workspace_bytes(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len);
+int gfd_paged_attention(const gfd_kv_cache* cache, const gfd_attention* call, void* workspace,
+                        size_t workspace_bytes, int* error_flag, void* stream);
+/* The same where the first prefix_len keys of every sequence are the same
+ * ones, in the pages prefix_table[j / page_size], and are read once for all
+ * sequences.  kv_len and positions count them; block_table holds what
+ * follows: key j >= prefix_len is slot (j - prefix_len) % page_size of its
+ * page (j - prefix_len) / page_size. */
+int gfd_shared_prefix_attention(const gfd_kv_cache* cache, const gfd_attention* call, const int* prefix_table,
+                                int prefix_len, void* workspace, size_t workspace_bytes, int* error_flag,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
