@@ -1,0 +1,406 @@
+#pragma once
+// Attention of few rows: single tokens, drafted tokens, small shared prefixes.
+//
+// Up to 16 or 32 rows share a head's keys and values, so each byte is used for
+// at most 32 rows and the cache's bytes bound the time.  What counts is loads in
+// flight: the waves of a workgroup take tiles of 32 keys by turns, straight
+// from memory to registers and without waiting for one another, the next
+// tile's keys under way during a tile's softmax and its values during the next
+// scores.  A long axis is split over workgroups.
+//
+// A tile: scores^T[32 keys][16 rows] by 16x16x32 products, keys as the left operand
+// (lane: key l % 16, 8 dims of a 32, by l / 16).  Result: lane holds row l % 16 and the keys
+// 4 (l / 16) + r of both halves.  As the right operand of out^T += V^T P the
+// lane has to hold 8 keys of a 32, and which 8 is free as long as the values agree: so it
+// keeps its own, and loads the values of those 8 keys, D / 16 adjacent
+// dims each (a row of D by 16 lanes).  Left operand i takes dim i of every lane: two
+// neighbouring keys' halves joined by a byte permutation, no LDS.
+#include "paged_attention.h"
+
+namespace gfd {
+namespace kv {
+
+constexpr int kRowsBlock = 256, kRowsTile = 32, kRowsMaxChunk = 1024;
+
+template <int N>
+struct Words {
+    uint32_t w[N];
+};
+
+template <int N>  // words
+__device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
+    Words<N> r;
+    if constexpr (N == 1) {
+        r.w[0] = *(const uint32_t*)p;
+    } else if constexpr (N == 2) {
+        const u32x2 x = *(const u32x2*)p;
+        r.w[0] = x[0];
+        r.w[1] = x[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const u32x4 x = *(const u32x4*)(p + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) r.w[i + j] = x[j];
+        }
+    }
+    return r;
+}
+
+template <typename T, typename S, int D, int R>
+struct RowsKernel {
+    static constexpr int kSize = S::kBytes;
+    static constexpr int kDims = D / 16;                   // a lane's dims of a value row
+    static constexpr int kSteps = D / 32;                  // products per 16 keys
+    static constexpr int kKeyWords = D / 4 * kSize / 4;    // a lane's words of a key: a quarter of its dims
+    static constexpr int kValWords = kDims * kSize / 4;
+    static constexpr int kAcc = kDims * 4;                 // a lane's outputs per 16 rows
+    // 32 rows of 128 dims and more: with the rows' operand in registers too, a lane would need more than it has.
+    static constexpr bool kLdsRows = R == 2 && D >= 128;
+
+    struct Tile {
+        Words<kKeyWords> k[2];
+        Words<kValWords> v[8];
+    };
+
+    // Dims of product step s and quarter g start here: 16-byte loads of 64 contiguous bytes per key.
+    static __device__ __forceinline__ int step_dim(int s, int g) {
+        return kSize == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
+    }
+
+    static __device__ __forceinline__ void load_keys(Tile& t, const Cache& c, const int64_t* off, int lane) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int64_t o = off[16 * h + (lane & 15)];
+            const uint8_t* p = c.k + (o < 0 ? 0 : o) + 16 * (lane >> 4);
+#pragma unroll
+            for (int i = 0; i < kKeyWords; i += 4) {
+                const u32x4 x = *(const u32x4*)(p + 16 * i);  // 64 bytes of the row by the four quarters
+#pragma unroll
+                for (int j = 0; j < 4; j++) t.k[h].w[i + j] = x[j];
+            }
+        }
+    }
+    static __device__ __forceinline__ int load_values(Tile& t, const Cache& c, const int64_t* off, int lane) {
+        int valid = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int64_t o = off[16 * (j >> 2) + 4 * (lane >> 4) + (j & 3)];
+            valid |= (o >= 0) << j;
+            t.v[j] = load_words<kValWords>(c.v + (o < 0 ? 0 : o) + (lane & 15) * kDims * kSize);
+        }
+        return valid;
+    }
+
+    // Keys' operand of step s.
+    static __device__ __forceinline__ u32x4 key_frag(const Words<kKeyWords>& k, int s) {
+        if constexpr (kSize == 2) {
+            return u32x4{k.w[4 * s], k.w[4 * s + 1], k.w[4 * s + 2], k.w[4 * s + 3]};
+        } else {
+            const uint32_t a = k.w[2 * s], b = k.w[2 * s + 1];
+            return u32x4{Mma<T>::widen_lo(a), Mma<T>::widen_hi(a), Mma<T>::widen_lo(b), Mma<T>::widen_hi(b)};
+        }
+    }
+    // Word i of a value row in 16-bit pairs.
+    static __device__ __forceinline__ uint32_t value_pair(const Words<kValWords>& v, int i) {
+        if constexpr (kSize == 2) return v.w[i];
+        else return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
+    }
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b, int odd) {
+        return __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
+    }
+};
+
+template <typename T, typename S, int D, int R>
+__global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kernel(Call a, Cache c,
+                                                                                    Stage prefix, Stage own) {
+    using K = RowsKernel<T, S, D, R>;
+    constexpr int kRows = 16 * R, kWaves = kRowsBlock / 64;
+    __shared__ i32x4 rows[kRows];
+    __shared__ int64_t offsets[kRowsMaxChunk];
+    __shared__ union {
+        int samples[kSamples + 1];
+        float merge[kWaves / 2][R * K::kAcc + 2 * R][64];
+    } lds;
+    __shared__ int any_bad;
+    __shared__ u32x4 lds_rows[K::kLdsRows ? R * K::kSteps : 1][64];
+
+    // Heads vary fastest: their keys lie side by side.  Ranges vary slowest: the last ones are often empty.
+    int item = (int)blockIdx.x;
+    const int prefix_items = prefix.blocks * prefix.splits * a.kv_heads;
+    const Stage st = item < prefix_items ? prefix : own;
+    if (item >= prefix_items) item -= prefix_items;
+    const int kv_head = item % a.kv_heads, block = item / a.kv_heads % st.blocks,
+              split = item / a.kv_heads / st.blocks;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+
+    Block k;
+    if (!find_rows<kRows>(a, st, block, &k)) return;
+    if (st.prefix) {
+        sample_starts(a, lds.samples, kRowsBlock);
+        __syncthreads();
+    }
+    Range g{0x7FFFFFFF, 0, 0, 0x7FFFFFFF};
+    if (wave == 0 && lane < kRows) {
+        const Row r = row_of(a, st, k, lds.samples, lane);
+        rows[lane] = i32x4{r.t, r.pos, r.lo, r.hi};
+    }
+    if (tid == 0) any_bad = 0;
+    __syncthreads();
+    Row row[R];
+    for (int i = 0; i < R; i++) {
+        const i32x4 x = rows[16 * i + col];
+        row[i] = Row{x[0], x[1], x[2], x[3]};
+        range_add(g, row[i]);
+    }
+    g.lo = lanes_min(g.lo);
+    g.hi = -lanes_min(-g.hi);
+    g.all_lo = -lanes_min(-g.all_lo);
+    g.all_hi = lanes_min(g.all_hi);
+    if (g.hi == 0) g.lo = 0;
+
+    const int splits = st.prefix ? st.splits : max(1, (g.hi - g.lo + st.chunk - 1) / st.chunk);
+    if (split >= splits) return;
+    const int base = (st.prefix ? 0 : g.lo) + split * st.chunk;
+    const int c0 = max(base, g.lo), c1 = min(base + st.chunk, g.hi);
+    const int64_t head = kv_head * c.head_stride;
+    const int tiles = c1 > c0 ? (c1 - c0 + kRowsTile - 1) / kRowsTile : 0;
+    for (int n = tid; n < tiles * kRowsTile; n += kRowsBlock) {
+        const int64_t o = c0 + n < c1 ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
+        if (o < 0 && c0 + n < c1) any_bad = 1;
+        offsets[n] = o;
+    }
+
+    // The rows' operand, zero where there is no row.
+    u32x4 q[K::kLdsRows ? 1 : R][K::kSteps];
+    Score sc[R];
+    const float raw = a.scale * c.k_scale;
+    const bool extras = a.softcap > 0.f || a.slopes;
+    for (int i = 0; i < R; i++) {
+        const int h = head_of(a, k, 16 * i + col, kv_head);
+        const uint16_t* p = a.q + row[i].t * a.q_stride + (int64_t)h * D;
+        for (int s = 0; s < K::kSteps; s++) {
+            if (K::kLdsRows && wave != (i * K::kSteps + s) % kWaves) continue;
+            const u32x4 x = row[i].t >= 0 ? *(const u32x4*)(p + K::step_dim(s, quarter)) : u32x4{0, 0, 0, 0};
+            if constexpr (K::kLdsRows) lds_rows[i * K::kSteps + s][lane] = x;
+            else q[i][s] = x;
+        }
+        sc[i].factor = raw * kLog2e;
+        sc[i].in = a.softcap > 0.f ? raw / a.softcap : 0.f;
+        sc[i].cap = a.softcap * kLog2e;
+        sc[i].slope = a.slopes && row[i].t >= 0 ? a.slopes[h] * kLog2e : 0.f;
+    }
+    const float factor = extras ? 1.f : raw * kLog2e;
+
+    __syncthreads();
+    const bool bad = any_bad != 0;
+    float m[R], sum[R];
+    f32x4 o[R][K::kDims];
+    for (int i = 0; i < R; i++) {
+        m[i] = -INFINITY;
+        sum[i] = 0.f;
+        for (int d = 0; d < K::kDims; d++) o[i][d] = f32x4{0, 0, 0, 0};
+    }
+    typename K::Tile t;
+    int valid = 0;
+    if (wave < tiles) {
+        K::load_keys(t, c, offsets + wave * kRowsTile, lane);
+        valid = K::load_values(t, c, offsets + wave * kRowsTile, lane);
+    }
+    for (int tile = wave; tile < tiles; tile += kWaves) {
+        const int n0 = c0 + tile * kRowsTile;
+        const bool more = tile + kWaves < tiles;
+        const int64_t* next = offsets + (tile + kWaves) * kRowsTile;
+        if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
+        f32x4 x[R][2];
+#pragma unroll
+        for (int i = 0; i < R; i++) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < K::kSteps; s++) {
+            const u32x4 k0 = K::key_frag(t.k[0], s), k1 = K::key_frag(t.k[1], s);
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                u32x4 qf;
+                if constexpr (K::kLdsRows) qf = lds_rows[i * K::kSteps + s][lane];
+                else qf = q[i][s];
+                x[i][0] = Mma<T>::m16(k0, qf, x[i][0]);
+                x[i][1] = Mma<T>::m16(k1, qf, x[i][1]);
+            }
+        }
+        if (more) K::load_keys(t, c, next, lane);
+        const bool whole = !bad && g.all_lo <= n0 && n0 + kRowsTile <= min(g.all_hi, c1);
+        u32x4 p[R];
+        uint32_t seen[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            if (extras) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[i][j >> 2][j & 3] = score<true>(sc[i], a, x[i][j >> 2][j & 3], row[i].pos,
+                                                      n0 + 16 * (j >> 2) + 4 * quarter + (j & 3));
+            }
+            seen[i] = 0xFF;
+            if (!whole) {
+                seen[i] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int n = n0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
+                    const bool on = n >= row[i].lo && n < row[i].hi && ((valid >> j) & 1);
+                    seen[i] |= (uint32_t)on << j;
+                    if (!on) x[i][j >> 2][j & 3] = -INFINITY;
+                }
+            }
+            float top = x[i][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) top = max_f32(top, x[i][j >> 2][j & 3]);
+            top = across16_max(top);
+            if (__any(!(top <= m[i]))) {
+                const float next_m = max_f32(m[i], top);
+                const float keep = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - next_m) * factor);
+                m[i] = next_m;
+                sum[i] *= keep;
+#pragma unroll
+                for (int d = 0; d < K::kDims; d++) o[i][d] *= keep;
+            }
+            const float base_m = m[i] == -INFINITY ? 0.f : m[i] * factor;
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j >> 2][j & 3], factor, -base_m));
+                sum[i] += e[j];
+            }
+            // A weight is rounded to the values' 16-bit type, as the matrix product takes it.
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[i][j] = T::pack(e[2 * j], e[2 * j + 1]);
+        }
+        if (whole) {
+#pragma unroll
+            for (int d = 0; d < K::kDims; d++) {
+                u32x4 vf;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
+#pragma unroll
+                for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
+            }
+        } else {
+            // Values of keys outside the range count as zeros, and of keys that some rows
+            // see and others do not, infinities and NaN reach only the rows that do: a weight
+            // of zero would not stop them.
+            uint32_t odd = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+#pragma unroll
+                for (int i = 0; i < K::kValWords; i++) t.v[j].w[i] = (valid >> j) & 1 ? t.v[j].w[i] : 0u;
+#pragma unroll
+                for (int i = 0; i < K::kDims / 2; i++) odd |= not_finite<T>(K::value_pair(t.v[j], i));
+            }
+            const bool any_odd = __any(odd != 0);
+#pragma unroll
+            for (int d = 0; d < K::kDims; d++) {
+                u32x4 vf;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
+                if (any_odd) {
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; kind++) {
+                        u32x4 is;
+                        for (int j = 0; j < 4; j++) is[j] = of_kind<T>(vf[j], kind);
+                        for (int i = 0; i < R; i++) {
+                            u32x4 on;
+                            for (int j = 0; j < 4; j++)
+                                on[j] = ((seen[i] >> (2 * j)) & 1 ? Mma<T>::kOne : 0u) |
+                                        ((seen[i] >> (2 * j + 1)) & 1 ? Mma<T>::kOne << 16 : 0u);
+                            const f32x4 count = Mma<T>::m16(is, on, f32x4{0, 0, 0, 0});
+                            for (int r = 0; r < 4; r++)
+                                if (count[r] > 0.f) o[i][d][r] += kind_value(kind);
+                        }
+                    }
+                    for (int j = 0; j < 4; j++) vf[j] = only_finite<T>(vf[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
+            }
+        }
+        if (more) valid = K::load_values(t, c, next, lane);
+    }
+
+    // The waves' results joined pairwise, in the lanes' own layout.
+#pragma unroll
+    for (int i = 0; i < R; i++) sum[i] = across16_sum(sum[i]);
+    for (int half = kWaves / 2; half; half /= 2) {
+        if (wave >= half && wave < 2 * half) {
+            float(*to)[64] = lds.merge[wave - half];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                to[2 * i][lane] = m[i];
+                to[2 * i + 1][lane] = sum[i];
+#pragma unroll
+                for (int d = 0; d < K::kAcc; d++) to[2 * R + i * K::kAcc + d][lane] = o[i][d >> 2][d & 3];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+            float(*from)[64] = lds.merge[wave];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const float m2 = from[2 * i][lane], top = max_f32(m[i], m2);
+                const float keep = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - top) * factor);
+                const float take = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - top) * factor);
+                m[i] = top;
+                sum[i] = sum[i] * keep + from[2 * i + 1][lane] * take;
+#pragma unroll
+                for (int d = 0; d < K::kAcc; d++)
+                    o[i][d >> 2][d & 3] = o[i][d >> 2][d & 3] * keep + from[2 * R + i * K::kAcc + d][lane] * take;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        if (row[i].t < 0) continue;
+        const int h = head_of(a, k, 16 * i + col, kv_head);
+        if (st.direct && splits == 1) {
+            const float w = sum[i] == 0.f ? 0.f : c.v_scale / sum[i];
+            uint16_t* out = a.out + row[i].t * a.out_stride + (int64_t)h * D + 4 * quarter * K::kDims;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int d = 0; d < K::kDims; d += 4) {
+                    const u32x2 y{T::pack(o[i][d][r] * w, o[i][d + 1][r] * w),
+                                  T::pack(o[i][d + 2][r] * w, o[i][d + 3][r] * w)};
+                    *(u32x2*)(out + r * K::kDims + d) = sum[i] == 0.f ? u32x2{0, 0} : y;
+                }
+            if (a.lse && quarter == 0)
+                a.lse[(int64_t)row[i].t * a.q_heads + h] =
+                    sum[i] == 0.f ? -INFINITY : (m[i] * factor + __builtin_amdgcn_logf(sum[i])) * kLn2;
+        } else {
+            const int64_t at = slot_of(a, st.first_slot + split, row[i].t, h);
+            if (quarter == 0) a.part_ml[at] = f32x2{m[i] == -INFINITY ? m[i] : m[i] * factor, sum[i]};
+            float* out = a.part_o + at * D + 4 * quarter * K::kDims;
+            if (sum[i] == 0.f) continue;  // its weight is zero and it is not read
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int d = 0; d < K::kDims; d += 4)
+                    *(f32x4*)(out + r * K::kDims + d) =
+                        f32x4{o[i][d][r], o[i][d + 1][r], o[i][d + 2][r], o[i][d + 3][r]};
+        }
+    }
+}
+
+template <typename T, typename S>
+int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+                hipStream_t st) {
+    const dim3 grid((unsigned)((prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads));
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kRowsBlock), 0, st, a, c, prefix, own); };
+    if (dim == 64) wide ? go(attend_rows_kernel<T, S, 64, 2>) : go(attend_rows_kernel<T, S, 64, 1>);
+    if (dim == 128) wide ? go(attend_rows_kernel<T, S, 128, 2>) : go(attend_rows_kernel<T, S, 128, 1>);
+    if (dim == 256) wide ? go(attend_rows_kernel<T, S, 256, 2>) : go(attend_rows_kernel<T, S, 256, 1>);
+    return (int)hipGetLastError();
+}
+
+}  // namespace kv
+}  // namespace gfd

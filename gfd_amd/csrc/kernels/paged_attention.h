@@ -1,0 +1,353 @@
+#pragma once
+// What the kernels of attention over the paged cache share: a call as a kernel
+// sees it, the rows and key ranges that a workgroup takes, and partial results
+// (HIP sources only).
+//
+// A query row is a (token, head) pair; the rows of one head of the cache are
+// packed token by token, group heads a token, so that keys and values are read
+// once for the whole group.  Scores are computed transposed, keys x rows: in the
+// matrix instructions' result layout a lane then holds the scores of one row,
+// which are, rounded, the very operand that the product with the values takes.
+// Maxima, sums and rescaling are a lane's own, but for one exchange a tile.
+#include "paged_kv.h"
+
+namespace gfd {
+namespace kv {
+
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+struct Call {
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    int64_t q_stride, out_stride;
+    const int* q_start;
+    const int* kv_len;
+    const int* table;
+    int64_t table_stride;
+    const int* prefix_table;
+    int prefix_len;
+    const int* doc_start;
+    const int* prefix_end;
+    const float* slopes;
+    float scale, softcap;
+    int window, batch, num_tokens, max_q_len, max_kv_len, q_heads, kv_heads;
+    Divider group;
+    int* error;
+    // Partial results, [slot][token][head]: maximum and sum, and the unnormalised output.
+    f32x2* part_ml;
+    float* part_o;
+};
+
+// One kind of work of a launch: row blocks times key ranges times the cache's heads.
+struct Stage {
+    int prefix;      // 1: the shared prefix's keys, rows of all tokens; 0: what follows, sequence by sequence
+    int blocks;      // row blocks; one per sequence if whole
+    int whole;       // a sequence's rows fit a block
+    int splits;      // key ranges per block, at most
+    int chunk;       // keys per range
+    int first_slot;  // of its partial results
+    int direct;      // a block with one range writes the result itself
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// A row as its lane needs it; keys count from the stage's first.  t < 0: no row.
+struct Row {
+    int t, pos, lo, hi;
+};
+
+// Tokens of sequence b that the call covers.
+struct Sequence {
+    int first, q_len, rows_q, kv_len;  // rows_q: at most max_q_len
+    bool cut;
+};
+
+__device__ __forceinline__ Sequence sequence(const Call& a, int b) {
+    Sequence s;
+    s.first = min(max(a.q_start[b], 0), a.num_tokens);
+    s.q_len = min(max(a.q_start[b + 1], s.first), a.num_tokens) - s.first;
+    s.rows_q = min(s.q_len, a.max_q_len);
+    const int n = a.kv_len[b];
+    s.kv_len = min(n, a.max_kv_len);
+    s.cut = s.q_len > a.max_q_len || n > a.max_kv_len;
+    return s;
+}
+
+__device__ __forceinline__ Row make_row(const Call& a, const Sequence& s, int i, bool prefix) {
+    Row r;
+    r.t = s.first + i;
+    r.pos = s.kv_len - s.q_len + i;
+    r.lo = a.doc_start ? max(a.doc_start[r.t], 0) : 0;
+    if (a.window > 0) r.lo = max(r.lo, r.pos - a.window + 1);
+    r.hi = min(s.kv_len, a.prefix_end ? max(r.pos + 1, a.prefix_end[r.t]) : r.pos + 1);
+    if (prefix) {
+        r.hi = min(r.hi, a.prefix_len);
+    } else {
+        r.pos -= a.prefix_len;
+        r.lo = max(r.lo - a.prefix_len, 0);
+        r.hi -= a.prefix_len;
+    }
+    if (r.hi <= r.lo) r.lo = r.hi = 0;
+    return r;
+}
+
+// Where index lies among the blocks of kRows rows that the sequences have, the
+// last block of a sequence first: it sees the most keys.  A wave's lanes each
+// count a sequence's blocks.
+template <int kRows>
+__device__ __forceinline__ bool find_block(const Call& a, int index, int* b, int* block) {
+    const int lane = (int)threadIdx.x & 63;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        int n = 0;
+        if (b0 + lane < a.batch) {
+            const int first = min(max(a.q_start[b0 + lane], 0), a.num_tokens);
+            const int q_len = min(min(max(a.q_start[b0 + lane + 1], first), a.num_tokens) - first, a.max_q_len);
+            n = (int)(((int64_t)q_len * a.group.d + kRows - 1) / kRows);
+        }
+        int sum = n;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(sum, off);
+            if (lane >= off) sum += up;
+        }
+        const int total = __shfl(sum, 63);
+        if (index < total) {
+            const int at = __ffsll((long long)__ballot(index < sum)) - 1;
+            *b = b0 + at;
+            *block = __builtin_amdgcn_readfirstlane(__shfl(sum, at) - 1 - index);
+            return true;
+        }
+        index -= total;
+    }
+    return false;
+}
+
+// The last sequence b with q_start[b] <= t, by every step-th entry in LDS.
+constexpr int kSamples = 512;
+__device__ __forceinline__ void sample_starts(const Call& a, int* samples, int threads) {
+    const int step = (a.batch + kSamples - 1) / kSamples;
+    for (int i = (int)threadIdx.x; i <= kSamples; i += threads) samples[i] = a.q_start[min(i * step, a.batch)];
+}
+__device__ __forceinline__ int sequence_of(const Call& a, const int* samples, int t) {
+    const int step = (a.batch + kSamples - 1) / kSamples;
+    if (t < samples[0] || t >= samples[kSamples]) return -1;
+    int lo = 0, hi = kSamples;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (samples[mid] <= t) lo = mid; else hi = mid;
+    }
+    lo *= step;
+    hi = min(lo + step, a.batch);
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.q_start[mid] <= t) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// The rows of a workgroup and the keys that any of them sees.
+struct Block {
+    int b, first_row, rows;  // rows of the sequence (own keys) or of all tokens (prefix)
+    const int* table;
+};
+
+// What rows [0, rows) of a block see: [lo, hi) by any, [all_lo, all_hi) by every one.
+struct Range {
+    int lo, hi, all_lo, all_hi;
+};
+
+__device__ __forceinline__ void range_add(Range& g, const Row& r) {
+    if (r.t < 0) return;
+    if (r.hi > r.lo) {
+        g.lo = min(g.lo, r.lo);
+        g.hi = max(g.hi, r.hi);
+    }
+    g.all_lo = max(g.all_lo, r.lo);
+    g.all_hi = min(g.all_hi, r.hi);
+}
+
+__device__ __forceinline__ int lanes_min(int x) {
+    for (int off = 32; off; off >>= 1) x = min(x, __shfl_xor(x, off));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Sets up rows[0, kRows) in LDS by one wave per 64 rows and returns what each
+// wave's rows see.  False: nothing for this block.
+template <int kRows>
+__device__ __forceinline__ bool find_rows(const Call& a, const Stage& st, int block_index, Block* k) {
+    k->b = 0;
+    if (st.prefix) {
+        k->first_row = block_index * kRows;
+        k->rows = (int)min((int64_t)kRows, (int64_t)a.num_tokens * a.group.d - k->first_row);
+        k->table = a.prefix_table;
+        return true;
+    }
+    int at = 0;
+    if (st.whole) {
+        k->b = block_index;
+    } else if (!find_block<kRows>(a, block_index, &k->b, &at)) {
+        return false;
+    }
+    k->first_row = at * kRows;
+    k->table = a.table + (int64_t)k->b * a.table_stride;
+    const int first = min(max(a.q_start[k->b], 0), a.num_tokens);
+    const int q_len = min(min(max(a.q_start[k->b + 1], first), a.num_tokens) - first, a.max_q_len);
+    k->rows = (int)min((int64_t)kRows, (int64_t)q_len * a.group.d - k->first_row);
+    return k->rows > 0;
+}
+
+// Row r of a block.
+__device__ __forceinline__ Row row_of(const Call& a, const Stage& st, const Block& k, const int* samples, int r) {
+    Row x{-1, 0, 0, 0};
+    if (r >= k.rows) return x;
+    const int i = (int)a.group.div((uint32_t)(k.first_row + r));
+    if (!st.prefix) {
+        const Sequence s = sequence(a, k.b);
+        if (s.cut && a.error) atomicOr(a.error, GFD_KV_ERR_LENGTH);
+        return make_row(a, s, i, false);
+    }
+    const int b = sequence_of(a, samples, i);
+    if (b < 0) return x;
+    const Sequence s = sequence(a, b);
+    if (i - s.first >= s.rows_q || i < s.first) return x;
+    return make_row(a, s, i - s.first, true);
+}
+
+__device__ __forceinline__ int head_of(const Call& a, const Block& k, int r, int kv_head) {
+    const uint32_t n = (uint32_t)(k.first_row + r);
+    return kv_head * (int)a.group.d + (int)(n - a.group.div(n) * a.group.d);
+}
+
+// Byte offset of a key, -1 where its page is none of the cache's.
+__device__ __forceinline__ int64_t key_offset(const Cache& c, const int* table, int n, int64_t head, int* error) {
+    const uint32_t page = c.page.div((uint32_t)n);
+    const int id = table[page];
+    if (id < 0 || id >= c.num_pages) {
+        if (error) atomicOr(error, GFD_KV_ERR_PAGE);
+        return -1;
+    }
+    return id * c.page_stride + (int64_t)((uint32_t)n - page * c.page.d) * c.slot_stride + head;
+}
+
+__device__ __forceinline__ int64_t slot_of(const Call& a, int slot, int t, int h) {
+    return ((int64_t)slot * a.num_tokens + t) * a.q_heads + h;
+}
+
+// Scores in the exponent's units (base 2).  Without cap and bias they stay the
+// product's raw sums: the factor is positive, so the maximum is the same, and
+// one multiply-add under the exponent applies it.
+struct Score {
+    float factor;    // raw -> exponent
+    float in, cap;   // with a cap: cap * tanh(raw * in)
+    float slope;
+    bool extras;
+};
+
+// tanh(y) = 1 - 2 / (e^2y + 1): off by a few 2^-24 of 1, as the sums are.
+__device__ __forceinline__ float capped(float y) {
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
+}
+
+template <bool kExtras>
+__device__ __forceinline__ float score(const Score& s, const Call& a, float raw, int pos, int key) {
+    if (!kExtras) return raw;
+    float x = a.softcap > 0.f ? s.cap * capped(raw * s.in) : raw * s.factor;
+    return __builtin_fmaf(-s.slope, fabsf((float)(pos - key)), x);
+}
+
+__device__ __forceinline__ float max_f32(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The maximum, or the sum, over the lanes that share a row.
+__device__ __forceinline__ float across32_max(float x) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_f32(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float across32_sum(float x) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float across16_max(float x) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return across32_max(max_f32(__uint_as_float(p[0]), __uint_as_float(p[1])));
+}
+__device__ __forceinline__ float across16_sum(float x) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return across32_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+}
+
+// Matrix instructions by element type, and tests on packed pairs.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<Bf16> {
+    static constexpr uint32_t kNear = 0x00800080u;  // added to a magnitude: bit 15 is set from infinity on
+    static constexpr uint32_t kOne = 0x3F80u;
+    static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    // Two 8-bit floats (bits 0..15 of w, or 16..31): exact.
+    static __device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    }
+    static __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+    }
+};
+template <>
+struct Mma<Fp16> {
+    static constexpr uint32_t kNear = 0x04000400u;
+    static constexpr uint32_t kOne = 0x3C00u;
+    static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+    }
+    static __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    }
+};
+
+// Bits 15 and 31 say which of a pair's values are infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & 0x7FFF7FFFu) + Mma<T>::kNear) & 0x80008000u;
+}
+// A pair with infinities and NaN made zero; and the pair of ones where the value is of a kind (0 NaN, 1 +inf, 2 -inf).
+template <typename T>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {
+    const uint32_t bad = not_finite<T>(w) >> 15;
+    return w & ~(bad * 0xFFFFu);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t of_kind(uint32_t w, int kind) {
+    uint32_t r = 0;
+    for (int h = 0; h < 2; h++) {
+        const uint32_t x = (w >> (16 * h)) & 0xFFFFu, inf = 0x8000u - (Mma<T>::kNear & 0xFFFFu);
+        const bool hit = kind == 0 ? (x & 0x7FFFu) > inf : x == (inf | (kind == 2 ? 0x8000u : 0u));
+        r |= (hit ? Mma<T>::kOne : 0u) << (16 * h);
+    }
+    return r;
+}
+__device__ __forceinline__ float kind_value(int kind) {
+    return kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
+}
+
+template <typename T, typename S>
+int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+                hipStream_t st);
+
+}  // namespace kv
+}  // namespace gfd
