@@ -348,6 +348,9 @@ __device__ __forceinline__ float kind_value(int kind) {
 template <typename T, typename S>
 int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
                 hipStream_t st);
+template <typename T, typename S>
+int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
+                 hipStream_t st);
 
 }  // namespace kv
 }  // namespace gfd

@@ -12,6 +12,7 @@
 #include <cstdio>
 
 #include "attend_rows.h"
+#include "attend_tiles.h"
 #include "capi_error.h"
 #include "gfd_capi.h"
 #include "paged_attention.h"
@@ -95,97 +96,98 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
     }
 }
 
-// The sequence that token t belongs to: the last b with q_start[b] <= t; -1 if none.
-__device__ __forceinline__ int simple_sequence_of(const Call& a, int t) {
-    int lo = 0, hi = a.batch;  // q_start[lo] <= t < q_start[hi]
-    if (t < a.q_start[0] || t >= a.q_start[a.batch]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.q_start[mid] <= t) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-struct Seen {
-    int pos, lo, hi;
+// How a call is cut into row blocks and key ranges.
+struct Plan {
+    int prefix_waves, own_waves;  // of a block of 32 rows a wave; 0: few rows (attend_rows.h)
+    int rows;                     // of an own-keys block
+    Stage prefix, own;
+    int slots;      // partial results per row
+    int64_t items;  // workgroups of the largest launch
+    int64_t bytes;  // of workspace
 };
 
-__device__ __forceinline__ Seen visible(const Call& a, int t, int i, int q_len, int kv_len) {
-    Seen s;
-    s.pos = kv_len - q_len + i;
-    s.lo = a.doc_start ? max(a.doc_start[t], 0) : 0;
-    if (a.window > 0) s.lo = max(s.lo, s.pos - a.window + 1);
-    s.hi = min(kv_len, a.prefix_end ? max(s.pos + 1, a.prefix_end[t]) : s.pos + 1);
-    return s;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Few rows: below kFill workgroups a block's keys are split, into ranges of at least a
+// tile per wave.  Ranges also end at kRowsMaxChunk, so that sequences of very different
+// lengths are evenly spread.
+constexpr int kFill = 2048, kMinChunk = 128;
+// Many rows: a workgroup fills a CU (or half of it), so two rounds of them do.
+constexpr int kTilesFill = 512, kTilesMinChunk = 256;
+
+void split(Stage* st, int64_t items, int64_t keys, bool few) {
+    if (few) {
+        const int64_t want = ceil_div(ceil_div(keys * items, kFill), kMinChunk) * kMinChunk;
+        st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max<int64_t>(kMinChunk, want));
+    } else {
+        const int64_t parts = std::max<int64_t>(1, kTilesFill / std::max<int64_t>(items, 1));
+        st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
+    }
+    st->splits = (int)std::max<int64_t>(1, ceil_div(keys, st->chunk));
 }
 
-template <typename T>
-__device__ __forceinline__ float load_one(const uint8_t* p, int i) { return T::unpack(((const uint16_t*)p)[i])[0]; }
-template <>
-__device__ __forceinline__ float load_one<E4m3>(const uint8_t* p, int i) {
-    return __builtin_amdgcn_cvt_f32_fp8((int)p[i], 0);
+// Waves of a block of many rows: 8 where that still fills the card, for half the reads of the cache.
+int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= 256 * 256 ? 8 : 4; }
+
+Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
+    Plan p{};
+    const int64_t group = w.num_q_heads / cache.num_heads, heads = cache.num_heads;
+    const int64_t seq_rows = std::min<int64_t>(w.max_q_len, w.num_tokens) * group;
+    const int64_t all_rows = w.num_tokens * group;
+    // Keys that a block can see: with a window, those of its tokens' windows (a prefix mask adds later keys).
+    int64_t keys = std::max(w.max_kv_len - prefix_len, 0);
+    if (w.window && !w.prefix_end) keys = std::min<int64_t>(keys, (int64_t)w.window + w.max_q_len);
+    if (seq_rows <= 32) {
+        p.rows = seq_rows <= 16 ? 16 : 32;
+        if (prefix_len && all_rows <= 32) p.rows = all_rows <= 16 ? 16 : 32;  // one launch takes both stages
+        p.own.blocks = w.batch;
+        p.own.whole = 1;
+    } else {
+        p.own_waves = tile_waves(all_rows, heads, cache.head_dim);
+        p.rows = 32 * p.own_waves;
+        p.own.blocks = (int)std::min<int64_t>(w.batch * ceil_div(seq_rows, p.rows), all_rows / p.rows + w.batch);
+    }
+    split(&p.own, p.own.blocks * heads, keys, !p.own_waves);
+    p.own.direct = !prefix_len;
+    if (prefix_len) {
+        p.prefix.prefix = 1;
+        p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : tile_waves(all_rows, heads, cache.head_dim);
+        p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
+        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves);
+        p.own.first_slot = p.prefix.splits;
+    }
+    p.slots = p.own.first_slot + p.own.splits;
+    p.items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
+    if (p.slots > 1) p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4;
+    return p;
 }
 
-// One wave per row: a lane scores one key of 64, then holds dim lane + 64 k of the sum.
-template <typename T, typename S, int D>
-__global__ __launch_bounds__(64) void attend_kernel(Call a, Cache c) {
-    const int t = (int)blockIdx.x, h = (int)blockIdx.y, lane = (int)threadIdx.x;
-    const int b = simple_sequence_of(a, t);
-    if (b < 0) return;
-    const int first = max(a.q_start[b], 0), q_len = a.q_start[b + 1] - first;
-    int kv_len = a.kv_len[b];
-    if (kv_len > a.max_kv_len || q_len > a.max_q_len) {
-        if (lane == 0 && a.error) atomicOr(a.error, GFD_KV_ERR_LENGTH);
-        kv_len = min(kv_len, a.max_kv_len);
+template <typename T, int D>
+int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
+    const dim3 grid((unsigned)(p.own.blocks * a.kv_heads), (unsigned)ceil_div(p.rows, kJoinRows));
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kJoinBlock), 0, st, a, c, p.prefix, p.own); };
+    if (p.rows == 16) go(join_kernel<T, D, 16>);
+    if (p.rows == 32) go(join_kernel<T, D, 32>);
+    if (p.rows == 128) go(join_kernel<T, D, 128>);
+    if (p.rows == 256) go(join_kernel<T, D, 256>);
+    return (int)hipGetLastError();
+}
+
+template <typename T, typename S>
+int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st) {
+    const Stage none{0, 0, 0, 0, 1, 0, 0};
+    int rc;
+    if (p.own_waves) {  // both stages have blocks of the same rows
+        rc = launch_tiles<T, S>(a, c, p.prefix, p.own, dim, p.own_waves, st);
+    } else if (p.prefix_waves) {
+        rc = launch_tiles<T, S>(a, c, p.prefix, none, dim, p.prefix_waves, st);
+        if (!rc) rc = launch_rows<T, S>(a, c, none, p.own, dim, p.rows == 32, st);
+    } else {
+        rc = launch_rows<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
     }
-    if (t - first >= a.max_q_len) return;
-    const Seen s = visible(a, t, t - first, q_len, kv_len);
-    const int kv_head = h / a.group.d;
-    __shared__ float q[D];
-    for (int d = lane; d < D; d += 64) q[d] = load_one<T>((const uint8_t*)(a.q + t * a.q_stride + (int64_t)h * D), d);
-    __syncthreads();
-    float m = -INFINITY, sum = 0.f, o[D / 64] = {};
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    for (int j0 = s.lo; j0 < s.hi; j0 += 64) {
-        const int j = j0 + lane;
-        float x = -INFINITY;
-        int64_t at = -1;
-        if (j < s.hi) {
-            const bool shared = j < a.prefix_len;
-            const uint32_t n = (uint32_t)(shared ? j : j - a.prefix_len), page = c.page.div(n);
-            const int id = shared ? a.prefix_table[page] : a.table[b * a.table_stride + page];
-            if (id < 0 || id >= c.num_pages) {
-                if (a.error) atomicOr(a.error, GFD_KV_ERR_PAGE);
-            } else {
-                at = id * c.page_stride + (int64_t)(n - page * c.page.d) * c.slot_stride + kv_head * c.head_stride;
-                float dot = 0.f;
-                for (int d = 0; d < D; d++) dot += q[d] * load_one<S>(c.k + at, d);
-                x = dot * (a.scale * c.k_scale);
-                if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-                if (a.slopes) x -= slope * fabsf((float)(s.pos - j));
-            }
-        }
-        float top = x;
-        for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-        // fmaxf leaves NaN out; a NaN score reaches the sum through its own exp.
-        const float next = fmaxf(m, top), base = next == -INFINITY ? 0.f : next;
-        const float p = at >= 0 ? expf(x - base) : 0.f, keep = expf(m - base);
-        float part = p;
-        for (int off = 32; off; off >>= 1) part += __shfl_xor(part, off);
-        sum = sum * keep + part;
-        m = next;
-        for (int k = 0; k < D / 64; k++) o[k] *= keep;
-        for (int n = 0; n < 64; n++) {
-            const int64_t from = __shfl(at, n);
-            const float w = __shfl(p, n);
-            if (from < 0) continue;
-            for (int k = 0; k < D / 64; k++) o[k] += w * load_one<S>(c.v + from, lane + 64 * k);
-        }
-    }
-    uint16_t* out = a.out + t * a.out_stride + (int64_t)h * D;
-    for (int k = 0; k < D / 64; k++)
-        out[lane + 64 * k] = (uint16_t)T::pack(sum == 0.f ? 0.f : o[k] * (c.v_scale / sum), 0.f);
-    if (a.lse && lane == 0) a.lse[(int64_t)t * a.q_heads + h] = sum == 0.f ? -INFINITY : m + logf(sum);
+    if (rc || p.slots == 1) return rc;
+    return dim == 64 ? launch_join<T, 64>(a, c, p, st) : dim == 128 ? launch_join<T, 128>(a, c, p, st)
+                                                                   : launch_join<T, 256>(a, c, p, st);
 }
 
 int refuse(const char* name, const char* why) {
@@ -214,80 +216,8 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
         return "rows' pointers or strides are not multiples of 16 bytes";
     const int64_t pages = ((int64_t)std::max(w.max_kv_len - prefix_len, 0) + cache->page_size - 1) / cache->page_size;
     if (w.table_stride < pages) return "block_table's rows are shorter than max_kv_len needs";
+    if (make_plan(*cache, w, prefix_len).items > (1 << 28)) return "more work than one launch takes";
     return nullptr;
-}
-
-// How a call is cut into row blocks and key ranges.
-struct Plan {
-    bool simple;      // more rows than 32 share keys: the kernel of one wave per row
-    int rows;         // of an own-keys block
-    Stage prefix, own;
-    int slots;        // partial results per row
-    int64_t bytes;    // of workspace
-};
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// Workgroups that fill the card: below kFill a block's keys are split, into ranges of
-// at least kMinChunk keys (a tile per wave).  Ranges also end at kRowsMaxChunk, so that
-// sequences of very different lengths are evenly spread.
-constexpr int kFill = 2048, kMinChunk = 128;
-
-void split(Stage* st, int64_t items, int64_t keys) {
-    const int64_t want = ceil_div(keys * items, kFill);
-    st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max<int64_t>(kMinChunk, ceil_div(want, kMinChunk) * kMinChunk));
-    st->splits = (int)std::max<int64_t>(1, ceil_div(keys, st->chunk));
-}
-
-Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
-    Plan p{};
-    const int64_t group = w.num_q_heads / cache.num_heads, heads = cache.num_heads;
-    const int64_t seq_rows = std::min<int64_t>(w.max_q_len, w.num_tokens) * group;
-    const int64_t all_rows = w.num_tokens * group;
-    p.simple = seq_rows > 32 || (prefix_len && all_rows > 32);
-    p.rows = seq_rows <= 16 && (!prefix_len || all_rows <= 16) ? 16 : 32;
-    // Keys that a block can see: with a window, those of its tokens' windows (a prefix mask only adds later keys).
-    int64_t keys = std::max(w.max_kv_len - prefix_len, 0);
-    if (w.window && !w.prefix_end) keys = std::min<int64_t>(keys, (int64_t)w.window + w.max_q_len);
-    p.own.blocks = w.batch;
-    p.own.whole = 1;
-    split(&p.own, p.own.blocks * heads, keys);
-    if (prefix_len) {
-        p.prefix.prefix = 1;
-        p.prefix.blocks = (int)ceil_div(all_rows, p.rows);
-        split(&p.prefix, p.prefix.blocks * heads, prefix_len);
-        p.own.first_slot = p.prefix.splits;
-    } else {
-        p.own.direct = 1;
-    }
-    p.slots = p.own.first_slot + p.own.splits;
-    if (p.slots > 1 && !p.simple) p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4;
-    return p;
-}
-
-template <typename T, int D>
-int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.own.blocks * a.kv_heads), (unsigned)ceil_div(p.rows, kJoinRows));
-    if (p.rows == 16)
-        hipLaunchKernelGGL((join_kernel<T, D, 16>), grid, dim3(kJoinBlock), 0, st, a, c, p.prefix, p.own);
-    else
-        hipLaunchKernelGGL((join_kernel<T, D, 32>), grid, dim3(kJoinBlock), 0, st, a, c, p.prefix, p.own);
-    return (int)hipGetLastError();
-}
-
-template <typename T, typename S>
-int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st) {
-    const dim3 grid((unsigned)a.num_tokens, (unsigned)a.q_heads);
-    if (p.simple) {
-    if (dim == 64) hipLaunchKernelGGL((attend_kernel<T, S, 64>), grid, dim3(64), 0, st, a, c);
-    if (dim == 128) hipLaunchKernelGGL((attend_kernel<T, S, 128>), grid, dim3(64), 0, st, a, c);
-    if (dim == 256) hipLaunchKernelGGL((attend_kernel<T, S, 256>), grid, dim3(64), 0, st, a, c);
-    return (int)hipGetLastError();
-    }
-    if (const int rc = launch_rows<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st)) return rc;
-    if (p.slots == 1) return 0;
-    return dim == 64 ? launch_join<T, 64>(a, c, p, st) : dim == 128 ? launch_join<T, 128>(a, c, p, st)
-                                                                   : launch_join<T, 256>(a, c, p, st);
 }
 
 int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* call, const int* prefix_table,
