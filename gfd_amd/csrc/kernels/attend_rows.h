@@ -9,7 +9,7 @@
 // scores.  A long axis is split over workgroups.
 //
 // A tile: scores^T[32 keys][16 rows] by 16x16x32 products, keys as the left operand
-// (lane: key l % 16, 8 dims of a 32, by l / 16).  Result: lane holds row l % 16 and the keys
+// (lane: key l % 16, 8 dims of a 32, by l / 16), for which they pass through the wave's own LDS.  Result: lane holds row l % 16 and the keys
 // 4 (l / 16) + r of both halves.  As the right operand of out^T += V^T P the
 // lane has to hold 8 keys of a 32, and which 8 is free as long as the values agree: so it
 // keeps its own, and loads the values of those 8 keys, D / 16 adjacent
@@ -20,7 +20,7 @@
 namespace gfd {
 namespace kv {
 
-constexpr int kRowsBlock = 256, kRowsTile = 32, kRowsMaxChunk = 1024;
+constexpr int kRowsBlock = 256, kRowsTile = 32;
 
 template <int N>
 struct Words {
@@ -31,15 +31,15 @@ template <int N>  // words
 __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
     Words<N> r;
     if constexpr (N == 1) {
-        r.w[0] = *(const uint32_t*)p;
+        r.w[0] = __builtin_nontemporal_load((const uint32_t*)p);
     } else if constexpr (N == 2) {
-        const u32x2 x = *(const u32x2*)p;
+        const u32x2 x = __builtin_nontemporal_load((const u32x2*)p);
         r.w[0] = x[0];
         r.w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const u32x4 x = *(const u32x4*)(p + 4 * i);
+            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + 4 * i));
 #pragma unroll
             for (int j = 0; j < 4; j++) r.w[i + j] = x[j];
         }
@@ -52,33 +52,43 @@ struct RowsKernel {
     static constexpr int kSize = S::kBytes;
     static constexpr int kDims = D / 16;                   // a lane's dims of a value row
     static constexpr int kSteps = D / 32;                  // products per 16 keys
-    static constexpr int kKeyWords = D / 4 * kSize / 4;    // a lane's words of a key: a quarter of its dims
+    static constexpr int kKeyChunks = D * kSize / 16;      // of 16 bytes a key
+    static constexpr int kKeyLoads = kRowsTile * kKeyChunks / 64;
     static constexpr int kValWords = kDims * kSize / 4;
     static constexpr int kAcc = kDims * 4;                 // a lane's outputs per 16 rows
     // 32 rows of 128 dims and more: with the rows' operand in registers too, a lane would need more than it has.
-    static constexpr bool kLdsRows = R == 2 && D >= 128;
+    static constexpr bool kLdsRows = (R == 2 && D >= 128) || D == 256;
 
     struct Tile {
-        Words<kKeyWords> k[2];
+        u32x4 k[kKeyLoads];
         Words<kValWords> v[8];
     };
 
-    // Dims of product step s and quarter g start here: 16-byte loads of 64 contiguous bytes per key.
+    // Dims of product step s and quarter g start here: a chunk of 16 bytes is one step's, or two steps'.
     static __device__ __forceinline__ int step_dim(int s, int g) {
         return kSize == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
     }
+    // Where a key's chunk lies in the wave's LDS: neighbours are spread over the banks.
+    static __device__ __forceinline__ int key_at(int key, int chunk) {
+        constexpr int kPerTurn = kKeyChunks >= 16 ? 1 : 16 / kKeyChunks;  // keys that span the banks
+        return key * kKeyChunks + (chunk ^ ((key / kPerTurn) & (kKeyChunks >= 8 ? 7 : kKeyChunks - 1)));
+    }
 
+    // A load takes whole keys, as many as 1024 bytes hold: the cache's bytes are not used again, and
+    // whole rows at a time come faster than the operand's own 64-byte pieces of 16 keys.
     static __device__ __forceinline__ void load_keys(Tile& t, const Cache& c, const int64_t* off, int lane) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int64_t o = off[16 * h + (lane & 15)];
-            const uint8_t* p = c.k + (o < 0 ? 0 : o) + 16 * (lane >> 4);
+        for (int i = 0; i < kKeyLoads; i++) {
+            const int n = i * 64 + lane;
+            const int64_t o = off[n / kKeyChunks];
+            t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + (o < 0 ? 0 : o) + n % kKeyChunks * 16));
+        }
+    }
+    static __device__ __forceinline__ void store_keys(const Tile& t, u32x4* lds, int lane) {
 #pragma unroll
-            for (int i = 0; i < kKeyWords; i += 4) {
-                const u32x4 x = *(const u32x4*)(p + 16 * i);  // 64 bytes of the row by the four quarters
-#pragma unroll
-                for (int j = 0; j < 4; j++) t.k[h].w[i + j] = x[j];
-            }
+        for (int i = 0; i < kKeyLoads; i++) {
+            const int n = i * 64 + lane;
+            lds[key_at(n / kKeyChunks, n % kKeyChunks)] = t.k[i];
         }
     }
     static __device__ __forceinline__ int load_values(Tile& t, const Cache& c, const int64_t* off, int lane) {
@@ -92,13 +102,18 @@ struct RowsKernel {
         return valid;
     }
 
-    // Keys' operand of step s.
-    static __device__ __forceinline__ u32x4 key_frag(const Words<kKeyWords>& k, int s) {
+    // Keys' operands of step s (two steps for 8-bit keys) for 16 keys from first on.
+    static constexpr int kStepsPerChunk = kSize == 2 ? 1 : 2;
+    static __device__ __forceinline__ void key_frags(const u32x4* lds, int first, int s, int lane,
+                                                     u32x4 (&f)[kStepsPerChunk]) {
+        const u32x4 x = lds[key_at(first + (lane & 15), s / kStepsPerChunk * 4 + (lane >> 4))];
         if constexpr (kSize == 2) {
-            return u32x4{k.w[4 * s], k.w[4 * s + 1], k.w[4 * s + 2], k.w[4 * s + 3]};
+            f[0] = x;
         } else {
-            const uint32_t a = k.w[2 * s], b = k.w[2 * s + 1];
-            return u32x4{Mma<T>::widen_lo(a), Mma<T>::widen_hi(a), Mma<T>::widen_lo(b), Mma<T>::widen_hi(b)};
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                f[i] = u32x4{Mma<T>::widen_lo(x[2 * i]), Mma<T>::widen_hi(x[2 * i]), Mma<T>::widen_lo(x[2 * i + 1]),
+                             Mma<T>::widen_hi(x[2 * i + 1])};
         }
     }
     // Word i of a value row in 16-bit pairs.
@@ -106,13 +121,19 @@ struct RowsKernel {
         if constexpr (kSize == 2) return v.w[i];
         else return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
     }
+    // A word as it lies in the cache, infinities and NaN made zero.
+    static __device__ __forceinline__ uint32_t only_finite_word(uint32_t w) {
+        if constexpr (kSize == 2) return only_finite<T>(w);
+        const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // e4m3: all ones but the sign
+        return w & ~((nan >> 7) * 0xFFu);
+    }
     static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b, int odd) {
         return __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
     }
 };
 
 template <typename T, typename S, int D, int R>
-__global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kernel(Call a, Cache c,
+__global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(Call a, Cache c,
                                                                                     Stage prefix, Stage own) {
     using K = RowsKernel<T, S, D, R>;
     constexpr int kRows = 16 * R, kWaves = kRowsBlock / 64;
@@ -121,6 +142,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
     __shared__ union {
         int samples[kSamples + 1];
         float merge[kWaves / 2][R * K::kAcc + 2 * R][64];
+        u32x4 keys[kWaves][kRowsTile * K::kKeyChunks];
     } lds;
     __shared__ int any_bad;
     __shared__ u32x4 lds_rows[K::kLdsRows ? R * K::kSteps : 1][64];
@@ -132,8 +154,11 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
     if (item >= prefix_items) item -= prefix_items;
     const int kv_head = item % a.kv_heads, block = item / a.kv_heads % st.blocks,
               split = item / a.kv_heads / st.blocks;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, quarter = lane >> 4;
+    const int tid = (int)threadIdx.x, lane = tid & 63, col = lane & 15, quarter = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+    // Most ranges of short sequences: nothing, and no need to look further.
+    if (!st.prefix && split > 0 && (int64_t)split * st.chunk >= min(a.kv_len[block], a.max_kv_len) - a.prefix_len) return;
     Block k;
     if (!find_rows<kRows>(a, st, block, &k)) return;
     if (st.prefix) {
@@ -202,7 +227,9 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
         for (int d = 0; d < K::kDims; d++) o[i][d] = f32x4{0, 0, 0, 0};
     }
     typename K::Tile t;
+    u32x4* const my_keys = lds.keys[wave];
     int valid = 0;
+    bool any_odd = false;
     if (wave < tiles) {
         K::load_keys(t, c, offsets + wave * kRowsTile, lane);
         valid = K::load_values(t, c, offsets + wave * kRowsTile, lane);
@@ -212,25 +239,33 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
         const bool more = tile + kWaves < tiles;
         const int64_t* next = offsets + (tile + kWaves) * kRowsTile;
         if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
+        K::store_keys(t, my_keys, lane);
+        // Other lanes of the wave read them: its LDS accesses are in order, the compiler has to keep them so.
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (more) K::load_keys(t, c, next, lane);
         f32x4 x[R][2];
 #pragma unroll
         for (int i = 0; i < R; i++) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < K::kSteps; s++) {
-            const u32x4 k0 = K::key_frag(t.k[0], s), k1 = K::key_frag(t.k[1], s);
+        for (int s = 0; s < K::kSteps; s += K::kStepsPerChunk) {
+            u32x4 k0[K::kStepsPerChunk], k1[K::kStepsPerChunk];
+            K::key_frags(my_keys, 0, s, lane, k0);
+            K::key_frags(my_keys, 16, s, lane, k1);
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                u32x4 qf;
-                if constexpr (K::kLdsRows) qf = lds_rows[i * K::kSteps + s][lane];
-                else qf = q[i][s];
-                x[i][0] = Mma<T>::m16(k0, qf, x[i][0]);
-                x[i][1] = Mma<T>::m16(k1, qf, x[i][1]);
-            }
+            for (int j = 0; j < K::kStepsPerChunk; j++)
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    u32x4 qf;
+                    if constexpr (K::kLdsRows) qf = lds_rows[i * K::kSteps + s + j][lane];
+                    else qf = q[i][s + j];
+                    x[i][0] = Mma<T>::m16(k0[j], qf, x[i][0]);
+                    x[i][1] = Mma<T>::m16(k1[j], qf, x[i][1]);
+                }
         }
-        if (more) K::load_keys(t, c, next, lane);
         const bool whole = !bad && g.all_lo <= n0 && n0 + kRowsTile <= min(g.all_hi, c1);
         u32x4 p[R];
-        uint32_t seen[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
             if (extras) {
@@ -239,14 +274,11 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
                     x[i][j >> 2][j & 3] = score<true>(sc[i], a, x[i][j >> 2][j & 3], row[i].pos,
                                                       n0 + 16 * (j >> 2) + 4 * quarter + (j & 3));
             }
-            seen[i] = 0xFF;
             if (!whole) {
-                seen[i] = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int n = n0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
                     const bool on = n >= row[i].lo && n < row[i].hi && ((valid >> j) & 1);
-                    seen[i] |= (uint32_t)on << j;
                     if (!on) x[i][j >> 2][j & 3] = -INFINITY;
                 }
             }
@@ -256,7 +288,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
             top = across16_max(top);
             if (__any(!(top <= m[i]))) {
                 const float next_m = max_f32(m[i], top);
-                const float keep = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - next_m) * factor);
+                const float keep = m[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[i] - next_m) * factor);
                 m[i] = next_m;
                 sum[i] *= keep;
 #pragma unroll
@@ -273,20 +305,10 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
 #pragma unroll
             for (int j = 0; j < 4; j++) p[i][j] = T::pack(e[2 * j], e[2 * j + 1]);
         }
-        if (whole) {
-#pragma unroll
-            for (int d = 0; d < K::kDims; d++) {
-                u32x4 vf;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
-#pragma unroll
-                for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
-            }
-        } else {
-            // Values of keys outside the range count as zeros, and of keys that some rows
-            // see and others do not, infinities and NaN reach only the rows that do: a weight
-            // of zero would not stop them.
+        if (!whole) {
+            // Values of keys outside the range count as zeros.  Of keys that some rows see and
+            // others do not, infinities and NaN reach only the rows that do: a weight of zero
+            // would not stop them.  They are zeros in the product and are added below.
             uint32_t odd = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -295,38 +317,51 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
 #pragma unroll
                 for (int i = 0; i < K::kDims / 2; i++) odd |= not_finite<T>(K::value_pair(t.v[j], i));
             }
-            const bool any_odd = __any(odd != 0);
+            if (__any(odd != 0)) {
+                any_odd = true;
 #pragma unroll
-            for (int d = 0; d < K::kDims; d++) {
-                u32x4 vf;
+                for (int j = 0; j < 8; j++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
-                if (any_odd) {
-#pragma unroll 1
-                    for (int kind = 0; kind < 3; kind++) {
-                        u32x4 is;
-                        for (int j = 0; j < 4; j++) is[j] = of_kind<T>(vf[j], kind);
-                        for (int i = 0; i < R; i++) {
-                            u32x4 on;
-                            for (int j = 0; j < 4; j++)
-                                on[j] = ((seen[i] >> (2 * j)) & 1 ? Mma<T>::kOne : 0u) |
-                                        ((seen[i] >> (2 * j + 1)) & 1 ? Mma<T>::kOne << 16 : 0u);
-                            const f32x4 count = Mma<T>::m16(is, on, f32x4{0, 0, 0, 0});
-                            for (int r = 0; r < 4; r++)
-                                if (count[r] > 0.f) o[i][d][r] += kind_value(kind);
-                        }
-                    }
-                    for (int j = 0; j < 4; j++) vf[j] = only_finite<T>(vf[j]);
-                }
-#pragma unroll
-                for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
+                    for (int i = 0; i < K::kValWords; i++) t.v[j].w[i] = K::only_finite_word(t.v[j].w[i]);
             }
+        }
+#pragma unroll
+        for (int d = 0; d < K::kDims; d++) {
+            u32x4 vf;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
+#pragma unroll
+            for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
         }
         if (more) valid = K::load_values(t, c, next, lane);
     }
 
-    // The waves' results joined pairwise, in the lanes' own layout.
+    // The infinities and NaN that were left out, key by key.  Where the product had some in, they add nothing new.
+    if (any_odd) {
+#pragma unroll 1
+        for (int tile = wave; tile < tiles; tile += kWaves)
+#pragma unroll 1
+            for (int n = tile * kRowsTile; n < (tile + 1) * kRowsTile; n++) {
+                const int64_t at = offsets[n];
+                const uint8_t* from = c.v + (at < 0 ? 0 : at) + 4 * quarter * K::kDims * K::kSize;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const auto v = load_words<K::kValWords>(from + r * K::kDims * K::kSize);
+#pragma unroll
+                    for (int d = 0; d < K::kDims; d++) {
+                        const uint32_t pair = K::value_pair(v, d / 2);
+                        const float x = T::unpack(pair & ~only_finite<T>(pair))[d & 1];
+#pragma unroll
+                        for (int i = 0; i < R; i++)
+                            o[i][d][r] += at >= 0 && c0 + n >= row[i].lo && c0 + n < row[i].hi ? x : 0.f;
+                    }
+                }
+            }
+    }
+
+    // The waves' results joined pairwise, in the lanes' own layout, where the keys were.
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; i++) sum[i] = across16_sum(sum[i]);
     for (int half = kWaves / 2; half; half /= 2) {
@@ -346,7 +381,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_rows_kern
 #pragma unroll
             for (int i = 0; i < R; i++) {
                 const float m2 = from[2 * i][lane], top = max_f32(m[i], m2);
-                const float keep = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - top) * factor);
+                const float keep = m[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[i] - top) * factor);
                 const float take = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - top) * factor);
                 m[i] = top;
                 sum[i] = sum[i] * keep + from[2 * i + 1][lane] * take;

@@ -283,7 +283,6 @@ struct Mma;
 template <>
 struct Mma<Bf16> {
     static constexpr uint32_t kNear = 0x00800080u;  // added to a magnitude: bit 15 is set from infinity on
-    static constexpr uint32_t kOne = 0x3F80u;
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -303,7 +302,6 @@ struct Mma<Bf16> {
 template <>
 struct Mma<Fp16> {
     static constexpr uint32_t kNear = 0x04000400u;
-    static constexpr uint32_t kOne = 0x3C00u;
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
@@ -325,29 +323,19 @@ template <typename T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & 0x7FFF7FFFu) + Mma<T>::kNear) & 0x80008000u;
 }
-// A pair with infinities and NaN made zero; and the pair of ones where the value is of a kind (0 NaN, 1 +inf, 2 -inf).
+// A pair with infinities and NaN made zero.
 template <typename T>
 __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
     const uint32_t bad = not_finite<T>(w) >> 15;
     return w & ~(bad * 0xFFFFu);
 }
-template <typename T>
-__device__ __forceinline__ uint32_t of_kind(uint32_t w, int kind) {
-    uint32_t r = 0;
-    for (int h = 0; h < 2; h++) {
-        const uint32_t x = (w >> (16 * h)) & 0xFFFFu, inf = 0x8000u - (Mma<T>::kNear & 0xFFFFu);
-        const bool hit = kind == 0 ? (x & 0x7FFFu) > inf : x == (inf | (kind == 2 ? 0x8000u : 0u));
-        r |= (hit ? Mma<T>::kOne : 0u) << (16 * h);
-    }
-    return r;
-}
-__device__ __forceinline__ float kind_value(int kind) {
-    return kind == 0 ? __builtin_nanf("") : kind == 1 ? __builtin_inff() : -__builtin_inff();
-}
 
+// Few rows (attend_rows.h): a range has at most so many keys.
+constexpr int kRowsMaxChunk = 1024;
 template <typename T, typename S>
 int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
                 hipStream_t st);
+// Many rows (attend_tiles.h).
 template <typename T, typename S>
 int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
                  hipStream_t st);

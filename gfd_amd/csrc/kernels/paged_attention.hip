@@ -11,8 +11,6 @@
 #include <cstdint>
 #include <cstdio>
 
-#include "attend_rows.h"
-#include "attend_tiles.h"
 #include "capi_error.h"
 #include "gfd_capi.h"
 #include "paged_attention.h"
@@ -21,7 +19,7 @@ namespace gfd {
 namespace kv {
 namespace {
 
-constexpr int kJoinBlock = 256, kJoinRows = 16;
+constexpr int kJoinBlock = 256, kJoinRows = kJoinBlock / 64;
 
 // A workgroup joins kJoinRows rows of an own-keys block, a wave per row: a lane
 // weighs one range of 64, then holds D / 64 dims.  Reads what the ranges
@@ -46,9 +44,11 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
     const int splits = max(1, (g.hi - g.lo + own.chunk - 1) / own.chunk), slots = own.first_slot + splits;
     if (own.direct && splits == 1) return;
 
-    const int first = (int)blockIdx.y * kJoinRows;
-    for (int r = first + wave; r < min(first + kJoinRows, k.rows); r += kWaves) {
-        const int t = row_of(a, own, k, nullptr, r).t, h = head_of(a, k, r, kv_head);
+    const int r = (int)blockIdx.y * kJoinRows + wave;
+    if (r >= k.rows) return;
+    {
+        const int t = min(max(a.q_start[k.b], 0), a.num_tokens) + (int)a.group.div((uint32_t)(k.first_row + r));
+        const int h = head_of(a, k, r, kv_head);
         float top = -INFINITY;
         for (int s0 = 0; s0 < slots; s0 += 64) {
             if (s0 + lane < slots) top = max_f32(top, a.part_ml[slot_of(a, s0 + lane, t, h)][0]);
@@ -68,17 +68,17 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
             const float* from = a.part_o + slot_of(a, s0, t, h) * D + lane * kDims;
             const int64_t step = (int64_t)a.num_tokens * a.q_heads * D;
             const int n = min(64, slots - s0);
-            for (int s = 0; s < n; s += 4) {  // lanes past the last range weigh nothing
-                Dims x[4];
-                float ws[4];
+            for (int s = 0; s < n; s += 8) {  // lanes past the last range weigh nothing
+                Dims x[8];
+                float ws[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < 8; j++) {
                     ws[j] = __shfl(w, s + j);
                     x[j] = 0.f;
                     if (__shfl(l, s + j) != 0.f) x[j] = *(const Dims*)(from + (s + j) * step);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) o += ws[j] * x[j];
+                for (int j = 0; j < 8; j++) o += ws[j] * x[j];
             }
         }
         total = across16_sum(total);
@@ -108,17 +108,19 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Few rows: below kFill workgroups a block's keys are split, into ranges of at least a
-// tile per wave.  Ranges also end at kRowsMaxChunk, so that sequences of very different
-// lengths are evenly spread.
-constexpr int kFill = 2048, kMinChunk = 128;
+// Few rows: two workgroups of a range each fit a CU, kRound the card.  Sequences of very different
+// lengths spread best over kRounds rounds of them (64 of up to 8192 keys: ranges of 1024 163 us, of 512 173),
+// but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
+// below one round the shortest range, a tile per wave, counts.
+constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
 // Many rows: a workgroup fills a CU (or half of it), so two rounds of them do.
 constexpr int kTilesFill = 512, kTilesMinChunk = 256;
 
 void split(Stage* st, int64_t items, int64_t keys, bool few) {
     if (few) {
-        const int64_t want = ceil_div(ceil_div(keys * items, kFill), kMinChunk) * kMinChunk;
-        st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max<int64_t>(kMinChunk, want));
+        const auto chunk_for = [&](int64_t groups) { return ceil_div(ceil_div(keys * items, groups), kMinChunk) * kMinChunk; };
+        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(kRound)));
+        st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max(least, chunk_for(kRound * kRounds)));
     } else {
         const int64_t parts = std::max<int64_t>(1, kTilesFill / std::max<int64_t>(items, 1));
         st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
