@@ -57,71 +57,178 @@ struct Rows {
     int* error;
 };
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256, kTokens = 4;
 
-template <typename T>
-__device__ __forceinline__ float load_one(const uint16_t* p) {
-    return T::unpack(*p)[0];
-}
-
-// Two values to the stored type, in the low bits of the result.
+// Eight values to the stored type.
 template <typename T>
 struct Store {
+    static __device__ __forceinline__ void eight(uint8_t* p, const float (&x)[8], float) {
+        *(u32x4*)p = u32x4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7])};
+    }
     static constexpr int kBytes = 2;
-    static __device__ __forceinline__ void one(uint8_t* p, float x) { *(uint16_t*)p = (uint16_t)T::pack(x, 0.f); }
 };
 template <>
 struct Store<E4m3> {
     static constexpr int kBytes = 1;
-    static __device__ __forceinline__ void one(uint8_t* p, float x) {
-        const float y = x != x ? x : fminf(fmaxf(x, -448.f), 448.f);
-        *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, 0.f, 0, false);
+    static __device__ __forceinline__ float cut(float x) {
+        return x != x ? x : __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
+    }
+    static __device__ __forceinline__ void eight(uint8_t* p, const float (&x)[8], float div) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            int y = __builtin_amdgcn_cvt_pk_fp8_f32(cut(x[4 * i] / div), cut(x[4 * i + 1] / div), 0, false);
+            w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cut(x[4 * i + 2] / div), cut(x[4 * i + 3] / div), y, true);
+        }
+        *(u32x2*)p = u32x2{w[0], w[1]};
     }
 };
 
-// One workgroup per token; a thread per element of its heads' halves.
-template <typename T, typename S, bool kPairs>
+template <typename T>
+__device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const f32x2 y = T::unpack(w[i]);
+        x[2 * i] = y[0];
+        x[2 * i + 1] = y[1];
+    }
+}
+
+// How the rotated pairs lie: side by side, a half apart in whole chunks of 8, or a half apart.
+enum { kSide, kChunksApart, kApart };
+
+// A workgroup takes kTokensHere tokens: their turns go to LDS, then each thread takes 16 values of a
+// head at a time, two chunks of 16 bytes.  A pair's two chunks are taken together; where
+// a half is no whole number of chunks, a head's lanes (of one wave) pass their chunks through LDS instead.
+// The first values are under way while the turns are computed.  Bound by the rows' and
+// the cache's bytes.
+template <typename T, typename S, int kPairs, int kTokensHere>
 __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
-    __shared__ f32x2 turn[128];
-    const int t = (int)blockIdx.x, half = r.rotary / 2;
-    for (int i = (int)threadIdx.x; i < half; i += kBlock) {
-        const double turns = (double)r.positions[t] * ((double)r.inv_freq[i] * 0.15915494309189533577);
+    __shared__ f32x2 turns[kTokensHere][128];
+    __shared__ int64_t places[kTokensHere];
+    __shared__ u32x4 chunks[kPairs == kApart ? kBlock * 2 : 1];
+    const int tid = (int)threadIdx.x, t0 = (int)blockIdx.x * kTokensHere, half = r.rotary / 2;
+    const int shift = r.dim == 64 ? 2 : r.dim == 128 ? 3 : 4;  // a head's units of 16 values
+    const int first = (r.q ? 0 : r.q_heads) << shift, per_token = ((r.q_heads + 2 * r.kv_heads) << shift) - first;
+    const int tokens = min(kTokensHere, r.num_tokens - t0), units = tokens * per_token;
+
+    struct Unit {
+        int t, head, kind, a, b;  // kind 0 q, 1 k, 2 v; first values of the chunks
+        u32x4 x, y;
+    };
+    const auto load = [&](int n) {
+        Unit u;
+        u.t = 0;
+        if constexpr (kTokensHere > 1) {
+            while (n >= per_token) n -= per_token, u.t++;
+        }
+        n += first;
+        const int h = n >> shift, i = n & ((1 << shift) - 1);
+        u.kind = h < r.q_heads ? 0 : h < r.q_heads + r.kv_heads ? 1 : 2;
+        u.head = u.kind == 0 ? h : u.kind == 1 ? h - r.q_heads : h - r.q_heads - r.kv_heads;
+        u.a = 16 * i;
+        u.b = u.a + 8;
+        if (kPairs == kChunksApart && u.kind != 2 && 8 * i < half) {
+            u.a = 8 * i;
+            u.b = u.a + half;
+        }
+        const int64_t t = t0 + u.t;
+        const uint16_t* p = (u.kind == 0   ? r.q + t * r.q_stride
+                             : u.kind == 1 ? r.k + t * r.k_stride
+                                           : r.v + t * r.v_stride) + (int64_t)u.head * r.dim;
+        u.x = *(const u32x4*)(p + u.a);
+        u.y = *(const u32x4*)(p + u.b);
+        return u;
+    };
+    Unit u;
+    if (tid < units) u = load(tid);
+
+    for (int n = tid; n < tokens * half; n += kBlock) {
+        const int t = n / half, i = n - t * half;
+        const double whole = (double)r.positions[t0 + t] * ((double)r.inv_freq[i] * 0.15915494309189533577);
         float s, co;
-        sincospif((float)(2.0 * (turns - rint(turns))), &s, &co);
-        turn[i] = f32x2{co, s};
+        sincospif((float)(2.0 * (whole - rint(whole))), &s, &co);
+        turns[t][i] = f32x2{co, s};
+    }
+    if (tid < tokens) {
+        const int64_t slot = r.slots[t0 + tid];
+        int64_t at = -1;
+        if (slot >= 0) {
+            if (slot < (int64_t)c.num_pages * c.page.d) {
+                const int64_t page = slot / c.page.d;
+                at = page * c.page_stride + (slot - page * c.page.d) * c.slot_stride;
+            } else if (r.error) {
+                atomicOr(r.error, GFD_KV_ERR_PAGE);
+            }
+        }
+        places[tid] = at;
     }
     __syncthreads();
-    const int64_t slot = r.slots[t];
-    const bool inside = slot < (int64_t)c.num_pages * c.page.d;
-    if (!inside && threadIdx.x == 0 && r.error) atomicOr(r.error, GFD_KV_ERR_PAGE);
-    const int64_t page = slot / c.page.d, at = page * c.page_stride + (slot - page * c.page.d) * c.slot_stride;
-    const int units = r.dim / 2;
-    const int first = r.q ? 0 : r.q_heads;
-    for (int u = first * units + (int)threadIdx.x; u < (r.q_heads + 2 * r.kv_heads) * units; u += kBlock) {
-        const int h = u / units, i = u - h * units;
-        const bool is_q = h < r.q_heads, is_v = h >= r.q_heads + r.kv_heads;
-        const int head = is_q ? h : is_v ? h - r.q_heads - r.kv_heads : h - r.q_heads;
-        const bool turned = i < half;
-        // Past the rotated dims the pairs are neighbours.
-        const int ia = turned && !kPairs ? i : 2 * i, ib = turned && !kPairs ? i + half : 2 * i + 1;
-        const uint16_t* src = is_q ? r.q + t * r.q_stride : is_v ? r.v + t * r.v_stride : r.k + t * r.k_stride;
-        const int va = is_v ? 2 * i : ia, vb = is_v ? 2 * i + 1 : ib;
-        float a = load_one<T>(src + (int64_t)head * r.dim + va), b = load_one<T>(src + (int64_t)head * r.dim + vb);
-        if (turned && !is_v) {
-            const f32x2 w = turn[i];
-            const float x = a * w[0] - b * w[1], y = b * w[0] + a * w[1];
-            a = x;
-            b = y;
+
+    for (int n = tid; n < units;) {
+        float x[8], y[8];
+        unpack8<T>(u.x, x);
+        unpack8<T>(u.y, y);
+        const f32x2* turn = turns[u.t];
+        if (kPairs == kSide) {
+            if (u.kind != 2 && u.a < 2 * half) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float& p = i < 8 ? x[i] : y[i - 8];
+                    float& q = i < 8 ? x[i + 1] : y[i - 7];
+                    const int at = (u.a + i) / 2;
+                    if (at >= half) continue;
+                    const f32x2 w = turn[at];
+                    const float p0 = p;
+                    p = p0 * w[0] - q * w[1];
+                    q = q * w[0] + p0 * w[1];
+                }
+            }
+        } else if (kPairs == kChunksApart) {
+            if (u.kind != 2 && u.a < half) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const f32x2 w = turn[u.a + i];
+                    const float p0 = x[i], q0 = y[i];
+                    x[i] = p0 * w[0] - q0 * w[1];
+                    y[i] = q0 * w[0] + p0 * w[1];
+                }
+            }
+        } else {
+            const uint16_t* row = (const uint16_t*)(chunks + (tid >> shift << shift) * 2);
+            chunks[2 * tid] = u.x;
+            chunks[2 * tid + 1] = u.y;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            if (u.kind != 2) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float& p = i < 8 ? x[i] : y[i - 8];
+                    const int at = u.a + i;
+                    if (at >= 2 * half) continue;
+                    const f32x2 w = turn[at < half ? at : at - half];
+                    const float q = T::unpack(row[at < half ? at + half : at - half])[0];
+                    p = at < half ? p * w[0] - q * w[1] : p * w[0] + q * w[1];
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
-        if (is_q) {
-            uint16_t* d = r.q_out + t * r.q_out_stride + (int64_t)head * r.dim;
-            Store<T>::one((uint8_t*)(d + va), a);
-            Store<T>::one((uint8_t*)(d + vb), b);
-        } else if (slot >= 0 && inside) {
-            uint8_t* d = (is_v ? c.v : c.k) + at + head * c.head_stride;
-            const float div = is_v ? r.v_div : r.k_div;
-            Store<S>::one(d + va * Store<S>::kBytes, Store<S>::kBytes == 1 ? a / div : a);
-            Store<S>::one(d + vb * Store<S>::kBytes, Store<S>::kBytes == 1 ? b / div : b);
+        const Unit now = u;
+        n += kBlock;
+        // In place, a head's queries are all loaded before any is stored: a thread holds both chunks of its
+        // pairs, and the next units are other heads'.
+        if (n < units) u = load(n);
+        if (now.kind == 0) {
+            uint16_t* d = r.q_out + (t0 + now.t) * r.q_out_stride + (int64_t)now.head * r.dim;
+            Store<T>::eight((uint8_t*)(d + now.a), x, 1.f);
+            Store<T>::eight((uint8_t*)(d + now.b), y, 1.f);
+        } else if (places[now.t] >= 0) {
+            uint8_t* d = (now.kind == 2 ? c.v : c.k) + places[now.t] + now.head * c.head_stride;
+            const float div = now.kind == 2 ? r.v_div : r.k_div;
+            Store<S>::eight(d + now.a * Store<S>::kBytes, x, div);
+            Store<S>::eight(d + now.b * Store<S>::kBytes, y, div);
         }
     }
 }
@@ -133,13 +240,20 @@ int refuse(const char* why) {
     return (int)hipErrorInvalidValue;
 }
 
+template <typename T, typename S, int kTokensHere>
+int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
+    const dim3 grid((unsigned)((r.num_tokens + kTokensHere - 1) / kTokensHere));
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, st, r, c); };
+    if (pairs) go(kv_append_kernel<T, S, kSide, kTokensHere>);
+    else if (r.rotary % 16 == 0) go(kv_append_kernel<T, S, kChunksApart, kTokensHere>);
+    else go(kv_append_kernel<T, S, kApart, kTokensHere>);
+    return (int)hipGetLastError();
+}
+
+// Tokens share a workgroup's start-up where that still fills the card.
 template <typename T, typename S>
 int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
-    if (pairs)
-        hipLaunchKernelGGL((kv_append_kernel<T, S, true>), dim3(r.num_tokens), dim3(kBlock), 0, st, r, c);
-    else
-        hipLaunchKernelGGL((kv_append_kernel<T, S, false>), dim3(r.num_tokens), dim3(kBlock), 0, st, r, c);
-    return (int)hipGetLastError();
+    return r.num_tokens >= 2048 * kTokens ? launch<T, S, kTokens>(r, c, pairs, st) : launch<T, S, 1>(r, c, pairs, st);
 }
 
 }  // namespace
