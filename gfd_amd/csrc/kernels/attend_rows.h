@@ -71,7 +71,7 @@ struct RowsKernel {
     // Where a key's chunk lies in the wave's LDS: neighbours are spread over the banks.
     static __device__ __forceinline__ int key_at(int key, int chunk) {
         constexpr int kPerTurn = kKeyChunks >= 16 ? 1 : 16 / kKeyChunks;  // keys that span the banks
-        return key * kKeyChunks + (chunk ^ ((key / kPerTurn) & (kKeyChunks >= 8 ? 7 : kKeyChunks - 1)));
+        return key * kKeyChunks + (chunk ^ ((key / kPerTurn) & (kKeyChunks >= 16 ? 15 : kKeyChunks - 1)));
     }
 
     // A load takes whole keys, as many as 1024 bytes hold: the cache's bytes are not used again, and

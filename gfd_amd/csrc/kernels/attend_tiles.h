@@ -36,9 +36,10 @@ struct TilesKernel {
         bool on[kUnits];
     };
 
-    // Rows of 256 bytes and more start in the same bank: 8 neighbours are spread by pairs of
-    // chunks.  Of 128: two rows span the banks, pairs of rows are spread.
-    static __device__ __forceinline__ int swap(int row) { return D == 64 ? ((row >> 1) & 3) * 2 : (row & 7) * 2; }
+    // Where a row's chunk lies, so that rows that are read together meet in no bank (64 of 4 bytes).  Keys: one chunk
+    // of 16 rows at once.  Values: two neighbouring chunks of 4 rows.  A row of 128 bytes (D 64) is half the banks.
+    static __device__ __forceinline__ int swap_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+    static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 
     static __device__ __forceinline__ void load(Staged& g, const Cache& c, const int64_t* off, int tid) {
 #pragma unroll
@@ -69,10 +70,10 @@ struct TilesKernel {
         uint32_t odd = 0;
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int n = tid + u * kThreads, row = n / kChunks, chunk = (n % kChunks) ^ swap(row);
+            const int n = tid + u * kThreads, row = n / kChunks, chunk = n % kChunks;
             const u32x4 v = widened(g.v[u], g.on[u]);
-            *(u32x4*)(kb + row * D + chunk * 8) = widened(g.k[u], g.on[u]);
-            *(u32x4*)(vb + row * D + chunk * 8) = v;
+            *(u32x4*)(kb + row * D + (chunk ^ swap_k(row)) * 8) = widened(g.k[u], g.on[u]);
+            *(u32x4*)(vb + row * D + (chunk ^ swap_v(row)) * 8) = v;
             if (look) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) odd |= not_finite<T>(v[i]);
@@ -207,14 +208,17 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     }
     __syncthreads();
 
-    const int swap_k = K::swap(col);
+    const int swap_k = K::swap_k(col);
     const int key_at = col * D;
     const int lane16 = lane & 15, v_row = 4 * hi + (lane16 >> 2);
     int value_at[K::kDims];
 #pragma unroll
     for (int i = 0; i < K::kDims; i++)
-        value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap(v_row)) * 8 + (lane16 & 1) * 4;
+        value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap_v(v_row)) * 8 + (lane16 & 1) * 4;
 
+    // The rows' operand is there before the first tile: left to the loop, its wait would stand in front of every
+    // tile's first product and cover the next tile's loads too.
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     for (int t = 0; t < tiles; t++) {
         const int n0 = c0 + t * kTile;
         const bool more = t + 1 < tiles;
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                 for (int d = 0; d < K::kDims; d++)
 #pragma unroll
                     for (int r = 0; r < 16; r += 4) {
-                        const int chunk = (4 * d + (r >> 2)) ^ K::swap(n);
+                        const int chunk = (4 * d + (r >> 2)) ^ K::swap_v(n);
                         const u32x2 v = *(const u32x2*)(vb + n * D + chunk * 8 + 4 * hi);
                         if (!(not_finite<T>(v[0]) | not_finite<T>(v[1]))) continue;
 #pragma unroll
@@ -262,6 +266,14 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
 #pragma unroll
                 for (int i = 0; i < K::kHalves; i++)
                     x[i] = Mma<T>::m32(*(const u32x4*)(kb + 32 * i * D + (((2 * s + hi) ^ swap_k) * 8)), q[s], x[i]);
+            // Keys are read two products ahead.
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int s = 0; s < K::kSteps * K::kHalves - 4; s++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
             if constexpr (kExtras) {
 #pragma unroll
                 for (int i = 0; i < K::kHalves; i++)
@@ -269,18 +281,25 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                     for (int r = 0; r < 16; r++)
                         x[i][r] = score<true>(sc, a, x[i][r], row.pos, n0 + 32 * i + 8 * (r >> 2) + 4 * hi + (r & 3));
             }
-            const bool all = !bad[t & 3] && whole(w, n0);
-            if (!all) {
-                const int end = min(row.hi, c1);
+            const bool gap = bad[t & 3];
+            if (gap || !whole(w, n0)) {
+                // A lane's keys are these constants and n0 + 4 hi.
+                const int from = row.lo - n0 - 4 * hi, to = min(row.hi, c1) - n0 - 4 * hi;
 #pragma unroll
                 for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        const int n = 32 * i + 8 * (r >> 2) + 4 * hi + (r & 3);
-                        bool on = n0 + n >= row.lo && n0 + n < end;
-                        if (bad[t & 3]) on = on && offsets[t & 3][n] >= 0;
-                        x[i][r] = on ? x[i][r] : -INFINITY;
+                        const int n = 32 * i + 8 * (r >> 2) + (r & 3);
+                        x[i][r] = n >= from && n < to ? x[i][r] : -INFINITY;
                     }
+                if (gap) {
+                    const uint64_t in = __ballot(offsets[t & 3][lane & (kTile - 1)] >= 0) >> (4 * hi);
+#pragma unroll
+                    for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            x[i][r] = (in >> (32 * i + 8 * (r >> 2) + (r & 3))) & 1 ? x[i][r] : -INFINITY;
+                }
             }
             float top = x[0][0];
 #pragma unroll
