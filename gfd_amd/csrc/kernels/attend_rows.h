@@ -186,6 +186,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
 
     const int splits = st.prefix ? st.splits : max(1, (g.hi - g.lo + st.chunk - 1) / st.chunk);
     if (split >= splits) return;
+    if (!st.prefix && split == 0 && tid == 0 && a.block_splits) a.block_splits[block * a.kv_heads + kv_head] = splits;
     const int base = (st.prefix ? 0 : g.lo) + split * st.chunk;
     const int c0 = max(base, g.lo), c1 = min(base + st.chunk, g.hi);
     const int64_t head = kv_head * c.head_stride;

@@ -5,7 +5,7 @@
 // workgroup of W waves takes 32 W rows, 32 a wave, and walks the keys in tiles
 // that all of its waves read from LDS.  A tile's keys and values lie there
 // as 16-bit numbers (8-bit ones are widened on the way in, once for the
-// workgroup), twice: the next tile is loaded to registers while this one is
+// workgroup), twice: the next tiles are loaded to registers while this one is
 // computed, and written behind it, so that a tile costs one barrier.
 //
 // A tile: scores^T[32 keys][32 rows] by 32x32x16 products, keys as the left operand.
@@ -88,15 +88,23 @@ struct TilesKernel {
     }
 };
 
-template <typename T, typename S, int D, int W, bool kExtras>
+// What happens to a score on its way to the exponent.
+enum { kPlain, kCapped, kBiased };
+
+template <typename T, typename S, int D, int W, int kScores>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(Call a, Cache c, Stage prefix, Stage own) {
     using K = TilesKernel<T, S, D, W>;
     constexpr int kTile = K::kTile, kRows = K::kRows;
+    // Tiles under way.  A tile's 64 keys take less time than a load from memory (1.9 us) where a CU has
+    // one workgroup or the dims are few, so two, where the registers hold them: not where 4 waves move 128
+    // dims of 16 bits, or do more with the scores.
+    constexpr int kAhead = W == 8 || D == 64 || (S::kBytes == 1 && (D == 256 || kScores == kPlain)) ||
+                                   (D == 256 && kScores != kBiased) ? 2 : 1;
     __shared__ u32x4 keys_lds[2][kTile * D / 8];
     __shared__ u32x4 values_lds[2][kTile * D / 8];
     __shared__ i32x4 rows[kRows];
     __shared__ int64_t offsets[4][kTile];
-    __shared__ int bad[4], odd[4], ranges[4][W];
+    __shared__ int bad[8], odd[8], ranges[4][W];
     int* const samples = (int*)keys_lds;
     static_assert(sizeof(keys_lds) >= (kSamples + 1) * sizeof(int), "samples fit the keys");
 
@@ -135,13 +143,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
         const Row r = row_of(a, st, k, samples, tid);
         rows[tid] = i32x4{r.t, r.pos, r.lo, r.hi};
     }
-    if (tid < 4) bad[tid] = odd[tid] = 0;
+    if (tid < 8) bad[tid] = odd[tid] = 0;
     __syncthreads();
     const int r0 = 32 * wave + col;
-    const i32x4 mine = rows[r0];
-    const Row row{mine[0], mine[1], mine[2], mine[3]};
+    // Read again where it is used: registers are short.
+    const auto my_row = [&] {
+        const i32x4 x = rows[r0];
+        return Row{x[0], x[1], x[2], x[3]};
+    };
     Range w{0x7FFFFFFF, 0, 0, 0x7FFFFFFF};
-    range_add(w, row);
+    range_add(w, my_row());
     w.lo = lanes_min(w.lo);
     w.hi = -lanes_min(-w.hi);
     w.all_lo = -lanes_min(-w.all_lo);
@@ -162,6 +173,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
 
     const int splits = st.prefix ? st.splits : max(1, (g.hi - g.lo + st.chunk - 1) / st.chunk);
     if (split >= splits) return;
+    if (!st.prefix && split == 0 && tid == 0 && a.block_splits) a.block_splits[block * a.kv_heads + kv_head] = splits;
     const int base = (st.prefix ? 0 : g.lo) + split * st.chunk;
     const int c0 = max(base, g.lo), c1 = min(base + st.chunk, g.hi);
     const int64_t head = kv_head * c.head_stride;
@@ -169,19 +181,25 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
 
     // The rows' operand, zero where there is no row.
     u32x4 q[K::kSteps];
-    const int h = head_of(a, k, r0, kv_head);
-    const float raw = a.scale * c.k_scale;
-    Score sc;
+    int pos;
+    float slope = 0.f;
     {
+        const Row row = my_row();
+        const int h = head_of(a, k, r0, kv_head);
+        pos = row.pos;
+        if (kScores == kBiased && a.slopes && row.t >= 0) slope = a.slopes[h] * kLog2e;
         const uint16_t* p = a.q + row.t * a.q_stride + (int64_t)h * D + 8 * hi;
 #pragma unroll
         for (int s = 0; s < K::kSteps; s++) q[s] = row.t >= 0 ? *(const u32x4*)(p + 16 * s) : u32x4{0, 0, 0, 0};
-        sc.factor = raw * kLog2e;
-        sc.in = a.softcap > 0.f ? raw / a.softcap : 0.f;
-        sc.cap = a.softcap * kLog2e;
-        sc.slope = a.slopes && row.t >= 0 ? a.slopes[h] * kLog2e : 0.f;
     }
-    const float factor = kExtras ? 1.f : raw * kLog2e;
+    // Exponents have base 2.  Plain scores stay the product's sums: the factor is positive, so the
+    // maximum is the same, and one multiply-add under the exponent applies it.  Capped ones,
+    // cap tanh y = cap - 2 cap / (e^2y + 1), stay -1 / (e^2y + 1): off by a few 2^-24 as the sums are.
+    const float raw = a.scale * c.k_scale, cap = a.softcap * kLog2e;
+    const float into_cap = a.softcap > 0.f ? raw / a.softcap * (2.f * kLog2e) : 0.f;
+    const float factor = kScores == kPlain ? raw * kLog2e : kScores == kCapped ? 2.f * cap : 1.f;
+    const float shift = kScores == kPlain ? 0.f : cap;
+    const int least_pos = kScores == kBiased ? lanes_min(my_row().t >= 0 ? pos : 0x7FFFFFFF) : 0;
     // A maximum that has grown by less than 2^8 is left as it is: weights and sums stay far from
     // what 16 and 32 bits hold, and the output is rescaled in a few tiles only.
     const float slack = 8.f / factor;
@@ -193,9 +211,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
 #pragma unroll
         for (int r = 0; r < 16; r++) o[i][r] = 0.f;
 
-    typename K::Staged staged;
+    typename K::Staged staged[kAhead];
     const auto whole = [&](const Range& x, int n0) { return x.all_lo <= n0 && n0 + kTile <= min(x.all_hi, c1); };
-    for (int n = tid; n < 2 * kTile; n += K::kThreads) {
+    for (int n = tid; n < 3 * kTile; n += K::kThreads) {
         const bool in = c0 + n < c1;
         const int64_t at = in ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
         if (in && at < 0) bad[n / kTile] = 1;
@@ -203,8 +221,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     }
     __syncthreads();
     if (tiles > 0) {
-        K::load(staged, c, offsets[0], tid);
-        if (K::store(staged, (uint16_t*)keys_lds[0], (uint16_t*)values_lds[0], tid, !whole(g, c0))) odd[0] = 1;
+        K::load(staged[0], c, offsets[0], tid);
+        if constexpr (kAhead == 2) K::load(staged[1], c, offsets[1], tid);
+        if (K::store(staged[0], (uint16_t*)keys_lds[0], (uint16_t*)values_lds[0], tid, !whole(g, c0))) odd[0] = 1;
     }
     __syncthreads();
 
@@ -216,23 +235,21 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     for (int i = 0; i < K::kDims; i++)
         value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap_v(v_row)) * 8 + (lane16 & 1) * 4;
 
-    // The rows' operand is there before the first tile: left to the loop, its wait would stand in front of every
-    // tile's first product and cover the next tile's loads too.
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    for (int t = 0; t < tiles; t++) {
+    // A tile: later ones' loads start, in the order of their use and whether or not there are such tiles (offsets
+    // past the end are -1, which reads the cache's start), so that each wait is for the oldest loads only.
+    const auto step = [&](int t, typename K::Staged& next, typename K::Staged& later) {
         const int n0 = c0 + t * kTile;
         const bool more = t + 1 < tiles;
-        if (more) K::load(staged, c, offsets[(t + 1) & 3], tid);
-        const int n2 = n0 + 2 * kTile + tid;
-        const bool look_up = tid < kTile && n2 < c1;
-        const uint32_t page2 = c.page.div((uint32_t)n2);
-        const int id2 = look_up ? k.table[page2] : 0;
+        const auto page_of = [&](int n) { return c.page.div((uint32_t)min(n, c1 - 1)); };
+        const int id3 = k.table[page_of(n0 + 3 * kTile + (tid & (kTile - 1)))];
+        K::load(later, c, offsets[(t + kAhead) & 3], tid);
 
-        if (odd[t & 3]) {
+        if (odd[t & 7]) {
             // Of keys that some rows see and others do not, infinities and NaN reach only the rows
             // that do: a weight of zero would not stop them.  They are added to those rows one by one
             // and are zeros in the product.
             uint16_t* vb = (uint16_t*)values_lds[t & 1];
+            const Row row = my_row();
 #pragma unroll 1
             for (int n = 0; n < kTile; n++) {
                 if (n0 + n < row.lo || n0 + n >= min(row.hi, c1)) continue;
@@ -274,16 +291,42 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
             __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-            if constexpr (kExtras) {
+            if constexpr (kScores != kPlain) {
+                const auto capped = [&](float y) {
+                    return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(y * into_cap));
+                };
+                if (kScores == kCapped || a.softcap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < K::kHalves; i++)
+                    for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        x[i][r] = score<true>(sc, a, x[i][r], row.pos, n0 + 32 * i + 8 * (r >> 2) + 4 * hi + (r & 3));
+                        for (int r = 0; r < 16; r++) x[i][r] = capped(x[i][r]);
+                }
+                if constexpr (kScores == kBiased) {
+                    const float by = a.softcap > 0.f ? 2.f * cap : raw * kLog2e;
+                    // Where all keys lie behind all rows, a row's bias grows by its slope from key to key.
+                    const int far = n0 + 4 * hi - pos;
+                    if (n0 + kTile - 1 <= least_pos) {
+                        const float bias = slope * (float)far;
+#pragma unroll
+                        for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++)
+                                x[i][r] = __builtin_fmaf(
+                                    x[i][r], by, __builtin_fmaf(slope, (float)(32 * i + 8 * (r >> 2) + (r & 3)), bias));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++)
+                                x[i][r] = __builtin_fmaf(
+                                    -slope, fabsf((float)(far + 32 * i + 8 * (r >> 2) + (r & 3))), x[i][r] * by);
+                    }
+                }
             }
-            const bool gap = bad[t & 3];
+            const bool gap = bad[t & 7];
             if (gap || !whole(w, n0)) {
                 // A lane's keys are these constants and n0 + 4 hi.
+                const Row row = my_row();
                 const int from = row.lo - n0 - 4 * hi, to = min(row.hi, c1) - n0 - 4 * hi;
 #pragma unroll
                 for (int i = 0; i < K::kHalves; i++)
@@ -340,26 +383,40 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                     }
         }
 
-        if (more && K::store(staged, (uint16_t*)keys_lds[(t + 1) & 1], (uint16_t*)values_lds[(t + 1) & 1], tid,
+        if (more && K::store(next, (uint16_t*)keys_lds[(t + 1) & 1], (uint16_t*)values_lds[(t + 1) & 1], tid,
                              !whole(g, n0 + kTile)))
-            odd[(t + 1) & 3] = 1;
+            odd[(t + 1) & 7] = 1;
         if (tid < kTile) {
             int64_t at = -1;
-            if (look_up) {
-                if (id2 < 0 || id2 >= c.num_pages) {
-                    bad[(t + 2) & 3] = 1;
+            const int n3 = n0 + 3 * kTile + tid;
+            if (n3 < c1) {
+                if (id3 < 0 || id3 >= c.num_pages) {
+                    bad[(t + 3) & 7] = 1;
                     if (a.error) atomicOr(a.error, GFD_KV_ERR_PAGE);
                 } else {
-                    at = id2 * c.page_stride + (int64_t)((uint32_t)n2 - page2 * c.page.d) * c.slot_stride + head;
+                    at = id3 * c.page_stride + (int64_t)((uint32_t)n3 - page_of(n3) * c.page.d) * c.slot_stride + head;
                 }
             }
-            offsets[(t + 2) & 3][tid] = at;
+            offsets[(t + 3) & 3][tid] = at;
         }
-        if (tid == 0) bad[(t + 3) & 3] = odd[(t + 3) & 3] = 0;
+        if (tid == 0) bad[(t + 5) & 7] = odd[(t + 5) & 7] = 0;
         __syncthreads();
+    };
+    // The rows' operand is there before the first tile: left to the loop, its wait would stand in front of every
+    // tile's first product and cover the next tiles' loads too.
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    if constexpr (kAhead == 1) {
+        for (int t = 0; t < tiles; t++) step(t, staged[0], staged[0]);
+    } else {
+        for (int t = 0; t < tiles; t += 2) {
+            step(t, staged[1], staged[0]);
+            if (t + 1 < tiles) step(t + 1, staged[0], staged[1]);
+        }
     }
 
     sum = across32_sum(sum);
+    const Row row = my_row();
+    const int h = head_of(a, k, r0, kv_head);
     if (row.t < 0) return;
     if (st.direct && splits == 1) {
         const float scale = sum == 0.f ? 0.f : c.v_scale / sum;
@@ -374,10 +431,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
             }
         if (a.lse && hi == 0)
             a.lse[(int64_t)row.t * a.q_heads + h] =
-                sum == 0.f ? -INFINITY : (m * factor + __builtin_amdgcn_logf(sum)) * kLn2;
+                sum == 0.f ? -INFINITY : (m * factor + shift + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
         const int64_t at = slot_of(a, st.first_slot + split, row.t, h);
-        if (hi == 0) a.part_ml[at] = f32x2{m == -INFINITY ? m : m * factor, sum};
+        if (hi == 0) a.part_ml[at] = f32x2{m == -INFINITY ? m : m * factor + shift, sum};
         if (sum == 0.f) return;  // its weight is zero and it is not read
         float* out = a.part_o + at * D + 4 * hi;
 #pragma unroll
@@ -400,16 +457,18 @@ int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage
     const auto go = [&](auto kernel, int w) {
         hipLaunchKernelGGL(kernel, grid, dim3(64 * w), 0, st, a, c, prefix, own);
     };
-    const bool extras = a.softcap > 0.f || a.slopes;
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if constexpr (D != 256) {
-            if (waves == 8) {
-                extras ? go(attend_tiles_kernel<T, S, D, 8, true>, 8) : go(attend_tiles_kernel<T, S, D, 8, false>, 8);
-                return;
+        const auto with = [&](auto scores) {
+            constexpr int kScores = decltype(scores)::value;
+            if constexpr (D != 256) {
+                if (waves == 8) return go(attend_tiles_kernel<T, S, D, 8, kScores>, 8);
             }
-        }
-        extras ? go(attend_tiles_kernel<T, S, D, 4, true>, 4) : go(attend_tiles_kernel<T, S, D, 4, false>, 4);
+            go(attend_tiles_kernel<T, S, D, 4, kScores>, 4);
+        };
+        if (a.slopes) with(std::integral_constant<int, kBiased>());
+        else if (a.softcap > 0.f) with(std::integral_constant<int, kCapped>());
+        else with(std::integral_constant<int, kPlain>());
     };
     if (dim == 64) pick(std::integral_constant<int, 64>());
     if (dim == 128) pick(std::integral_constant<int, 128>());

@@ -39,6 +39,7 @@ struct Call {
     // Partial results, [slot][token][head]: maximum and sum, and the unnormalised output.
     f32x2* part_ml;
     float* part_o;
+    int* block_splits;  // ranges that an own-keys block has, [block][head of the cache]
 };
 
 // One kind of work of a launch: row blocks times key ranges times the cache's heads.
@@ -65,15 +66,17 @@ struct Sequence {
     bool cut;
 };
 
-__device__ __forceinline__ Sequence sequence(const Call& a, int b) {
+__device__ __forceinline__ Sequence sequence(const Call& a, int start, int end, int kv_len) {
     Sequence s;
-    s.first = min(max(a.q_start[b], 0), a.num_tokens);
-    s.q_len = min(max(a.q_start[b + 1], s.first), a.num_tokens) - s.first;
+    s.first = min(max(start, 0), a.num_tokens);
+    s.q_len = min(max(end, s.first), a.num_tokens) - s.first;
     s.rows_q = min(s.q_len, a.max_q_len);
-    const int n = a.kv_len[b];
-    s.kv_len = min(n, a.max_kv_len);
-    s.cut = s.q_len > a.max_q_len || n > a.max_kv_len;
+    s.kv_len = min(kv_len, a.max_kv_len);
+    s.cut = s.q_len > a.max_q_len || kv_len > a.max_kv_len;
     return s;
+}
+__device__ __forceinline__ Sequence sequence(const Call& a, int b) {
+    return sequence(a, a.q_start[b], a.q_start[b + 1], a.kv_len[b]);
 }
 
 __device__ __forceinline__ Row make_row(const Call& a, const Sequence& s, int i, bool prefix) {
@@ -94,19 +97,24 @@ __device__ __forceinline__ Row make_row(const Call& a, const Sequence& s, int i,
     return r;
 }
 
+// The rows of a workgroup.
+struct Block {
+    int b, first_row, rows;  // rows of sequence b (own keys) or of all tokens (prefix)
+    Sequence seq;            // own keys
+    const int* table;
+};
+
 // Where index lies among the blocks of kRows rows that the sequences have, the
 // last block of a sequence first: it sees the most keys.  A wave's lanes each
 // count a sequence's blocks.
 template <int kRows>
-__device__ __forceinline__ bool find_block(const Call& a, int index, int* b, int* block) {
+__device__ __forceinline__ bool find_block(const Call& a, int index, Block* k) {
     const int lane = (int)threadIdx.x & 63;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        int n = 0;
-        if (b0 + lane < a.batch) {
-            const int first = min(max(a.q_start[b0 + lane], 0), a.num_tokens);
-            const int q_len = min(min(max(a.q_start[b0 + lane + 1], first), a.num_tokens) - first, a.max_q_len);
-            n = (int)(((int64_t)q_len * a.group.d + kRows - 1) / kRows);
-        }
+        const int b = min(b0 + lane, a.batch - 1), start = a.q_start[b], end = a.q_start[b + 1], kv_len = a.kv_len[b];
+        const int n = b0 + lane < a.batch
+                          ? (int)(((int64_t)sequence(a, start, end, kv_len).rows_q * a.group.d + kRows - 1) / kRows)
+                          : 0;
         int sum = n;
         for (int off = 1; off < 64; off <<= 1) {
             const int up = __shfl_up(sum, off);
@@ -115,8 +123,10 @@ __device__ __forceinline__ bool find_block(const Call& a, int index, int* b, int
         const int total = __shfl(sum, 63);
         if (index < total) {
             const int at = __ffsll((long long)__ballot(index < sum)) - 1;
-            *b = b0 + at;
-            *block = __builtin_amdgcn_readfirstlane(__shfl(sum, at) - 1 - index);
+            const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+            k->b = b0 + at;
+            k->first_row = (of(sum) - 1 - index) * kRows;
+            k->seq = sequence(a, of(start), of(end), of(kv_len));
             return true;
         }
         index -= total;
@@ -147,12 +157,6 @@ __device__ __forceinline__ int sequence_of(const Call& a, const int* samples, in
     return lo;
 }
 
-// The rows of a workgroup and the keys that any of them sees.
-struct Block {
-    int b, first_row, rows;  // rows of the sequence (own keys) or of all tokens (prefix)
-    const int* table;
-};
-
 // What rows [0, rows) of a block see: [lo, hi) by any, [all_lo, all_hi) by every one.
 struct Range {
     int lo, hi, all_lo, all_hi;
@@ -173,8 +177,7 @@ __device__ __forceinline__ int lanes_min(int x) {
     return __builtin_amdgcn_readfirstlane(x);
 }
 
-// Sets up rows[0, kRows) in LDS by one wave per 64 rows and returns what each
-// wave's rows see.  False: nothing for this block.
+// The rows of block block_index; false: none.
 template <int kRows>
 __device__ __forceinline__ bool find_rows(const Call& a, const Stage& st, int block_index, Block* k) {
     k->b = 0;
@@ -184,17 +187,15 @@ __device__ __forceinline__ bool find_rows(const Call& a, const Stage& st, int bl
         k->table = a.prefix_table;
         return true;
     }
-    int at = 0;
     if (st.whole) {
         k->b = block_index;
-    } else if (!find_block<kRows>(a, block_index, &k->b, &at)) {
+        k->first_row = 0;
+        k->seq = sequence(a, k->b);
+    } else if (!find_block<kRows>(a, block_index, k)) {
         return false;
     }
-    k->first_row = at * kRows;
     k->table = a.table + (int64_t)k->b * a.table_stride;
-    const int first = min(max(a.q_start[k->b], 0), a.num_tokens);
-    const int q_len = min(min(max(a.q_start[k->b + 1], first), a.num_tokens) - first, a.max_q_len);
-    k->rows = (int)min((int64_t)kRows, (int64_t)q_len * a.group.d - k->first_row);
+    k->rows = (int)min((int64_t)kRows, (int64_t)k->seq.rows_q * a.group.d - k->first_row);
     return k->rows > 0;
 }
 
@@ -204,9 +205,8 @@ __device__ __forceinline__ Row row_of(const Call& a, const Stage& st, const Bloc
     if (r >= k.rows) return x;
     const int i = (int)a.group.div((uint32_t)(k.first_row + r));
     if (!st.prefix) {
-        const Sequence s = sequence(a, k.b);
-        if (s.cut && a.error) atomicOr(a.error, GFD_KV_ERR_LENGTH);
-        return make_row(a, s, i, false);
+        if (k.seq.cut && a.error) atomicOr(a.error, GFD_KV_ERR_LENGTH);
+        return make_row(a, k.seq, i, false);
     }
     const int b = sequence_of(a, samples, i);
     if (b < 0) return x;

@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 
 #include "capi_error.h"
 #include "gfd_capi.h"
@@ -19,35 +20,25 @@ namespace gfd {
 namespace kv {
 namespace {
 
-constexpr int kJoinBlock = 256, kJoinRows = kJoinBlock / 64;
+constexpr int kJoinBlock = 256;
 
-// A workgroup joins kJoinRows rows of an own-keys block, a wave per row: a lane
+// A workgroup joins kPart rows of an own-keys block, a wave per row: a lane
 // weighs one range of 64, then holds D / 64 dims.  Reads what the ranges
 // left once; bound by the launch's latency for small batches.
-template <typename T, int D, int kRows>
-__global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage prefix, Stage own) {
+template <typename T, int D, int kRows, int kPart>
+__global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage own) {
     constexpr int kDims = D / 64, kWaves = kJoinBlock / 64;
     typedef float Dims __attribute__((ext_vector_type(kDims)));
-    __shared__ int lo[kWaves], hi[kWaves];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int kv_head = (int)blockIdx.x % a.kv_heads;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int kv_head = (int)blockIdx.x % a.kv_heads, block = (int)blockIdx.x / a.kv_heads;
     Block k;
-    if (!find_rows<kRows>(a, own, (int)blockIdx.x / a.kv_heads, &k)) return;
-    Range g{0x7FFFFFFF, 0, 0, 0};
-    if (tid < kRows) range_add(g, row_of(a, own, k, nullptr, tid));
-    g.lo = lanes_min(g.lo);
-    g.hi = -lanes_min(-g.hi);
-    if (lane == 0) lo[wave] = g.lo, hi[wave] = g.hi;
-    __syncthreads();
-    for (int i = 0; i < kWaves; i++) g.lo = min(g.lo, lo[i]), g.hi = max(g.hi, hi[i]);
-    if (g.hi == 0) g.lo = 0;
-    const int splits = max(1, (g.hi - g.lo + own.chunk - 1) / own.chunk), slots = own.first_slot + splits;
+    if (!find_rows<kRows>(a, own, block, &k)) return;
+    const int splits = a.block_splits[blockIdx.x], slots = own.first_slot + splits;
     if (own.direct && splits == 1) return;
 
-    const int r = (int)blockIdx.y * kJoinRows + wave;
-    if (r >= k.rows) return;
-    {
-        const int t = min(max(a.q_start[k.b], 0), a.num_tokens) + (int)a.group.div((uint32_t)(k.first_row + r));
+    const int first = (int)blockIdx.y * kPart;
+    for (int r = first + wave; r < min(first + kPart, k.rows); r += kWaves) {
+        const int t = k.seq.first + (int)a.group.div((uint32_t)(k.first_row + r));
         const int h = head_of(a, k, r, kv_head);
         float top = -INFINITY;
         for (int s0 = 0; s0 < slots; s0 += 64) {
@@ -114,7 +105,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // below one round the shortest range, a tile per wave, counts.
 constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
 // Many rows: a workgroup fills a CU (or half of it), so two rounds of them do.
-constexpr int kTilesFill = 512, kTilesMinChunk = 256;
+const int kTilesFill = getenv("X_TFILL") ? atoi(getenv("X_TFILL")) : 512, kTilesMinChunk = getenv("X_TMIN") ? atoi(getenv("X_TMIN")) : 256, kW8 = getenv("X_W8") ? atoi(getenv("X_W8")) : 65536;
 
 void split(Stage* st, int64_t items, int64_t keys, bool few) {
     if (few) {
@@ -129,7 +120,7 @@ void split(Stage* st, int64_t items, int64_t keys, bool few) {
 }
 
 // Waves of a block of many rows: 8 where that still fills the card, for half the reads of the cache.
-int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= 256 * 256 ? 8 : 4; }
+int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= kW8 ? 8 : 4; }
 
 Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
     Plan p{};
@@ -160,19 +151,23 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
     }
     p.slots = p.own.first_slot + p.own.splits;
     p.items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
-    if (p.slots > 1) p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4;
+    if (p.slots > 1)
+        p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4 + p.own.blocks * heads * 4;
     return p;
 }
 
+template <typename T, int D, int kRows, int kPart>
+int launch_join(const Call& a, const Cache& c, const Stage& own, hipStream_t st) {
+    hipLaunchKernelGGL((join_kernel<T, D, kRows, kPart>), dim3((unsigned)(own.blocks * a.kv_heads), kRows / kPart),
+                       dim3(kJoinBlock), 0, st, a, c, own);
+    return (int)hipGetLastError();
+}
 template <typename T, int D>
 int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
-    const dim3 grid((unsigned)(p.own.blocks * a.kv_heads), (unsigned)ceil_div(p.rows, kJoinRows));
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kJoinBlock), 0, st, a, c, p.prefix, p.own); };
-    if (p.rows == 16) go(join_kernel<T, D, 16>);
-    if (p.rows == 32) go(join_kernel<T, D, 32>);
-    if (p.rows == 128) go(join_kernel<T, D, 128>);
-    if (p.rows == 256) go(join_kernel<T, D, 256>);
-    return (int)hipGetLastError();
+    return p.rows == 16    ? launch_join<T, D, 16, 4>(a, c, p.own, st)
+           : p.rows == 32  ? launch_join<T, D, 32, 4>(a, c, p.own, st)
+           : p.rows == 128 ? launch_join<T, D, 128, 16>(a, c, p.own, st)
+                           : launch_join<T, D, 256, 16>(a, c, p.own, st);
 }
 
 template <typename T, typename S>
@@ -234,12 +229,14 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     if (p.bytes && (!workspace || workspace_bytes < (size_t)p.bytes || (uintptr_t)workspace % 16 != 0))
         return refuse(name, "workspace is missing, not 16-byte aligned or smaller than gfd_attention_workspace_bytes says");
     const int64_t rows = (int64_t)w.num_tokens * w.num_q_heads;
-    float* const part_o = (float*)workspace;
+    float* const part_o = p.bytes ? (float*)workspace : nullptr;
+    float* const part_ml = p.bytes ? part_o + p.slots * rows * cache->head_dim : nullptr;
+    float* const splits = p.bytes ? part_ml + p.slots * rows * 2 : nullptr;
     const Call a{(const uint16_t*)w.q, (uint16_t*)w.out, w.lse, w.q_stride, w.out_stride, w.q_start, w.kv_len,
                  w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, w.scale,
                  w.softcap, w.window, w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
                  cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
-                 (f32x2*)(part_o + p.slots * rows * cache->head_dim), part_o};
+                 (f32x2*)part_ml, part_o, (int*)splits};
     const Cache c = make_cache(*cache);
     const hipStream_t st = (hipStream_t)stream;
     if (cache->dtype == GFD_E4M3)
