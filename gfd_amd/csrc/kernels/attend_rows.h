@@ -133,22 +133,26 @@ struct RowsKernel {
 };
 
 template <typename T, typename S, int D, int R>
-__global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(Call a, Cache c,
-                                                                                    Stage prefix, Stage own) {
+struct RowsLds {
     using K = RowsKernel<T, S, D, R>;
-    constexpr int kRows = 16 * R, kWaves = kRowsBlock / 64;
-    __shared__ i32x4 rows[kRows];
-    __shared__ int64_t offsets[kRowsMaxChunk];
-    __shared__ union {
+    static constexpr int kWaves = kRowsBlock / 64;
+    i32x4 rows[16 * R];
+    int64_t offsets[kRowsMaxChunk];
+    union {
         int samples[kSamples + 1];
         float merge[kWaves / 2][R * K::kAcc + 2 * R][64];
         u32x4 keys[kWaves][kRowsTile * K::kKeyChunks];
-    } lds;
-    __shared__ int any_bad;
-    __shared__ u32x4 lds_rows[K::kLdsRows ? R * K::kSteps : 1][64];
+    };
+    u32x4 queries[K::kLdsRows ? R * K::kSteps : 1][64];
+    int any_bad;
+};
 
+template <typename T, typename S, int D, int R>
+__device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int item,
+                                            RowsLds<T, S, D, R>& lds) {
+    using K = RowsKernel<T, S, D, R>;
+    constexpr int kRows = 16 * R, kWaves = kRowsBlock / 64;
     // Heads vary fastest: their keys lie side by side.  Ranges vary slowest: the last ones are often empty.
-    int item = (int)blockIdx.x;
     const int prefix_items = prefix.blocks * prefix.splits * a.kv_heads;
     const Stage st = item < prefix_items ? prefix : own;
     if (item >= prefix_items) item -= prefix_items;
@@ -168,13 +172,13 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
     Range g{0x7FFFFFFF, 0, 0, 0x7FFFFFFF};
     if (wave == 0 && lane < kRows) {
         const Row r = row_of(a, st, k, lds.samples, lane);
-        rows[lane] = i32x4{r.t, r.pos, r.lo, r.hi};
+        lds.rows[lane] = i32x4{r.t, r.pos, r.lo, r.hi};
     }
-    if (tid == 0) any_bad = 0;
+    if (tid == 0) lds.any_bad = 0;
     __syncthreads();
     Row row[R];
     for (int i = 0; i < R; i++) {
-        const i32x4 x = rows[16 * i + col];
+        const i32x4 x = lds.rows[16 * i + col];
         row[i] = Row{x[0], x[1], x[2], x[3]};
         range_add(g, row[i]);
     }
@@ -193,8 +197,8 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
     const int tiles = c1 > c0 ? (c1 - c0 + kRowsTile - 1) / kRowsTile : 0;
     for (int n = tid; n < tiles * kRowsTile; n += kRowsBlock) {
         const int64_t o = c0 + n < c1 ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
-        if (o < 0 && c0 + n < c1) any_bad = 1;
-        offsets[n] = o;
+        if (o < 0 && c0 + n < c1) lds.any_bad = 1;
+        lds.offsets[n] = o;
     }
 
     // The rows' operand, zero where there is no row.
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
         for (int s = 0; s < K::kSteps; s++) {
             if (K::kLdsRows && wave != (i * K::kSteps + s) % kWaves) continue;
             const u32x4 x = row[i].t >= 0 ? *(const u32x4*)(p + K::step_dim(s, quarter)) : u32x4{0, 0, 0, 0};
-            if constexpr (K::kLdsRows) lds_rows[i * K::kSteps + s][lane] = x;
+            if constexpr (K::kLdsRows) lds.queries[i * K::kSteps + s][lane] = x;
             else q[i][s] = x;
         }
         sc[i].factor = raw * kLog2e;
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
     const float factor = extras ? 1.f : raw * kLog2e;
 
     __syncthreads();
-    const bool bad = any_bad != 0;
+    const bool bad = lds.any_bad != 0;
     float m[R], sum[R];
     f32x4 o[R][K::kDims];
     for (int i = 0; i < R; i++) {
@@ -232,13 +236,13 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
     int valid = 0;
     bool any_odd = false;
     if (wave < tiles) {
-        K::load_keys(t, c, offsets + wave * kRowsTile, lane);
-        valid = K::load_values(t, c, offsets + wave * kRowsTile, lane);
+        K::load_keys(t, c, lds.offsets + wave * kRowsTile, lane);
+        valid = K::load_values(t, c, lds.offsets + wave * kRowsTile, lane);
     }
     for (int tile = wave; tile < tiles; tile += kWaves) {
         const int n0 = c0 + tile * kRowsTile;
         const bool more = tile + kWaves < tiles;
-        const int64_t* next = offsets + (tile + kWaves) * kRowsTile;
+        const int64_t* next = lds.offsets + (tile + kWaves) * kRowsTile;
         if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
         K::store_keys(t, my_keys, lane);
         // Other lanes of the wave read them: its LDS accesses are in order, the compiler has to keep them so.
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
 #pragma unroll
                 for (int i = 0; i < R; i++) {
                     u32x4 qf;
-                    if constexpr (K::kLdsRows) qf = lds_rows[i * K::kSteps + s + j][lane];
+                    if constexpr (K::kLdsRows) qf = lds.queries[i * K::kSteps + s + j][lane];
                     else qf = q[i][s + j];
                     x[i][0] = Mma<T>::m16(k0[j], qf, x[i][0]);
                     x[i][1] = Mma<T>::m16(k1[j], qf, x[i][1]);
@@ -344,7 +348,7 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
         for (int tile = wave; tile < tiles; tile += kWaves)
 #pragma unroll 1
             for (int n = tile * kRowsTile; n < (tile + 1) * kRowsTile; n++) {
-                const int64_t at = offsets[n];
+                const int64_t at = lds.offsets[n];
                 const uint8_t* from = c.v + (at < 0 ? 0 : at) + 4 * quarter * K::kDims * K::kSize;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -425,6 +429,13 @@ __global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) 
                         f32x4{o[i][d][r], o[i][d + 1][r], o[i][d + 2][r], o[i][d + 3][r]};
         }
     }
+}
+
+template <typename T, typename S, int D, int R>
+__global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(
+    Call a, Cache c, Stage prefix, Stage own) {
+    __shared__ RowsLds<T, S, D, R> lds;
+    attend_rows<T, S, D, R>(a, c, prefix, own, (int)blockIdx.x, lds);
 }
 
 template <typename T, typename S>

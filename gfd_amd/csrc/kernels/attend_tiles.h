@@ -33,51 +33,63 @@ struct TilesKernel {
 
     struct Staged {
         uint32_t k[kUnits][kUnitWords], v[kUnits][kUnitWords];
-        bool on[kUnits];
     };
+    // A thread moves the same chunk of every kStride-th row.
+    static constexpr int kStride = kThreads / kChunks;
+    static_assert(kThreads % kChunks == 0, "a thread's chunks are all the same");
 
     // Where a row's chunk lies, so that rows that are read together meet in no bank (64 of 4 bytes).  Keys: one chunk
     // of 16 rows at once.  Values: two neighbouring chunks of 4 rows.  A row of 128 bytes (D 64) is half the banks.
     static __device__ __forceinline__ int swap_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
     static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 
-    static __device__ __forceinline__ void load(Staged& g, const Cache& c, const int64_t* off, int tid) {
+    // kc and vc: the thread's chunk of the cache's first row.
+    static __device__ __forceinline__ void load(Staged& g, const uint8_t* kc, const uint8_t* vc, const int64_t* off, int tid) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int n = tid + u * kThreads, row = n / kChunks, chunk = n % kChunks;
-            const int64_t o = off[row];
-            g.on[u] = o >= 0;
-            const int64_t at = (o < 0 ? 0 : o) + chunk * 8 * S::kBytes;
+            const int64_t o = off[tid / kChunks + u * kStride];
             if constexpr (S::kBytes == 2) {
-                const u32x4 k = *(const u32x4*)(c.k + at), v = *(const u32x4*)(c.v + at);
+                const u32x4 k = *(const u32x4*)(kc + o), v = *(const u32x4*)(vc + o);
 #pragma unroll
                 for (int i = 0; i < 4; i++) g.k[u][i] = k[i], g.v[u][i] = v[i];
             } else {
-                const u32x2 k = *(const u32x2*)(c.k + at), v = *(const u32x2*)(c.v + at);
+                const u32x2 k = *(const u32x2*)(kc + o), v = *(const u32x2*)(vc + o);
 #pragma unroll
                 for (int i = 0; i < 2; i++) g.k[u][i] = k[i], g.v[u][i] = v[i];
             }
         }
     }
-    static __device__ __forceinline__ u32x4 widened(const uint32_t (&w)[kUnitWords], bool on) {
-        u32x4 r;
-        if constexpr (S::kBytes == 2) r = u32x4{w[0], w[1], w[2], w[3]};
-        else r = u32x4{Mma<T>::widen_lo(w[0]), Mma<T>::widen_hi(w[0]), Mma<T>::widen_lo(w[1]), Mma<T>::widen_hi(w[1])};
-        return on ? r : u32x4{0, 0, 0, 0};
+    static __device__ __forceinline__ u32x4 widened(const uint32_t (&w)[kUnitWords]) {
+        if constexpr (S::kBytes == 2) return u32x4{w[0], w[1], w[2], w[3]};
+        else return u32x4{Mma<T>::widen_lo(w[0]), Mma<T>::widen_hi(w[0]), Mma<T>::widen_lo(w[1]), Mma<T>::widen_hi(w[1])};
     }
-    // Nonzero where look is set and a value is infinite or NaN.
-    static __device__ __forceinline__ uint32_t store(const Staged& g, uint16_t* kb, uint16_t* vb, int tid, bool look) {
-        uint32_t odd = 0;
+    // Values of keys that are not there (there: not NULL if there may be such) become zeros; keys may be anything,
+    // their scores are not used.  Nonzero where look is set and a value is infinite or NaN.
+    static __device__ __forceinline__ uint32_t store(const Staged& g, uint16_t* kb, uint16_t* vb, int tid,
+                                                     const int* there, bool look) {
+        const int chunk = tid % kChunks;
+        u32x4 v[kUnits];
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int n = tid + u * kThreads, row = n / kChunks, chunk = n % kChunks;
-            const u32x4 v = widened(g.v[u], g.on[u]);
-            *(u32x4*)(kb + row * D + (chunk ^ swap_k(row)) * 8) = widened(g.k[u], g.on[u]);
-            *(u32x4*)(vb + row * D + (chunk ^ swap_v(row)) * 8) = v;
-            if (look) {
+            const int row = tid / kChunks + u * kStride;
+            v[u] = widened(g.v[u]);
+            *(u32x4*)(kb + row * D + (chunk ^ swap_k(row)) * 8) = widened(g.k[u]);
+        }
+        if (there) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) odd |= not_finite<T>(v[i]);
-            }
+            for (int u = 0; u < kUnits; u++) v[u] = there[tid / kChunks + u * kStride] ? v[u] : u32x4{0, 0, 0, 0};
+        }
+        uint32_t odd = 0;
+        if (look) {
+#pragma unroll
+            for (int u = 0; u < kUnits; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) odd |= not_finite<T>(v[u][i]);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            const int row = tid / kChunks + u * kStride;
+            *(u32x4*)(vb + row * D + (chunk ^ swap_v(row)) * 8) = v[u];
         }
         return odd;
     }
@@ -91,22 +103,35 @@ struct TilesKernel {
 // What happens to a score on its way to the exponent.
 enum { kPlain, kCapped, kBiased };
 
+template <typename T, typename S, int D, int W>
+struct TilesLds {
+    using K = TilesKernel<T, S, D, W>;
+    union {
+        u32x4 keys[2][K::kTile * D / 8];
+        int samples[kSamples + 1];
+    };
+    u32x4 values[2][K::kTile * D / 8];
+    i32x4 rows[K::kRows];
+    int64_t offsets[4][K::kTile];  // of keys, 0 where none is
+    int there[4][K::kTile];
+    int bad[8], odd[8], ranges[4][W];
+};
+
 template <typename T, typename S, int D, int W, int kScores>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(Call a, Cache c, Stage prefix, Stage own) {
+__device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int id,
+                                             TilesLds<T, S, D, W>& lds) {
     using K = TilesKernel<T, S, D, W>;
     constexpr int kTile = K::kTile, kRows = K::kRows;
-    // Tiles under way.  A tile's 64 keys take less time than a load from memory (1.9 us) where a CU has
-    // one workgroup or the dims are few, so two, where the registers hold them: not where 4 waves move 128
-    // dims of 16 bits, or do more with the scores.
-    constexpr int kAhead = W == 8 || D == 64 || (S::kBytes == 1 && (D == 256 || kScores == kPlain)) ||
-                                   (D == 256 && kScores != kBiased) ? 2 : 1;
-    __shared__ u32x4 keys_lds[2][kTile * D / 8];
-    __shared__ u32x4 values_lds[2][kTile * D / 8];
-    __shared__ i32x4 rows[kRows];
-    __shared__ int64_t offsets[4][kTile];
-    __shared__ int bad[8], odd[8], ranges[4][W];
-    int* const samples = (int*)keys_lds;
-    static_assert(sizeof(keys_lds) >= (kSamples + 1) * sizeof(int), "samples fit the keys");
+    // Tiles under way: two where the registers hold them (4096 tokens over 16384 keys, 8 waves: 948 us, with one 1056).
+    // 4 waves that move 128 dims of 16 bits hold one.
+    constexpr int kAhead = W == 8 || D == 64 || S::kBytes == 1 || (D == 256 && kScores != kBiased) ? 2 : 1;
+    auto &keys_lds = lds.keys, &values_lds = lds.values;
+    auto &rows = lds.rows;
+    auto &offsets = lds.offsets;
+    auto &there = lds.there;
+    auto &bad = lds.bad, &odd = lds.odd;
+    auto &ranges = lds.ranges;
+    int* const samples = lds.samples;
 
     const int tid = (int)threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -114,7 +139,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     // L2 then holds them, wherever the heads divide that way.
     int kv_head, item;
     {
-        const int id = (int)blockIdx.x, xcd = id & 7, turn = id >> 3;
+        const int xcd = id & 7, turn = id >> 3;
         const int items = prefix.blocks * prefix.splits + own.blocks * own.splits;
         if (a.kv_heads % 8 == 0) {
             kv_head = xcd + 8 * (turn / items);
@@ -187,7 +212,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
         const Row row = my_row();
         const int h = head_of(a, k, r0, kv_head);
         pos = row.pos;
-        if (kScores == kBiased && a.slopes && row.t >= 0) slope = a.slopes[h] * kLog2e;
+        if (kScores == kBiased && row.t >= 0) slope = a.slopes[h];
         const uint16_t* p = a.q + row.t * a.q_stride + (int64_t)h * D + 8 * hi;
 #pragma unroll
         for (int s = 0; s < K::kSteps; s++) q[s] = row.t >= 0 ? *(const u32x4*)(p + 16 * s) : u32x4{0, 0, 0, 0};
@@ -197,9 +222,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     // cap tanh y = cap - 2 cap / (e^2y + 1), stay -1 / (e^2y + 1): off by a few 2^-24 as the sums are.
     const float raw = a.scale * c.k_scale, cap = a.softcap * kLog2e;
     const float into_cap = a.softcap > 0.f ? raw / a.softcap * (2.f * kLog2e) : 0.f;
-    const float factor = kScores == kPlain ? raw * kLog2e : kScores == kCapped ? 2.f * cap : 1.f;
+    const float factor = a.softcap > 0.f && kScores != kPlain ? 2.f * cap : raw * kLog2e;
     const float shift = kScores == kPlain ? 0.f : cap;
+    // A bias in the scores' units: the sums of the product start from it, or it is added to what a cap leaves.
+    slope *= kLog2e / factor;
     const int least_pos = kScores == kBiased ? lanes_min(my_row().t >= 0 ? pos : 0x7FFFFFFF) : 0;
+    const int last_pos = kScores == kBiased ? -lanes_min(my_row().t >= 0 ? -pos : 0x7FFFFFFF) : 0;
     // A maximum that has grown by less than 2^8 is left as it is: weights and sums stay far from
     // what 16 and 32 bits hold, and the output is rescaled in a few tiles only.
     const float slack = 8.f / factor;
@@ -217,13 +245,23 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
         const bool in = c0 + n < c1;
         const int64_t at = in ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
         if (in && at < 0) bad[n / kTile] = 1;
-        offsets[n / kTile][n % kTile] = at;
+        offsets[n / kTile][n % kTile] = max(at, (int64_t)0);
+        there[n / kTile][n % kTile] = at >= 0;
     }
+    const uint8_t* const kc = c.k + tid % K::kChunks * 8 * S::kBytes;
+    const uint8_t* const vc = c.v + tid % K::kChunks * 8 * S::kBytes;
+    const auto keep = [&](const typename K::Staged& x, int t) {  // tile t to LDS
+        const int n0 = c0 + t * kTile;
+        const bool full = n0 + kTile <= c1 && !bad[t & 7];
+        if (K::store(x, (uint16_t*)keys_lds[t & 1], (uint16_t*)values_lds[t & 1], tid, full ? nullptr : there[t & 3],
+                     !whole(g, n0)))
+            odd[t & 7] = 1;
+    };
     __syncthreads();
     if (tiles > 0) {
-        K::load(staged[0], c, offsets[0], tid);
-        if constexpr (kAhead == 2) K::load(staged[1], c, offsets[1], tid);
-        if (K::store(staged[0], (uint16_t*)keys_lds[0], (uint16_t*)values_lds[0], tid, !whole(g, c0))) odd[0] = 1;
+        K::load(staged[0], kc, vc, offsets[0], tid);
+        if constexpr (kAhead == 2) K::load(staged[1], kc, vc, offsets[1], tid);
+        keep(staged[0], 0);
     }
     __syncthreads();
 
@@ -236,13 +274,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
         value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap_v(v_row)) * 8 + (lane16 & 1) * 4;
 
     // A tile: later ones' loads start, in the order of their use and whether or not there are such tiles (offsets
-    // past the end are -1, which reads the cache's start), so that each wait is for the oldest loads only.
+    // past the end are 0, which reads the cache's start), so that each wait is for the oldest loads only.
     const auto step = [&](int t, typename K::Staged& next, typename K::Staged& later) {
         const int n0 = c0 + t * kTile;
         const bool more = t + 1 < tiles;
+        // The pages of the tile after those, by the first wave's lanes.
+        const int n3 = n0 + 3 * kTile + (lane & (kTile - 1));
         const auto page_of = [&](int n) { return c.page.div((uint32_t)min(n, c1 - 1)); };
-        const int id3 = k.table[page_of(n0 + 3 * kTile + (tid & (kTile - 1)))];
-        K::load(later, c, offsets[(t + kAhead) & 3], tid);
+        int id3 = 0;
+        if (wave == 0) id3 = k.table[page_of(n3)];
+        K::load(later, kc, vc, offsets[(t + kAhead) & 3], tid);
 
         if (odd[t & 7]) {
             // Of keys that some rows see and others do not, infinities and NaN reach only the rows
@@ -274,10 +315,37 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
             const uint16_t* kb = (const uint16_t*)keys_lds[t & 1] + key_at;
             const uint16_t* vb = (const uint16_t*)values_lds[t & 1];
             f32x16 x[K::kHalves];
+            const auto add_bias = [&](auto first) {
+                // Where all keys lie behind all rows, or before them, it grows by a slope from key to key.
+                const float far = (float)(n0 + 4 * hi - pos);
+                const bool behind = n0 + kTile - 1 <= least_pos;
+                if (behind || n0 >= last_pos) {
+                    const float by = behind ? slope : -slope, from = by * far;
 #pragma unroll
-            for (int i = 0; i < K::kHalves; i++)
+                    for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) x[i][r] = 0.f;
+                        for (int r = 0; r < 16; r++) {
+                            const float b = __builtin_fmaf(by, (float)(32 * i + 8 * (r >> 2) + (r & 3)), from);
+                            x[i][r] = decltype(first)::value ? b : x[i][r] + b;
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const float b = -slope * fabsf(far + (float)(32 * i + 8 * (r >> 2) + (r & 3)));
+                            x[i][r] = decltype(first)::value ? b : x[i][r] + b;
+                        }
+                }
+            };
+            if (kScores == kBiased && !(a.softcap > 0.f)) {
+                add_bias(std::true_type());
+            } else {
+#pragma unroll
+                for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) x[i][r] = 0.f;
+            }
 #pragma unroll
             for (int s = 0; s < K::kSteps; s++)
 #pragma unroll
@@ -291,37 +359,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
             __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-            if constexpr (kScores != kPlain) {
-                const auto capped = [&](float y) {
-                    return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(y * into_cap));
-                };
-                if (kScores == kCapped || a.softcap > 0.f) {
+            if (kScores == kCapped || (kScores == kBiased && a.softcap > 0.f)) {
 #pragma unroll
-                    for (int i = 0; i < K::kHalves; i++)
+                for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) x[i][r] = capped(x[i][r]);
-                }
-                if constexpr (kScores == kBiased) {
-                    const float by = a.softcap > 0.f ? 2.f * cap : raw * kLog2e;
-                    // Where all keys lie behind all rows, a row's bias grows by its slope from key to key.
-                    const int far = n0 + 4 * hi - pos;
-                    if (n0 + kTile - 1 <= least_pos) {
-                        const float bias = slope * (float)far;
-#pragma unroll
-                        for (int i = 0; i < K::kHalves; i++)
-#pragma unroll
-                            for (int r = 0; r < 16; r++)
-                                x[i][r] = __builtin_fmaf(
-                                    x[i][r], by, __builtin_fmaf(slope, (float)(32 * i + 8 * (r >> 2) + (r & 3)), bias));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < K::kHalves; i++)
-#pragma unroll
-                            for (int r = 0; r < 16; r++)
-                                x[i][r] = __builtin_fmaf(
-                                    -slope, fabsf((float)(far + 32 * i + 8 * (r >> 2) + (r & 3))), x[i][r] * by);
-                    }
-                }
+                    for (int r = 0; r < 16; r++)
+                        x[i][r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[i][r] * into_cap));
+                if (kScores == kBiased) add_bias(std::false_type());
             }
             const bool gap = bad[t & 7];
             if (gap || !whole(w, n0)) {
@@ -336,7 +380,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                         x[i][r] = n >= from && n < to ? x[i][r] : -INFINITY;
                     }
                 if (gap) {
-                    const uint64_t in = __ballot(offsets[t & 3][lane & (kTile - 1)] >= 0) >> (4 * hi);
+                    const uint64_t in = __ballot(there[t & 3][lane & (kTile - 1)]) >> (4 * hi);
 #pragma unroll
                     for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
@@ -383,12 +427,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                     }
         }
 
-        if (more && K::store(next, (uint16_t*)keys_lds[(t + 1) & 1], (uint16_t*)values_lds[(t + 1) & 1], tid,
-                             !whole(g, n0 + kTile)))
-            odd[(t + 1) & 7] = 1;
-        if (tid < kTile) {
+        if (more) keep(next, t + 1);
+        if (wave == 0) {
             int64_t at = -1;
-            const int n3 = n0 + 3 * kTile + tid;
             if (n3 < c1) {
                 if (id3 < 0 || id3 >= c.num_pages) {
                     bad[(t + 3) & 7] = 1;
@@ -397,7 +438,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
                     at = id3 * c.page_stride + (int64_t)((uint32_t)n3 - page_of(n3) * c.page.d) * c.slot_stride + head;
                 }
             }
-            offsets[(t + 3) & 3][tid] = at;
+            if (lane < kTile) {
+                offsets[(t + 3) & 3][lane] = max(at, (int64_t)0);
+                there[(t + 3) & 3][lane] = at >= 0;
+            }
         }
         if (tid == 0) bad[(t + 5) & 7] = odd[(t + 5) & 7] = 0;
         __syncthreads();
@@ -445,30 +489,45 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(
     }
 }
 
-template <typename T, typename S>
-int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
-                 hipStream_t st) {
+template <typename T, typename S, int D, int W, int kScores>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(Call a, Cache c, Stage prefix, Stage own) {
+    __shared__ TilesLds<T, S, D, W> lds;
+    attend_tiles<T, S, D, W, kScores>(a, c, prefix, own, (int)blockIdx.x, lds);
+}
+
+// Workgroups that a launch has for these stages: XCDs' shares are rounded up to whole turns.
+inline int64_t tiles_groups(const Call& a, const Stage& prefix, const Stage& own) {
     const int64_t items = (int64_t)prefix.blocks * prefix.splits + (int64_t)own.blocks * own.splits;
-    // See the kernel: XCDs' shares are rounded up to whole turns.
     const int64_t turns = a.kv_heads % 8 == 0   ? items * (a.kv_heads / 8)
                           : 8 % a.kv_heads == 0 ? (items + 8 / a.kv_heads - 1) / (8 / a.kv_heads)
                                                 : (items * a.kv_heads + 7) / 8;
-    const dim3 grid((unsigned)(turns * 8));
+    return turns * 8;
+}
+
+// f(scores) with the kind of scores that the call has, as a constant.
+template <typename F>
+void with_scores(const Call& a, F f) {
+    if (a.slopes) f(std::integral_constant<int, kBiased>());
+    else if (a.softcap > 0.f) f(std::integral_constant<int, kCapped>());
+    else f(std::integral_constant<int, kPlain>());
+}
+
+template <typename T, typename S>
+int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
+                 hipStream_t st) {
+    const dim3 grid((unsigned)tiles_groups(a, prefix, own));
     const auto go = [&](auto kernel, int w) {
         hipLaunchKernelGGL(kernel, grid, dim3(64 * w), 0, st, a, c, prefix, own);
     };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        const auto with = [&](auto scores) {
+        with_scores(a, [&](auto scores) {
             constexpr int kScores = decltype(scores)::value;
             if constexpr (D != 256) {
                 if (waves == 8) return go(attend_tiles_kernel<T, S, D, 8, kScores>, 8);
             }
             go(attend_tiles_kernel<T, S, D, 4, kScores>, 4);
-        };
-        if (a.slopes) with(std::integral_constant<int, kBiased>());
-        else if (a.softcap > 0.f) with(std::integral_constant<int, kCapped>());
-        else with(std::integral_constant<int, kPlain>());
+        });
     };
     if (dim == 64) pick(std::integral_constant<int, 64>());
     if (dim == 128) pick(std::integral_constant<int, 128>());

@@ -340,5 +340,10 @@ template <typename T, typename S>
 int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
                  hipStream_t st);
 
+// A prefix of many rows and few rows that follow (attend_both.h).
+template <typename T, typename S>
+int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+                hipStream_t st);
+
 }  // namespace kv
 }  // namespace gfd

@@ -10,7 +10,6 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
-#include <cstdlib>
 
 #include "capi_error.h"
 #include "gfd_capi.h"
@@ -31,10 +30,10 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
     typedef float Dims __attribute__((ext_vector_type(kDims)));
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int kv_head = (int)blockIdx.x % a.kv_heads, block = (int)blockIdx.x / a.kv_heads;
+    const int splits = a.block_splits[blockIdx.x], slots = own.first_slot + splits;  // unset without rows
+    if (own.direct && splits == 1) return;
     Block k;
     if (!find_rows<kRows>(a, own, block, &k)) return;
-    const int splits = a.block_splits[blockIdx.x], slots = own.first_slot + splits;
-    if (own.direct && splits == 1) return;
 
     const int first = (int)blockIdx.y * kPart;
     for (int r = first + wave; r < min(first + kPart, k.rows); r += kWaves) {
@@ -104,8 +103,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
 // below one round the shortest range, a tile per wave, counts.
 constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
-// Many rows: a workgroup fills a CU (or half of it), so two rounds of them do.
-const int kTilesFill = getenv("X_TFILL") ? atoi(getenv("X_TFILL")) : 512, kTilesMinChunk = getenv("X_TMIN") ? atoi(getenv("X_TMIN")) : 256, kW8 = getenv("X_W8") ? atoi(getenv("X_W8")) : 65536;
+// Many rows: a workgroup fills a CU, or half of it, and what ranges leave has to be joined, so blocks are split only to
+// fill the card once (64 requests on 32768 shared keys: ranges for 256 workgroups 92 us, for 512 101, for 128 129), and
+// not below 4 tiles.  Longer blocks are left whole: 4096 tokens of 64 dims take 112 us, in ranges of at most 1024 keys 186.
+constexpr int kTilesFill = 256, kTilesMinChunk = 256;
 
 void split(Stage* st, int64_t items, int64_t keys, bool few) {
     if (few) {
@@ -119,8 +120,9 @@ void split(Stage* st, int64_t items, int64_t keys, bool few) {
     st->splits = (int)std::max<int64_t>(1, ceil_div(keys, st->chunk));
 }
 
-// Waves of a block of many rows: 8 where that still fills the card, for half the reads of the cache.
-int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= kW8 ? 8 : 4; }
+// Waves of a block of many rows: 8, for half the reads of the cache, where that still gives every CU two blocks
+// (4096 tokens over 16384 keys: 950 us, with 4 waves 1077; 2048 tokens of 32 heads, one block each: 87 us, with 4 73).
+int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= 2 * 256 * 256 ? 8 : 4; }
 
 Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
     Plan p{};
@@ -144,7 +146,7 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
     p.own.direct = !prefix_len;
     if (prefix_len) {
         p.prefix.prefix = 1;
-        p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : tile_waves(all_rows, heads, cache.head_dim);
+        p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : 4;
         p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
         split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves);
         p.own.first_slot = p.prefix.splits;
@@ -172,13 +174,11 @@ int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
 
 template <typename T, typename S>
 int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st) {
-    const Stage none{0, 0, 0, 0, 1, 0, 0};
     int rc;
     if (p.own_waves) {  // both stages have blocks of the same rows
         rc = launch_tiles<T, S>(a, c, p.prefix, p.own, dim, p.own_waves, st);
     } else if (p.prefix_waves) {
-        rc = launch_tiles<T, S>(a, c, p.prefix, none, dim, p.prefix_waves, st);
-        if (!rc) rc = launch_rows<T, S>(a, c, none, p.own, dim, p.rows == 32, st);
+        rc = launch_both<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
     } else {
         rc = launch_rows<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
     }
