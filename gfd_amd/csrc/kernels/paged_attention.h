@@ -71,7 +71,7 @@ __device__ __forceinline__ Sequence sequence(const Call& a, int start, int end, 
     s.first = min(max(start, 0), a.num_tokens);
     s.q_len = min(max(end, s.first), a.num_tokens) - s.first;
     s.rows_q = min(s.q_len, a.max_q_len);
-    s.kv_len = min(kv_len, a.max_kv_len);
+    s.kv_len = max(min(kv_len, a.max_kv_len), 0);
     s.cut = s.q_len > a.max_q_len || kv_len > a.max_kv_len;
     return s;
 }

@@ -213,7 +213,8 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
         return "rows' pointers or strides are not multiples of 16 bytes";
     const int64_t pages = ((int64_t)std::max(w.max_kv_len - prefix_len, 0) + cache->page_size - 1) / cache->page_size;
     if (w.table_stride < pages) return "block_table's rows are shorter than max_kv_len needs";
-    if (make_plan(*cache, w, prefix_len).items > (1 << 28)) return "more work than one launch takes";
+    if ((int64_t)w.num_tokens * w.num_q_heads > (1 << 30) || make_plan(*cache, w, prefix_len).items > (1 << 28))
+        return "more work than one launch takes";
     return nullptr;
 }
 
@@ -234,7 +235,7 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     float* const splits = p.bytes ? part_ml + p.slots * rows * 2 : nullptr;
     const Call a{(const uint16_t*)w.q, (uint16_t*)w.out, w.lse, w.q_stride, w.out_stride, w.q_start, w.kv_len,
                  w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, w.scale,
-                 w.softcap, w.window, w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
+                 w.softcap, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
                  cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
     const Cache c = make_cache(*cache);

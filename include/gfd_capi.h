@@ -603,8 +603,11 @@ typedef struct gfd_attention {
 } gfd_attention;
 
 /* Workspace that the next two need for such a call (prefix_len 0: the first);
- * -1: the call would be refused.  It grows with num_tokens, max_kv_len and
- * batch, so that of a program's largest call is enough for all. */
+ * -1: the call would be refused.  It holds what ranges of keys leave to be
+ * joined, and depends on every size of the call (a batch that fills the card
+ * by itself needs none), so a program keeps the largest of its calls' values;
+ * a call that is given less is refused.  16-byte aligned; what it holds before
+ * and after a call does not matter, but calls that may run at the same time need one each. */
 int64_t gfd_attention_workspace_bytes(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len);
 int gfd_paged_attention(const gfd_kv_cache* cache, const gfd_attention* call, void* workspace,
                         size_t workspace_bytes, int* error_flag, void* stream);
