@@ -103,10 +103,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
 // below one round the shortest range, a tile per wave, counts.
 constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
-// Many rows: a workgroup fills a CU, or half of it, and what ranges leave has to be joined, so blocks are split only to
-// fill the card once (64 requests on 32768 shared keys: ranges for 256 workgroups 92 us, for 512 101, for 128 129), and
-// not below 4 tiles.  Longer blocks are left whole: 4096 tokens of 64 dims take 112 us, in ranges of at most 1024 keys 186.
-constexpr int kTilesFill = 256, kTilesMinChunk = 256;
+// Many rows: what ranges leave has to be joined, so blocks are split only where they leave half of the CUs empty,
+// and not below 4 tiles.  Then two workgroups a CU (4 times 60 tokens over 4000 keys: 33 us, with one 36; 1000
+// tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
+// of the CUs one (64 requests on 32768 shared keys: 92 us, with two 101).
+constexpr int kCus = 256, kTilesMinChunk = 256;
 
 void split(Stage* st, int64_t items, int64_t keys, bool few) {
     if (few) {
@@ -114,7 +115,8 @@ void split(Stage* st, int64_t items, int64_t keys, bool few) {
         const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(kRound)));
         st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max(least, chunk_for(kRound * kRounds)));
     } else {
-        const int64_t parts = std::max<int64_t>(1, kTilesFill / std::max<int64_t>(items, 1));
+        const int64_t fill = st->prefix ? kCus : 2 * kCus;
+        const int64_t parts = items * 2 > kCus ? 1 : fill / std::max<int64_t>(items, 1);
         st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
     }
     st->splits = (int)std::max<int64_t>(1, ceil_div(keys, st->chunk));
@@ -166,10 +168,13 @@ int launch_join(const Call& a, const Cache& c, const Stage& own, hipStream_t st)
 }
 template <typename T, int D>
 int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
-    return p.rows == 16    ? launch_join<T, D, 16, 4>(a, c, p.own, st)
-           : p.rows == 32  ? launch_join<T, D, 32, 4>(a, c, p.own, st)
-           : p.rows == 128 ? launch_join<T, D, 128, 16>(a, c, p.own, st)
-                           : launch_join<T, D, 256, 16>(a, c, p.own, st);
+    // A wave a row takes the least time where few rows leave the card empty (100 tokens over 4196 keys: 33 us in all,
+    // with four rows a wave 38); with many it does not matter.
+    const bool few = (int64_t)p.own.blocks * p.rows * a.kv_heads <= 16384;
+    if (p.rows == 16) return launch_join<T, D, 16, 4>(a, c, p.own, st);
+    if (p.rows == 32) return launch_join<T, D, 32, 4>(a, c, p.own, st);
+    if (p.rows == 128) return few ? launch_join<T, D, 128, 4>(a, c, p.own, st) : launch_join<T, D, 128, 16>(a, c, p.own, st);
+    return few ? launch_join<T, D, 256, 4>(a, c, p.own, st) : launch_join<T, D, 256, 16>(a, c, p.own, st);
 }
 
 template <typename T, typename S>
