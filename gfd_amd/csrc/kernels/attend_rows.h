@@ -3,24 +3,53 @@
 //
 // Up to 16 or 32 rows share a head's keys and values, so each byte is used for
 // at most 32 rows and the cache's bytes bound the time.  What counts is loads in
-// flight: the waves of a workgroup take tiles of 32 keys by turns, straight
-// from memory to registers and without waiting for one another, the next
-// tile's keys under way during a tile's softmax and its values during the next
-// scores.  A long axis is split over workgroups.
+// flight: the waves of a workgroup take tiles of 32 keys by turns and without
+// waiting for one another, the next tile's keys under way during a tile's
+// softmax and its values during the next scores.  A long axis is split over workgroups.
 //
 // A tile: scores^T[32 keys][16 rows] by 16x16x32 products, keys as the left operand
-// (lane: key l % 16, 8 dims of a 32, by l / 16), for which they pass through the wave's own LDS.  Result: lane holds row l % 16 and the keys
-// 4 (l / 16) + r of both halves.  As the right operand of out^T += V^T P the
-// lane has to hold 8 keys of a 32, and which 8 is free as long as the values agree: so it
-// keeps its own, and loads the values of those 8 keys, D / 16 adjacent
-// dims each (a row of D by 16 lanes).  Left operand i takes dim i of every lane: two
-// neighbouring keys' halves joined by a byte permutation, no LDS.
+// (lane: key l % 16, 8 dims of a 32, by l / 16), for which they pass through the
+// wave's own LDS: whole rows come from memory faster than the operand's 64-byte
+// pieces (64 ragged contexts of up to 8192 keys: 182 us for 191).  The result's lane holds row
+// l % 16 and the keys 4 (l / 16) + r of both halves.  As the right operand of out^T += V^T P
+// the lane has to hold 8 keys of a 32, and which 8 is free as long as the values
+// agree: so it keeps its own, and loads the values of those 8 keys, D / 16
+// adjacent dims each (a row of D by 16 lanes).  Left operand i takes dim i of every
+// lane: two neighbouring keys' halves joined by a byte permutation, no LDS.
+//
+// Nothing is read twice, and loads say so (nontemporal: 64 x 8192 keys 361 us for 390).  Spills would
+// undo it, a reload waits for every load: two waves a SIMD without spills take 165 us
+// where three with eight of them take 187.
+//
+// 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 371 us, 5.8 TB/s (a large read: 6.2).
+// 64 ragged contexts of up to 8192: 161 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
+// capped: 61 us, 4.8 TB/s.  700 keys of one token: 7.4 us and 3.4 to join, a chain of loads
+// (lengths, pages, keys) and a launch each.
 #include "paged_attention.h"
 
 namespace gfd {
 namespace kv {
 
 constexpr int kRowsBlock = 256, kRowsTile = 32;
+
+// Scores get the exponent's base 2.  Without cap and bias they stay the product's raw
+// sums: the factor is positive, so the maximum is the same, and one multiply-add
+// under the exponent applies it.
+struct Score {
+    float factor;   // raw -> exponent
+    float in, cap;  // with a cap: cap * tanh(raw * in)
+    float slope;
+};
+
+// tanh(y) = 1 - 2 / (e^2y + 1): off by a few 2^-24 of 1, as the sums are.
+__device__ __forceinline__ float capped(float y) {
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
+}
+
+__device__ __forceinline__ float score(const Score& s, bool cap, float raw, int pos, int key) {
+    const float x = cap ? s.cap * capped(raw * s.in) : raw * s.factor;
+    return __builtin_fmaf(-s.slope, fabsf((float)(pos - key)), x);
+}
 
 template <int N>
 struct Words {
@@ -276,8 +305,8 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             if (extras) {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    x[i][j >> 2][j & 3] = score<true>(sc[i], a, x[i][j >> 2][j & 3], row[i].pos,
-                                                      n0 + 16 * (j >> 2) + 4 * quarter + (j & 3));
+                    x[i][j >> 2][j & 3] = score(sc[i], a.softcap > 0.f, x[i][j >> 2][j & 3], row[i].pos,
+                                                n0 + 16 * (j >> 2) + 4 * quarter + (j & 3));
             }
             if (!whole) {
 #pragma unroll

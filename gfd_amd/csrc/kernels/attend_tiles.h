@@ -12,7 +12,16 @@
 // The result's lane holds row l % 32 and the keys 8 (r / 4) + 4 (l / 32) + r % 4;
 // eight of these, rounded, are the right operand of out^T[32 dims][32 rows] += V^T P
 // as they lie.  V^T comes from LDS by transposing reads, 4 keys of one dim a lane.
-// Chunks of 16 bytes are swapped by row, so that neither read finds two rows in a bank.
+// Chunks of 16 bytes are swapped by row, so that neither read finds two rows in a bank
+// (with a swap by 8 rows, 43% of the LDS's cycles were conflicts).
+//
+// 4096 tokens over 16384 keys, 32 heads of 128 in bf16: 945 us, 1020 TFLOP/s, where a library product of
+// 8192^3 reaches 1186 (the card's power holds both: 1.9 GHz with the matrix pipes at 45%,
+// and 1.6 to 1.9 GHz at 70%).  8192 packed tokens with capped scores: 211 us, 485 TFLOP/s; a cap costs
+// two more transcendental instructions a score, and the longest document's blocks end last.
+// 7 ragged prompts of 64 dims with a bias: 55 us, the 30 tiles of the longest one by 4 waves.
+// Tried and slower: half of the waves a product behind the others (1130 us for 1096), tiles of 32 keys with
+// three under way (2048 tokens 85 us for 74), two groups of 4 waves to a block (packed tokens 263 us for 223).
 #include <type_traits>
 
 #include "paged_attention.h"
@@ -44,7 +53,8 @@ struct TilesKernel {
     static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 
     // kc and vc: the thread's chunk of the cache's first row.
-    static __device__ __forceinline__ void load(Staged& g, const uint8_t* kc, const uint8_t* vc, const int64_t* off, int tid) {
+    static __device__ __forceinline__ void load(Staged& g, const uint8_t* kc, const uint8_t* vc, const int64_t* off,
+                                                int tid) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             const int64_t o = off[tid / kChunks + u * kStride];
@@ -250,7 +260,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     }
     const uint8_t* const kc = c.k + tid % K::kChunks * 8 * S::kBytes;
     const uint8_t* const vc = c.v + tid % K::kChunks * 8 * S::kBytes;
-    const auto keep = [&](const typename K::Staged& x, int t) {  // tile t to LDS
+    const auto place = [&](const typename K::Staged& x, int t) {  // tile t to LDS
         const int n0 = c0 + t * kTile;
         const bool full = n0 + kTile <= c1 && !bad[t & 7];
         if (K::store(x, (uint16_t*)keys_lds[t & 1], (uint16_t*)values_lds[t & 1], tid, full ? nullptr : there[t & 3],
@@ -261,7 +271,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     if (tiles > 0) {
         K::load(staged[0], kc, vc, offsets[0], tid);
         if constexpr (kAhead == 2) K::load(staged[1], kc, vc, offsets[1], tid);
-        keep(staged[0], 0);
+        place(staged[0], 0);
     }
     __syncthreads();
 
@@ -271,7 +281,8 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     int value_at[K::kDims];
 #pragma unroll
     for (int i = 0; i < K::kDims; i++)
-        value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap_v(v_row)) * 8 + (lane16 & 1) * 4;
+        value_at[i] = v_row * D + ((4 * i + 2 * ((lane >> 4) & 1) + ((lane16 & 3) >> 1)) ^ K::swap_v(v_row)) * 8 +
+                      (lane16 & 1) * 4;
 
     // A tile: later ones' loads start, in the order of their use and whether or not there are such tiles (offsets
     // past the end are 0, which reads the cache's start), so that each wait is for the oldest loads only.
@@ -279,10 +290,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
         const int n0 = c0 + t * kTile;
         const bool more = t + 1 < tiles;
         // The pages of the tile after those, by the first wave's lanes.
-        const int n3 = n0 + 3 * kTile + (lane & (kTile - 1));
+        const int n_look = n0 + 3 * kTile + (lane & (kTile - 1));
         const auto page_of = [&](int n) { return c.page.div((uint32_t)min(n, c1 - 1)); };
-        int id3 = 0;
-        if (wave == 0) id3 = k.table[page_of(n3)];
+        int id_look = 0;
+        if (wave == 0) id_look = k.table[page_of(n_look)];
         K::load(later, kc, vc, offsets[(t + kAhead) & 3], tid);
 
         if (odd[t & 7]) {
@@ -427,15 +438,15 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
                     }
         }
 
-        if (more) keep(next, t + 1);
+        if (more) place(next, t + 1);
         if (wave == 0) {
             int64_t at = -1;
-            if (n3 < c1) {
-                if (id3 < 0 || id3 >= c.num_pages) {
+            if (n_look < c1) {
+                if (id_look < 0 || id_look >= c.num_pages) {
                     bad[(t + 3) & 7] = 1;
                     if (a.error) atomicOr(a.error, GFD_KV_ERR_PAGE);
                 } else {
-                    at = id3 * c.page_stride + (int64_t)((uint32_t)n3 - page_of(n3) * c.page.d) * c.slot_stride + head;
+                    at = id_look * c.page_stride + (int64_t)((uint32_t)n_look - page_of(n_look) * c.page.d) * c.slot_stride + head;
                 }
             }
             if (lane < kTile) {

@@ -14,7 +14,6 @@
 namespace gfd {
 namespace kv {
 
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -233,28 +232,6 @@ __device__ __forceinline__ int64_t key_offset(const Cache& c, const int* table, 
 
 __device__ __forceinline__ int64_t slot_of(const Call& a, int slot, int t, int h) {
     return ((int64_t)slot * a.num_tokens + t) * a.q_heads + h;
-}
-
-// Scores in the exponent's units (base 2).  Without cap and bias they stay the
-// product's raw sums: the factor is positive, so the maximum is the same, and
-// one multiply-add under the exponent applies it.
-struct Score {
-    float factor;    // raw -> exponent
-    float in, cap;   // with a cap: cap * tanh(raw * in)
-    float slope;
-    bool extras;
-};
-
-// tanh(y) = 1 - 2 / (e^2y + 1): off by a few 2^-24 of 1, as the sums are.
-__device__ __forceinline__ float capped(float y) {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
-}
-
-template <bool kExtras>
-__device__ __forceinline__ float score(const Score& s, const Call& a, float raw, int pos, int key) {
-    if (!kExtras) return raw;
-    float x = a.softcap > 0.f ? s.cap * capped(raw * s.in) : raw * s.factor;
-    return __builtin_fmaf(-s.slope, fabsf((float)(pos - key)), x);
 }
 
 __device__ __forceinline__ float max_f32(float a, float b) { return __builtin_elementwise_maximum(a, b); }
