@@ -3,6 +3,6 @@
 #include "attend_tiles.h"
 
 template int gfd::kv::launch_rows<gfd::kv::Bf16, gfd::kv::E4m3>(const Call&, const Cache&, const Stage&, const Stage&, int,
-                                                          bool, hipStream_t);
+                                                          bool, int, hipStream_t);
 template int gfd::kv::launch_tiles<gfd::kv::Bf16, gfd::kv::E4m3>(const Call&, const Cache&, const Stage&, const Stage&, int,
                                                            int, hipStream_t);

@@ -11,19 +11,19 @@ namespace gfd {
 namespace kv {
 
 template <typename T, typename S, int D, int R, int kScores>
-__global__ __launch_bounds__(kRowsBlock, D == 256 ? 1 : 2) void attend_both_kernel(Call a, Cache c, Stage prefix,
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call a, Cache c, Stage prefix,
                                                                                   Stage own, int prefix_turns) {
     __shared__ union Lds {
-        RowsLds<T, S, D, R> rows;
+        RowsLds<T, S, D, R, 4> rows;
         TilesLds<T, S, D, 4> tiles;
     } lds;
-    static_assert(TilesKernel<T, S, D, 4>::kThreads == kRowsBlock, "both bodies have the same workgroups");
+    static_assert(TilesKernel<T, S, D, 4>::kThreads == 256, "both bodies have the same workgroups");
     // Turns of 8 workgroups, one for each XCD; the long ones first.
     const int xcd = (int)blockIdx.x & 7, turn = (int)blockIdx.x >> 3;
     const Stage none{0, 0, 0, 0, 1, 0, 0};
     if (turn >= prefix_turns) {
         const int item = (turn - prefix_turns) * 8 + xcd;
-        if (item < own.blocks * own.splits * a.kv_heads) attend_rows<T, S, D, R>(a, c, none, own, item, lds.rows);
+        if (item < own.blocks * own.splits * a.kv_heads) attend_rows<T, S, D, R, 4>(a, c, none, own, item, lds.rows);
     } else {
         attend_tiles<T, S, D, 4, kScores>(a, c, prefix, none, turn * 8 + xcd, lds.tiles);
     }
@@ -36,7 +36,7 @@ int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage&
     const int prefix_turns = (int)(tiles_groups(a, prefix, none) / 8),
               own_turns = (int)(((int64_t)own.blocks * own.splits * a.kv_heads + 7) / 8);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * (prefix_turns + own_turns))), dim3(kRowsBlock), 0, st, a, c,
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * (prefix_turns + own_turns))), dim3(256), 0, st, a, c,
                            prefix, own, prefix_turns);
     };
     const auto pick = [&](auto d) {

@@ -24,13 +24,15 @@
 // 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 371 us, 5.8 TB/s (a large read: 6.2).
 // 64 ragged contexts of up to 8192: 161 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
 // capped: 61 us, 4.8 TB/s.  700 keys of one token: 7.4 us and 3.4 to join, a chain of loads
-// (lengths, pages, keys) and a launch each.
+// (lengths, pages, keys) and a launch each.  Many short contexts take a wave each: 128 of 128 keys in 16 us, 4.2 TB/s.
+#include <type_traits>
+
 #include "paged_attention.h"
 
 namespace gfd {
 namespace kv {
 
-constexpr int kRowsBlock = 256, kRowsTile = 32;
+constexpr int kRowsTile = 32;
 
 // Scores get the exponent's base 2.  Without cap and bias they stay the product's raw
 // sums: the factor is positive, so the maximum is the same, and one multiply-add
@@ -161,26 +163,26 @@ struct RowsKernel {
     }
 };
 
-template <typename T, typename S, int D, int R>
+template <typename T, typename S, int D, int R, int kWaves>
 struct RowsLds {
     using K = RowsKernel<T, S, D, R>;
-    static constexpr int kWaves = kRowsBlock / 64;
     i32x4 rows[16 * R];
-    int64_t offsets[kRowsMaxChunk];
+    int64_t offsets[kWaves == 1 ? kRowsShort : kRowsMaxChunk];
     union {
         int samples[kSamples + 1];
-        float merge[kWaves / 2][R * K::kAcc + 2 * R][64];
+        float merge[kWaves == 1 ? 1 : kWaves / 2][kWaves == 1 ? 1 : R * K::kAcc + 2 * R][64];
         u32x4 keys[kWaves][kRowsTile * K::kKeyChunks];
     };
     u32x4 queries[K::kLdsRows ? R * K::kSteps : 1][64];
     int any_bad;
 };
 
-template <typename T, typename S, int D, int R>
+// kWaves 1: ranges of at most kRowsShort keys.
+template <typename T, typename S, int D, int R, int kWaves>
 __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int item,
-                                            RowsLds<T, S, D, R>& lds) {
+                                            RowsLds<T, S, D, R, kWaves>& lds) {
     using K = RowsKernel<T, S, D, R>;
-    constexpr int kRows = 16 * R, kWaves = kRowsBlock / 64;
+    constexpr int kRows = 16 * R, kThreads = 64 * kWaves;
     // Heads vary fastest: their keys lie side by side.  Ranges vary slowest: the last ones are often empty.
     const int prefix_items = prefix.blocks * prefix.splits * a.kv_heads;
     const Stage st = item < prefix_items ? prefix : own;
@@ -195,7 +197,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     Block k;
     if (!find_rows<kRows>(a, st, block, &k)) return;
     if (st.prefix) {
-        sample_starts(a, lds.samples, kRowsBlock);
+        sample_starts(a, lds.samples, kThreads);
         __syncthreads();
     }
     Range g{0x7FFFFFFF, 0, 0, 0x7FFFFFFF};
@@ -224,7 +226,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     const int c0 = max(base, g.lo), c1 = min(base + st.chunk, g.hi);
     const int64_t head = kv_head * c.head_stride;
     const int tiles = c1 > c0 ? (c1 - c0 + kRowsTile - 1) / kRowsTile : 0;
-    for (int n = tid; n < tiles * kRowsTile; n += kRowsBlock) {
+    for (int n = tid; n < tiles * kRowsTile; n += kThreads) {
         const int64_t o = c0 + n < c1 ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
         if (o < 0 && c0 + n < c1) lds.any_bad = 1;
         lds.offsets[n] = o;
@@ -460,21 +462,26 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     }
 }
 
-template <typename T, typename S, int D, int R>
-__global__ __launch_bounds__(kRowsBlock, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(
+template <typename T, typename S, int D, int R, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(
     Call a, Cache c, Stage prefix, Stage own) {
-    __shared__ RowsLds<T, S, D, R> lds;
-    attend_rows<T, S, D, R>(a, c, prefix, own, (int)blockIdx.x, lds);
+    __shared__ RowsLds<T, S, D, R, kWaves> lds;
+    attend_rows<T, S, D, R, kWaves>(a, c, prefix, own, (int)blockIdx.x, lds);
 }
 
 template <typename T, typename S>
-int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st) {
     const dim3 grid((unsigned)((prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads));
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kRowsBlock), 0, st, a, c, prefix, own); };
-    if (dim == 64) wide ? go(attend_rows_kernel<T, S, 64, 2>) : go(attend_rows_kernel<T, S, 64, 1>);
-    if (dim == 128) wide ? go(attend_rows_kernel<T, S, 128, 2>) : go(attend_rows_kernel<T, S, 128, 1>);
-    if (dim == 256) wide ? go(attend_rows_kernel<T, S, 256, 2>) : go(attend_rows_kernel<T, S, 256, 1>);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, c, prefix, own); };
+    const auto pick = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (waves == 1) wide ? go(attend_rows_kernel<T, S, D, 2, 1>) : go(attend_rows_kernel<T, S, D, 1, 1>);
+        else wide ? go(attend_rows_kernel<T, S, D, 2, 4>) : go(attend_rows_kernel<T, S, D, 1, 4>);
+    };
+    if (dim == 64) pick(std::integral_constant<int, 64>());
+    if (dim == 128) pick(std::integral_constant<int, 128>());
+    if (dim == 256) pick(std::integral_constant<int, 256>());
     return (int)hipGetLastError();
 }
 

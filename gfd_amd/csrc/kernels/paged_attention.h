@@ -309,8 +309,9 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
 
 // Few rows (attend_rows.h): a range has at most so many keys.
 constexpr int kRowsMaxChunk = 1024;
+constexpr int kRowsShort = 128;  // with one wave
 template <typename T, typename S>
-int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st);
 // Many rows (attend_tiles.h).
 template <typename T, typename S>

@@ -89,6 +89,7 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
 // How a call is cut into row blocks and key ranges.
 struct Plan {
     int prefix_waves, own_waves;  // of a block of 32 rows a wave; 0: few rows (attend_rows.h)
+    int few_waves;                // of a workgroup of few rows
     int rows;                     // of an own-keys block
     Stage prefix, own;
     int slots;      // partial results per row
@@ -103,6 +104,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
 // below one round the shortest range, a tile per wave, counts.
 constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
+// From so many workgroups on (one round of four waves), short contexts get a wave each: of four waves most would
+// find no tile or one, and what takes the time is a workgroup's start (91 times 12 heads of 256 dims and 27 keys:
+// 46 us, with one wave 17; 70 times 8 heads of 128 dims and 128 keys: 15.2, 12.7).
+constexpr int kOneWave = 512;
 // Many rows: what ranges leave has to be joined, so blocks are split only where they leave half of the CUs empty,
 // and not below 4 tiles.  Then two workgroups a CU (4 times 60 tokens over 4000 keys: 33 us, with one 36; 1000
 // tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
@@ -147,6 +152,12 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.own.blocks = (int)std::min<int64_t>(w.batch * ceil_div(seq_rows, p.rows), all_rows / p.rows + w.batch);
     }
     split(&p.own, p.own.blocks * heads, keys, !p.own_waves);
+    p.few_waves = 4;
+    if (!p.own_waves && !prefix_len && keys <= kRowsShort && p.own.blocks * heads >= kOneWave) {
+        p.few_waves = 1;
+        p.own.chunk = kRowsShort;
+        p.own.splits = 1;
+    }
     p.own.direct = !prefix_len;
     if (prefix_len) {
         p.prefix.prefix = 1;
@@ -187,7 +198,7 @@ int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st
     } else if (p.prefix_waves) {
         rc = launch_both<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
     } else {
-        rc = launch_rows<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
+        rc = launch_rows<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, p.few_waves, st);
     }
     if (rc || p.slots == 1) return rc;
     return dim == 64 ? launch_join<T, 64>(a, c, p, st) : dim == 128 ? launch_join<T, 128>(a, c, p, st)

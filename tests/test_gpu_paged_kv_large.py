@@ -71,6 +71,35 @@ def test_a_prefix_for_more_sequences_than_starts_are_sampled(batch):
     case(54, q, kv, prefix=20, hq=4, hk=2, d=64, page=8)
 
 
+@pytest.mark.parametrize("opts", [dict(), dict(softcap=5.0, slopes=True), dict(window=19)], ids=str)
+@pytest.mark.parametrize("d,dtype,cache", [(64, FP16, None), (128, BF16, None), (128, BF16, E4M3), (256, BF16, None),
+                                           (256, FP16, E4M3)])
+@pytest.mark.parametrize("q", [1, 3])  # 16 and 32 rows of a wave
+def test_many_short_contexts(q, d, dtype, cache, opts):
+    rng = np.random.default_rng(64)
+    q_lens = rng.integers(0, q + 1, 260).tolist()
+    kv = rng.integers(0, 129, 260).tolist()
+    kv[:6] = [1, 31, 32, 33, 128, 0]
+    assert max(q_lens) == q and len(kv) * 2 >= 512  # enough for a wave each
+    case(65, q_lens, kv, hq=12, hk=2, d=d, dtype=dtype, cache=cache, **opts)
+
+
+@pytest.mark.parametrize("bits", [0x7FC0, 0x7F80])
+def test_values_that_are_no_numbers_in_many_short_contexts(bits):
+    rng = np.random.default_rng(66)
+    q, kv = [2] * 256, [50] * 256
+    pages = ref.Pages(rng, kv, 16, 2, 128, BF16)
+    for b in range(0, 256, 2):  # the last key: the second token sees it, the first does not
+        pages.view(pages.table[b, 49 // 16], 49 % 16, pages.v_offset)[:, 3] = bits
+    a = Attend(rng, pages, q, kv, 8, BF16)
+    want, _, tol, _ = ref.attention64(a.q, pages, ref.intervals(q, kv), BF16, a.scale)
+    out, _ = a.run()
+    odd = np.zeros(out.shape, bool)
+    odd[1::4, :, 3] = True
+    close(out[~odd], want[~odd], tol[~odd], "what sees none")
+    assert np.isnan(out[odd]).all() if bits == 0x7FC0 else (out[odd] == np.inf).all()
+
+
 @pytest.mark.parametrize("q,kv", [([70], [5000]), ([40, 1, 33], [2900, 3000, 33])], ids=str)
 @pytest.mark.parametrize("dtype,cache", [(BF16, None), (BF16, E4M3)])
 @pytest.mark.parametrize("d", [64, 256])
