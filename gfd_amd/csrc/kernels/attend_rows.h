@@ -34,25 +34,6 @@ namespace kv {
 
 constexpr int kRowsTile = 32;
 
-// Scores get the exponent's base 2.  Without cap and bias they stay the product's raw
-// sums: the factor is positive, so the maximum is the same, and one multiply-add
-// under the exponent applies it.
-struct Score {
-    float factor;   // raw -> exponent
-    float in, cap;  // with a cap: cap * tanh(raw * in)
-    float slope;
-};
-
-// tanh(y) = 1 - 2 / (e^2y + 1): off by a few 2^-24 of 1, as the sums are.
-__device__ __forceinline__ float capped(float y) {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
-}
-
-__device__ __forceinline__ float score(const Score& s, bool cap, float raw, int pos, int key) {
-    const float x = cap ? s.cap * capped(raw * s.in) : raw * s.factor;
-    return __builtin_fmaf(-s.slope, fabsf((float)(pos - key)), x);
-}
-
 template <int N>
 struct Words {
     uint32_t w[N];
@@ -234,9 +215,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 
     // The rows' operand, zero where there is no row.
     u32x4 q[K::kLdsRows ? 1 : R][K::kSteps];
-    Score sc[R];
-    const float raw = a.scale * c.k_scale;
-    const bool extras = a.softcap > 0.f || a.slopes;
+    // Scores stay in units of the product's sums, also capped and biased: the factor to the exponent of base 2 is
+    // positive, so the maximum is the same, and one multiply-add under the exponent applies it.
+    const float factor = a.raw * kLog2e;
+    float slope[R];
     for (int i = 0; i < R; i++) {
         const int h = head_of(a, k, 16 * i + col, kv_head);
         const uint16_t* p = a.q + row[i].t * a.q_stride + (int64_t)h * D;
@@ -246,12 +228,8 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             if constexpr (K::kLdsRows) lds.queries[i * K::kSteps + s][lane] = x;
             else q[i][s] = x;
         }
-        sc[i].factor = raw * kLog2e;
-        sc[i].in = a.softcap > 0.f ? raw / a.softcap : 0.f;
-        sc[i].cap = a.softcap * kLog2e;
-        sc[i].slope = a.slopes && row[i].t >= 0 ? a.slopes[h] * kLog2e : 0.f;
+        slope[i] = a.slopes && row[i].t >= 0 ? a.slopes[h] / a.raw : 0.f;
     }
-    const float factor = extras ? 1.f : raw * kLog2e;
 
     __syncthreads();
     const bool bad = lds.any_bad != 0;
@@ -304,11 +282,26 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         u32x4 p[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            if (extras) {
+            if (a.cap_in >= 0.f) {
+                float most = fabsf(x[i][0][0]);
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    x[i][j >> 2][j & 3] = score(sc[i], a.softcap > 0.f, x[i][j >> 2][j & 3], row[i].pos,
-                                                n0 + 16 * (j >> 2) + 4 * quarter + (j & 3));
+                for (int j = 1; j < 8; j++) most = max_f32(most, fabsf(x[i][j >> 2][j & 3]));
+                if (__any(!(most * a.cap_in <= kCapNear))) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        x[i][j >> 2][j & 3] = capped(x[i][j >> 2][j & 3], a.cap_in, a.cap_out);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[i][j >> 2][j & 3] = capped_near(x[i][j >> 2][j & 3], a.cap_in);
+                }
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int n = n0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
+                    x[i][j >> 2][j & 3] =
+                        __builtin_fmaf(-slope[i], fabsf((float)(row[i].pos - n)), x[i][j >> 2][j & 3]);
+                }
             }
             if (!whole) {
 #pragma unroll

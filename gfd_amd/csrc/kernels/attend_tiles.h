@@ -18,7 +18,7 @@
 // 4096 tokens over 16384 keys, 32 heads of 128 in bf16: 945 us, 1020 TFLOP/s, where a library product of
 // 8192^3 reaches 1186 (the card's power holds both: 1.9 GHz with the matrix pipes at 45%,
 // and 1.6 to 1.9 GHz at 70%).  8192 packed tokens with capped scores: 211 us, 485 TFLOP/s; a cap costs
-// two more transcendental instructions a score, and the longest document's blocks end last.
+// ten more instructions a score, and the longest document's blocks end last.
 // 7 ragged prompts of 64 dims with a bias: 55 us, the 30 tiles of the longest one by 4 waves.
 // Tried and slower: half of the waves a product behind the others (1130 us for 1096), tiles of 32 keys with
 // three under way (2048 tokens 85 us for 74), two groups of 4 waves to a block (packed tokens 263 us for 223).
@@ -227,15 +227,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
 #pragma unroll
         for (int s = 0; s < K::kSteps; s++) q[s] = row.t >= 0 ? *(const u32x4*)(p + 16 * s) : u32x4{0, 0, 0, 0};
     }
-    // Exponents have base 2.  Plain scores stay the product's sums: the factor is positive, so the
-    // maximum is the same, and one multiply-add under the exponent applies it.  Capped ones,
-    // cap tanh y = cap - 2 cap / (e^2y + 1), stay -1 / (e^2y + 1): off by a few 2^-24 as the sums are.
-    const float raw = a.scale * c.k_scale, cap = a.softcap * kLog2e;
-    const float into_cap = a.softcap > 0.f ? raw / a.softcap * (2.f * kLog2e) : 0.f;
-    const float factor = a.softcap > 0.f && kScores != kPlain ? 2.f * cap : raw * kLog2e;
-    const float shift = kScores == kPlain ? 0.f : cap;
-    // A bias in the scores' units: the sums of the product start from it, or it is added to what a cap leaves.
-    slope *= kLog2e / factor;
+    // Scores stay in units of the product's sums, also capped and biased: the factor to the exponent of base 2 is
+    // positive, so the maximum is the same, and one multiply-add under the exponent applies it.
+    const float factor = a.raw * kLog2e;
+    slope /= a.raw;
     const int least_pos = kScores == kBiased ? lanes_min(my_row().t >= 0 ? pos : 0x7FFFFFFF) : 0;
     const int last_pos = kScores == kBiased ? -lanes_min(my_row().t >= 0 ? -pos : 0x7FFFFFFF) : 0;
     // A maximum that has grown by less than 2^8 is left as it is: weights and sums stay far from
@@ -349,7 +344,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
                         }
                 }
             };
-            if (kScores == kBiased && !(a.softcap > 0.f)) {
+            if (kScores == kBiased && a.cap_in < 0.f) {
                 add_bias(std::true_type());
             } else {
 #pragma unroll
@@ -370,12 +365,23 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
             __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
-            if (kScores == kCapped || (kScores == kBiased && a.softcap > 0.f)) {
+            if (kScores == kCapped || (kScores == kBiased && a.cap_in >= 0.f)) {
+                float most = fabsf(x[0][0]);
 #pragma unroll
                 for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        x[i][r] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x[i][r] * into_cap));
+                    for (int r = 0; r < 16; r++) most = max_f32(most, fabsf(x[i][r]));
+                if (__any(!(most * a.cap_in <= kCapNear))) {
+#pragma unroll
+                    for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[i][r] = capped(x[i][r], a.cap_in, a.cap_out);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K::kHalves; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) x[i][r] = capped_near(x[i][r], a.cap_in);
+                }
                 if (kScores == kBiased) add_bias(std::false_type());
             }
             const bool gap = bad[t & 7];
@@ -486,10 +492,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
             }
         if (a.lse && hi == 0)
             a.lse[(int64_t)row.t * a.q_heads + h] =
-                sum == 0.f ? -INFINITY : (m * factor + shift + __builtin_amdgcn_logf(sum)) * kLn2;
+                sum == 0.f ? -INFINITY : (m * factor + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
         const int64_t at = slot_of(a, st.first_slot + split, row.t, h);
-        if (hi == 0) a.part_ml[at] = f32x2{m == -INFINITY ? m : m * factor + shift, sum};
+        if (hi == 0) a.part_ml[at] = f32x2{m == -INFINITY ? m : m * factor, sum};
         if (sum == 0.f) return;  // its weight is zero and it is not read
         float* out = a.part_o + at * D + 4 * hi;
 #pragma unroll
@@ -519,7 +525,7 @@ inline int64_t tiles_groups(const Call& a, const Stage& prefix, const Stage& own
 template <typename F>
 void with_scores(const Call& a, F f) {
     if (a.slopes) f(std::integral_constant<int, kBiased>());
-    else if (a.softcap > 0.f) f(std::integral_constant<int, kCapped>());
+    else if (a.cap_in >= 0.f) f(std::integral_constant<int, kCapped>());
     else f(std::integral_constant<int, kPlain>());
 }
 

@@ -31,7 +31,8 @@ struct Call {
     const int* doc_start;
     const int* prefix_end;
     const float* slopes;
-    float scale, softcap;
+    float raw;                // scale * k_scale: a score is this times the product of q and the stored key
+    float cap_in, cap_out;    // softcap > 0: raw / softcap and softcap / raw; cap_in < 0: no cap
     int window, batch, num_tokens, max_q_len, max_kv_len, q_heads, kv_heads;
     Divider group;
     int* error;
@@ -252,6 +253,26 @@ __device__ __forceinline__ float across16_max(float x) {
 __device__ __forceinline__ float across16_sum(float x) {
     const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return across32_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+}
+
+// softcap tanh(s / softcap) in units of the products' sums x, y = x cap_in.  Where |y| <= kCapNear: x (1 + z P(z)),
+// z = y^2, off by 2 2^-24 of itself however large the cap (P: a least-maximum fit of tanh(y) / y there, off by 0.6 2^-24).
+// 1 - 2 / (e^2y + 1), which loses what is small, is for the others, off by 4 2^-24 of itself.
+// The first form is also the shorter one, and a tile's scores take it together where all of them may.
+constexpr float kCapNear = 0.75f;
+__device__ __forceinline__ float capped_near(float x, float cap_in) {
+    const float y = x * cap_in, z = y * y;
+    float p = -4.769478459e-03f;
+    p = __builtin_fmaf(p, z, 1.966489665e-02f);
+    p = __builtin_fmaf(p, z, -5.339024961e-02f);
+    p = __builtin_fmaf(p, z, 1.332652122e-01f);
+    p = __builtin_fmaf(p, z, -3.333306909e-01f);
+    return __builtin_fmaf(x * z, p, x);
+}
+__device__ __forceinline__ float capped(float x, float cap_in, float cap_out) {
+    const float y = x * cap_in;
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
+    return fabsf(y) <= kCapNear ? capped_near(x, cap_in) : far * cap_out;
 }
 
 // Matrix instructions by element type, and tests on packed pairs.

@@ -251,12 +251,17 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     float* const part_o = p.bytes ? (float*)workspace : nullptr;
     float* const part_ml = p.bytes ? part_o + p.slots * rows * cache->head_dim : nullptr;
     float* const splits = p.bytes ? part_ml + p.slots * rows * 2 : nullptr;
+    const Cache c = make_cache(*cache);
+    const float raw = w.scale * c.k_scale;
+    // Of a cap past what 32 bits hold of it, the quotients' ends: scores far below it stay as they are, others are +-cap_out.
+    const auto held = [](double x) { return (float)std::min(x, 3.4028234e38); };
+    const float cap_in = w.softcap > 0.f ? held((double)raw / w.softcap) : -1.f;
+    const float cap_out = w.softcap > 0.f ? held((double)w.softcap / raw) : 0.f;
     const Call a{(const uint16_t*)w.q, (uint16_t*)w.out, w.lse, w.q_stride, w.out_stride, w.q_start, w.kv_len,
-                 w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, w.scale,
-                 w.softcap, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
+                 w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, raw, cap_in,
+                 cap_out, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
                  cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
-    const Cache c = make_cache(*cache);
     const hipStream_t st = (hipStream_t)stream;
     if (cache->dtype == GFD_E4M3)
         return w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(a, c, p, cache->head_dim, st)
