@@ -215,10 +215,8 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 
     // The rows' operand, zero where there is no row.
     u32x4 q[K::kLdsRows ? 1 : R][K::kSteps];
-    // Scores stay in units of the product's sums, also capped and biased: the factor to the exponent of base 2 is
-    // positive, so the maximum is the same, and one multiply-add under the exponent applies it.
-    const float factor = a.raw * kLog2e;
-    float slope[R];
+    const float factor = a.factor;
+    float slope[R];  // in the scores' units
     for (int i = 0; i < R; i++) {
         const int h = head_of(a, k, 16 * i + col, kv_head);
         const uint16_t* p = a.q + row[i].t * a.q_stride + (int64_t)h * D;
@@ -228,7 +226,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             if constexpr (K::kLdsRows) lds.queries[i * K::kSteps + s][lane] = x;
             else q[i][s] = x;
         }
-        slope[i] = a.slopes && row[i].t >= 0 ? a.slopes[h] / a.raw : 0.f;
+        slope[i] = a.slopes && row[i].t >= 0 ? a.slopes[h] * (kLog2e / factor) : 0.f;
     }
 
     __syncthreads();
@@ -283,17 +281,16 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 #pragma unroll
         for (int i = 0; i < R; i++) {
             if (a.cap_in >= 0.f) {
-                float most = fabsf(x[i][0][0]);
+                const auto most = [&] {
+                    float y = fabsf(x[i][0][0]);
 #pragma unroll
-                for (int j = 1; j < 8; j++) most = max_f32(most, fabsf(x[i][j >> 2][j & 3]));
-                if (__any(!(most * a.cap_in <= kCapNear))) {
+                    for (int j = 1; j < 8; j++) y = max_f32(y, fabsf(x[i][j >> 2][j & 3]));
+                    return y;
+                };
+                cap_scores(a, most, [&](auto form) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        x[i][j >> 2][j & 3] = capped(x[i][j >> 2][j & 3], a.cap_in, a.cap_out);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[i][j >> 2][j & 3] = capped_near(x[i][j >> 2][j & 3], a.cap_in);
-                }
+                    for (int j = 0; j < 8; j++) x[i][j >> 2][j & 3] = form(x[i][j >> 2][j & 3]);
+                });
             }
             if (a.slopes) {
 #pragma unroll
@@ -439,10 +436,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
                 }
             if (a.lse && quarter == 0)
                 a.lse[(int64_t)row[i].t * a.q_heads + h] =
-                    sum[i] == 0.f ? -INFINITY : (m[i] * factor + __builtin_amdgcn_logf(sum[i])) * kLn2;
+                    sum[i] == 0.f ? -INFINITY : (m[i] * factor + a.shift + __builtin_amdgcn_logf(sum[i])) * kLn2;
         } else {
             const int64_t at = slot_of(a, st.first_slot + split, row[i].t, h);
-            if (quarter == 0) a.part_ml[at] = f32x2{m[i] == -INFINITY ? m[i] : m[i] * factor, sum[i]};
+            if (quarter == 0) a.part_ml[at] = f32x2{m[i] * factor + a.shift, sum[i]};
             float* out = a.part_o + at * D + 4 * quarter * K::kDims;
             if (sum[i] == 0.f) continue;  // its weight is zero and it is not read
 #pragma unroll

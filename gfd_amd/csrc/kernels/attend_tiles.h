@@ -18,7 +18,7 @@
 // 4096 tokens over 16384 keys, 32 heads of 128 in bf16: 945 us, 1020 TFLOP/s, where a library product of
 // 8192^3 reaches 1186 (the card's power holds both: 1.9 GHz with the matrix pipes at 45%,
 // and 1.6 to 1.9 GHz at 70%).  8192 packed tokens with capped scores: 211 us, 485 TFLOP/s; a cap costs
-// ten more instructions a score, and the longest document's blocks end last.
+// two more transcendental instructions a score, and the longest document's blocks end last.
 // 7 ragged prompts of 64 dims with a bias: 55 us, the 30 tiles of the longest one by 4 waves.
 // Tried and slower: half of the waves a product behind the others (1130 us for 1096), tiles of 32 keys with
 // three under way (2048 tokens 85 us for 74), two groups of 4 waves to a block (packed tokens 263 us for 223).
@@ -227,10 +227,9 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
 #pragma unroll
         for (int s = 0; s < K::kSteps; s++) q[s] = row.t >= 0 ? *(const u32x4*)(p + 16 * s) : u32x4{0, 0, 0, 0};
     }
-    // Scores stay in units of the product's sums, also capped and biased: the factor to the exponent of base 2 is
-    // positive, so the maximum is the same, and one multiply-add under the exponent applies it.
-    const float factor = a.raw * kLog2e;
-    slope /= a.raw;
+    // A bias in the scores' units: the sums of the product start from it, or it is added to what a cap leaves.
+    const float factor = a.factor;
+    slope *= kLog2e / factor;
     const int least_pos = kScores == kBiased ? lanes_min(my_row().t >= 0 ? pos : 0x7FFFFFFF) : 0;
     const int last_pos = kScores == kBiased ? -lanes_min(my_row().t >= 0 ? -pos : 0x7FFFFFFF) : 0;
     // A maximum that has grown by less than 2^8 is left as it is: weights and sums stay far from
@@ -366,22 +365,20 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
             }
             __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
             if (kScores == kCapped || (kScores == kBiased && a.cap_in >= 0.f)) {
-                float most = fabsf(x[0][0]);
-#pragma unroll
-                for (int i = 0; i < K::kHalves; i++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) most = max_f32(most, fabsf(x[i][r]));
-                if (__any(!(most * a.cap_in <= kCapNear))) {
+                const auto most = [&] {
+                    float y = fabsf(x[0][0]);
 #pragma unroll
                     for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) x[i][r] = capped(x[i][r], a.cap_in, a.cap_out);
-                } else {
+                        for (int r = 0; r < 16; r++) y = max_f32(y, fabsf(x[i][r]));
+                    return y;
+                };
+                cap_scores(a, most, [&](auto form) {
 #pragma unroll
                     for (int i = 0; i < K::kHalves; i++)
 #pragma unroll
-                        for (int r = 0; r < 16; r++) x[i][r] = capped_near(x[i][r], a.cap_in);
-                }
+                        for (int r = 0; r < 16; r++) x[i][r] = form(x[i][r]);
+                });
                 if (kScores == kBiased) add_bias(std::false_type());
             }
             const bool gap = bad[t & 7];
@@ -492,10 +489,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
             }
         if (a.lse && hi == 0)
             a.lse[(int64_t)row.t * a.q_heads + h] =
-                sum == 0.f ? -INFINITY : (m * factor + __builtin_amdgcn_logf(sum)) * kLn2;
+                sum == 0.f ? -INFINITY : (m * factor + a.shift + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
         const int64_t at = slot_of(a, st.first_slot + split, row.t, h);
-        if (hi == 0) a.part_ml[at] = f32x2{m == -INFINITY ? m : m * factor, sum};
+        if (hi == 0) a.part_ml[at] = f32x2{m * factor + a.shift, sum};
         if (sum == 0.f) return;  // its weight is zero and it is not read
         float* out = a.part_o + at * D + 4 * hi;
 #pragma unroll

@@ -31,8 +31,11 @@ struct Call {
     const int* doc_start;
     const int* prefix_end;
     const float* slopes;
-    float raw;                // scale * k_scale: a score is this times the product of q and the stored key
-    float cap_in, cap_out;    // softcap > 0: raw / softcap and softcap / raw; cap_in < 0: no cap
+    // Scores are kept as x, the product of q and the stored key or what a cap makes of it; their exponent of base 2 is
+    // x factor + shift.  The factor is positive, so maxima are the same, and one multiply-add under the exponent applies it.
+    float factor, shift;
+    float cap_in, cap_out;  // of a product x: x cap_in = s / softcap, cap_out softcap's own; cap_in < 0: no cap
+    int cap_small;
     int window, batch, num_tokens, max_q_len, max_kv_len, q_heads, kv_heads;
     Divider group;
     int* error;
@@ -255,11 +258,14 @@ __device__ __forceinline__ float across16_sum(float x) {
     return across32_sum(__uint_as_float(p[0]) + __uint_as_float(p[1]));
 }
 
-// softcap tanh(s / softcap) in units of the products' sums x, y = x cap_in.  Where |y| <= kCapNear: x (1 + z P(z)),
-// z = y^2, off by 2 2^-24 of itself however large the cap (P: a least-maximum fit of tanh(y) / y there, off by 0.6 2^-24).
-// 1 - 2 / (e^2y + 1), which loses what is small, is for the others, off by 4 2^-24 of itself.
-// The first form is also the shorter one, and a tile's scores take it together where all of them may.
-constexpr float kCapNear = 0.75f;
+// softcap tanh(s / softcap) in units of the products' sums x, y = x cap_in.  Three forms:
+// far, for caps of kCapLeast to kCapSmall: cap - 2 cap / (e^2y + 1), kept as -1 / (e^2y + 1), off by 4 2^-24 of the cap: 2^-16
+//   of a score's unit at most, little against the weights' rounding (2^-12, 2^-9);
+// near, where |y| <= kCapNear for all of a tile's scores: x (1 + z P(z)), z = y^2, off by 2 2^-24 of itself however large
+//   the cap (P: a least-maximum fit of tanh(y) / y there, off by 0.6 2^-24);
+// any: both, and a choice.
+// 8192 packed tokens, whose scores have a spread of 1.5: without a cap 174 us, far 211, near 214, any 290.
+constexpr float kCapNear = 0.75f, kCapSmall = 64.f, kCapLeast = 0x1p-20f;
 __device__ __forceinline__ float capped_near(float x, float cap_in) {
     const float y = x * cap_in, z = y * y;
     float p = -4.769478459e-03f;
@@ -269,10 +275,24 @@ __device__ __forceinline__ float capped_near(float x, float cap_in) {
     p = __builtin_fmaf(p, z, -3.333306909e-01f);
     return __builtin_fmaf(x * z, p, x);
 }
-__device__ __forceinline__ float capped(float x, float cap_in, float cap_out) {
-    const float y = x * cap_in;
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.f * kLog2e)) + 1.f);
-    return fabsf(y) <= kCapNear ? capped_near(x, cap_in) : far * cap_out;
+__device__ __forceinline__ float capped_far(float x, float cap_in) {
+    return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x * (cap_in * (2.f * kLog2e))));
+}
+__device__ __forceinline__ float capped_any(float x, float cap_in, float cap_out) {
+    const float near = capped_near(x, cap_in), far = __builtin_fmaf(capped_far(x, cap_in), 2.f * cap_out, cap_out);
+    return fabsf(x * cap_in) <= kCapNear ? near : far;
+}
+// all(f): every score becomes f(score); most(): the largest magnitude among a lane's, NaN if one is.
+template <typename M, typename F>
+__device__ __forceinline__ void cap_scores(const Call& a, M most, F all) {
+    // The forms are not to share what they have in common: a tile's worth of it would be held.
+    const auto apart = [](float x) {
+        asm("" : "+v"(x));
+        return x;
+    };
+    if (a.cap_small) all([&](float x) { return capped_far(x, a.cap_in); });
+    else if (__any(!(most() * a.cap_in <= kCapNear))) all([&](float x) { return capped_any(apart(x), a.cap_in, a.cap_out); });
+    else all([&](float x) { return capped_near(apart(x), a.cap_in); });
 }
 
 // Matrix instructions by element type, and tests on packed pairs.

@@ -257,10 +257,12 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     const auto held = [](double x) { return (float)std::min(x, 3.4028234e38); };
     const float cap_in = w.softcap > 0.f ? held((double)raw / w.softcap) : -1.f;
     const float cap_out = w.softcap > 0.f ? held((double)w.softcap / raw) : 0.f;
+    const bool cap_small = w.softcap >= kCapLeast && w.softcap <= kCapSmall;
+    const float factor = (cap_small ? 2.f * w.softcap : raw) * kLog2e, shift = cap_small ? w.softcap * kLog2e : 0.f;
     const Call a{(const uint16_t*)w.q, (uint16_t*)w.out, w.lse, w.q_stride, w.out_stride, w.q_start, w.kv_len,
-                 w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, raw, cap_in,
-                 cap_out, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len, w.num_q_heads,
-                 cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
+                 w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, factor, shift,
+                 cap_in, cap_out, cap_small, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len,
+                 w.num_q_heads, cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
     const hipStream_t st = (hipStream_t)stream;
     if (cache->dtype == GFD_E4M3)

@@ -579,7 +579,7 @@ int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows, int* error
  *   hi = min(kv_len[b], max(p + 1, prefix_end[token]))   (prefix_end NULL: p + 1)
  * with the score
  *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[head] |p - j| if slopes
- * (right relative to the score for caps of any size: a cap far above the scores changes nothing)
+ * (a cap of any size: off by 2^-22 of the cap up to 64 and of the score above, so one far above the scores changes nothing)
  * out = sum of softmax(s) v (zeros where nothing is visible), lse = the
  * natural logarithm of the sum of exp(s) (-inf there; NULL: not wanted).
  * Values of slots that no token of the sequence sees are never used. */
