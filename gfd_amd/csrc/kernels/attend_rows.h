@@ -215,7 +215,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 
     // The rows' operand, zero where there is no row.
     u32x4 q[K::kLdsRows ? 1 : R][K::kSteps];
-    const float factor = a.factor;
+    const float factor = a.factor, shift = a.shift - Mma<T>::kRaise;  // of a weight and of a maximum
     float slope[R];  // in the scores' units
     for (int i = 0; i < R; i++) {
         const int h = head_of(a, k, 16 * i + col, kv_head);
@@ -320,7 +320,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 #pragma unroll
                 for (int d = 0; d < K::kDims; d++) o[i][d] *= keep;
             }
-            const float base_m = m[i] == -INFINITY ? 0.f : m[i] * factor;
+            const float base_m = (m[i] == -INFINITY ? 0.f : m[i] * factor) - Mma<T>::kRaise;
             float e[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -436,10 +436,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
                 }
             if (a.lse && quarter == 0)
                 a.lse[(int64_t)row[i].t * a.q_heads + h] =
-                    sum[i] == 0.f ? -INFINITY : (m[i] * factor + a.shift + __builtin_amdgcn_logf(sum[i])) * kLn2;
+                    sum[i] == 0.f ? -INFINITY : (m[i] * factor + shift + __builtin_amdgcn_logf(sum[i])) * kLn2;
         } else {
             const int64_t at = slot_of(a, st.first_slot + split, row[i].t, h);
-            if (quarter == 0) a.part_ml[at] = f32x2{m[i] * factor + a.shift, sum[i]};
+            if (quarter == 0) a.part_ml[at] = f32x2{m[i] * factor + shift, sum[i]};
             float* out = a.part_o + at * D + 4 * quarter * K::kDims;
             if (sum[i] == 0.f) continue;  // its weight is zero and it is not read
 #pragma unroll

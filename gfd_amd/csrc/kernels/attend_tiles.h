@@ -232,9 +232,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     slope *= kLog2e / factor;
     const int least_pos = kScores == kBiased ? lanes_min(my_row().t >= 0 ? pos : 0x7FFFFFFF) : 0;
     const int last_pos = kScores == kBiased ? -lanes_min(my_row().t >= 0 ? -pos : 0x7FFFFFFF) : 0;
-    // A maximum that has grown by less than 2^8 is left as it is: weights and sums stay far from
+    // A maximum that has grown by less than 2^kSlack is left as it is: weights and sums stay within
     // what 16 and 32 bits hold, and the output is rescaled in a few tiles only.
-    const float slack = 8.f / factor;
+    constexpr float kRaise = Mma<T>::kRaise > 0.f ? Mma<T>::kRaise - Mma<T>::kSlack : 0.f;
+    const float slack = Mma<T>::kSlack / factor;
 
     float m = -INFINITY, sum = 0.f;
     f32x16 o[K::kDims];
@@ -416,7 +417,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
 #pragma unroll
                 for (int i = 0; i < K::kDims; i++) o[i] *= keep;
             }
-            const float base_m = m == -INFINITY ? 0.f : m * factor;
+            const float base_m = (m == -INFINITY ? 0.f : m * factor) - kRaise;
             // A weight is rounded to the values' 16-bit type, as the matrix product takes it.
             u32x4 p[K::kHalves][2];
 #pragma unroll
@@ -489,10 +490,10 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
             }
         if (a.lse && hi == 0)
             a.lse[(int64_t)row.t * a.q_heads + h] =
-                sum == 0.f ? -INFINITY : (m * factor + a.shift + __builtin_amdgcn_logf(sum)) * kLn2;
+                sum == 0.f ? -INFINITY : (m * factor + (a.shift - kRaise) + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
         const int64_t at = slot_of(a, st.first_slot + split, row.t, h);
-        if (hi == 0) a.part_ml[at] = f32x2{m * factor + a.shift, sum};
+        if (hi == 0) a.part_ml[at] = f32x2{m * factor + (a.shift - kRaise), sum};
         if (sum == 0.f) return;  // its weight is zero and it is not read
         float* out = a.part_o + at * D + 4 * hi;
 #pragma unroll

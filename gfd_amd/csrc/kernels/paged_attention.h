@@ -300,6 +300,9 @@ template <typename T>
 struct Mma;
 template <>
 struct Mma<Bf16> {
+    // A weight is 2^kRaise e^(s - m), m the running maximum, which a score may pass by 2^kSlack (in kernels that
+    // let it): 16 bits of this type hold weights of any size to the same relative step.
+    static constexpr float kRaise = 0.f, kSlack = 8.f;
     static constexpr uint32_t kNear = 0x00800080u;  // added to a magnitude: bit 15 is set from infinity on
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
@@ -319,6 +322,11 @@ struct Mma<Bf16> {
 };
 template <>
 struct Mma<Fp16> {
+    // This type holds 2^-14 to 2^16 in full, below in steps of 2^-24.  Weights use its upper end, so that those of
+    // many keys far below a maximum are not lost: down to 2^-29 of the largest they are rounded relatively, and what a
+    // key loses below that is 2^-40 of the largest, or 2^-39 where scores may pass the maximum by 2^1.
+    // The small slack costs a few rescalings more: 7 ragged prompts of 64 dims 61 us, with 2^8 and no offset 59.5.
+    static constexpr float kRaise = 15.f, kSlack = 1.f;
     static constexpr uint32_t kNear = 0x04000400u;
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
