@@ -36,20 +36,18 @@ int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage&
     const int prefix_turns = (int)(tiles_groups(a, prefix, none) / 8),
               own_turns = (int)(((int64_t)own.blocks * own.splits * a.kv_heads + 7) / 8);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(8 * (prefix_turns + own_turns))), dim3(256), 0, st, a, c,
-                           prefix, own, prefix_turns);
+        return start(kernel, dim3((unsigned)(8 * (prefix_turns + own_turns))), 256, st, a, c, prefix, own, prefix_turns);
     };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        with_scores(a, [&](auto scores) {
+        return with_scores(a, [&](auto scores) {
             constexpr int kScores = decltype(scores)::value;
-            wide ? go(attend_both_kernel<T, S, D, 2, kScores>) : go(attend_both_kernel<T, S, D, 1, kScores>);
+            return wide ? go(attend_both_kernel<T, S, D, 2, kScores>) : go(attend_both_kernel<T, S, D, 1, kScores>);
         });
     };
-    if (dim == 64) pick(std::integral_constant<int, 64>());
-    if (dim == 128) pick(std::integral_constant<int, 128>());
-    if (dim == 256) pick(std::integral_constant<int, 256>());
-    return (int)hipGetLastError();
+    if (dim == 64) return pick(std::integral_constant<int, 64>());
+    if (dim == 128) return pick(std::integral_constant<int, 128>());
+    return pick(std::integral_constant<int, 256>());
 }
 
 }  // namespace kv

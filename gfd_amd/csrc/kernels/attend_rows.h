@@ -463,16 +463,15 @@ template <typename T, typename S>
 int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st) {
     const dim3 grid((unsigned)((prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads));
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, c, prefix, own); };
+    const auto go = [&](auto kernel) { return start(kernel, grid, 64 * waves, st, a, c, prefix, own); };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (waves == 1) wide ? go(attend_rows_kernel<T, S, D, 2, 1>) : go(attend_rows_kernel<T, S, D, 1, 1>);
-        else wide ? go(attend_rows_kernel<T, S, D, 2, 4>) : go(attend_rows_kernel<T, S, D, 1, 4>);
+        if (waves == 1) return wide ? go(attend_rows_kernel<T, S, D, 2, 1>) : go(attend_rows_kernel<T, S, D, 1, 1>);
+        return wide ? go(attend_rows_kernel<T, S, D, 2, 4>) : go(attend_rows_kernel<T, S, D, 1, 4>);
     };
-    if (dim == 64) pick(std::integral_constant<int, 64>());
-    if (dim == 128) pick(std::integral_constant<int, 128>());
-    if (dim == 256) pick(std::integral_constant<int, 256>());
-    return (int)hipGetLastError();
+    if (dim == 64) return pick(std::integral_constant<int, 64>());
+    if (dim == 128) return pick(std::integral_constant<int, 128>());
+    return pick(std::integral_constant<int, 256>());
 }
 
 }  // namespace kv

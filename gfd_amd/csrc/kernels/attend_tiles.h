@@ -521,10 +521,10 @@ inline int64_t tiles_groups(const Call& a, const Stage& prefix, const Stage& own
 
 // f(scores) with the kind of scores that the call has, as a constant.
 template <typename F>
-void with_scores(const Call& a, F f) {
-    if (a.slopes) f(std::integral_constant<int, kBiased>());
-    else if (a.cap_in >= 0.f) f(std::integral_constant<int, kCapped>());
-    else f(std::integral_constant<int, kPlain>());
+int with_scores(const Call& a, F f) {
+    if (a.slopes) return f(std::integral_constant<int, kBiased>());
+    if (a.cap_in >= 0.f) return f(std::integral_constant<int, kCapped>());
+    return f(std::integral_constant<int, kPlain>());
 }
 
 template <typename T, typename S>
@@ -532,22 +532,21 @@ int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage
                  hipStream_t st) {
     const dim3 grid((unsigned)tiles_groups(a, prefix, own));
     const auto go = [&](auto kernel, int w) {
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * w), 0, st, a, c, prefix, own);
+        return start(kernel, grid, 64 * w, st, a, c, prefix, own);
     };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        with_scores(a, [&](auto scores) {
+        return with_scores(a, [&](auto scores) {
             constexpr int kScores = decltype(scores)::value;
             if constexpr (D != 256) {
                 if (waves == 8) return go(attend_tiles_kernel<T, S, D, 8, kScores>, 8);
             }
-            go(attend_tiles_kernel<T, S, D, 4, kScores>, 4);
+            return go(attend_tiles_kernel<T, S, D, 4, kScores>, 4);
         });
     };
-    if (dim == 64) pick(std::integral_constant<int, 64>());
-    if (dim == 128) pick(std::integral_constant<int, 128>());
-    if (dim == 256) pick(std::integral_constant<int, 256>());
-    return (int)hipGetLastError();
+    if (dim == 64) return pick(std::integral_constant<int, 64>());
+    if (dim == 128) return pick(std::integral_constant<int, 128>());
+    return pick(std::integral_constant<int, 256>());
 }
 
 }  // namespace kv

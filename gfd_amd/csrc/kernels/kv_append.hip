@@ -41,6 +41,22 @@ Cache make_cache(const gfd_kv_cache& c) {
                  c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f};
 }
 
+int refused(const char* name, const char* why) {
+    static thread_local char text[192];
+    snprintf(text, sizeof(text), "%s: %s", name, why);
+    gfd_internal_set_error(text);
+    return (int)hipErrorInvalidValue;
+}
+
+int launched(const char* name, int rc) {
+    if (rc) {
+        static thread_local char text[192];
+        snprintf(text, sizeof(text), "%s: the launch failed: %s", name, hipGetErrorString((hipError_t)rc));
+        gfd_internal_set_error(text);
+    }
+    return rc;
+}
+
 namespace {
 
 struct Rows {
@@ -234,21 +250,16 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
     }
 }
 
-int refuse(const char* why) {
-    static thread_local char text[160];
-    snprintf(text, sizeof(text), "gfd_kv_append: %s", why);
-    gfd_internal_set_error(text);
-    return (int)hipErrorInvalidValue;
-}
+constexpr char kName[] = "gfd_kv_append";
+int refuse(const char* why) { return refused(kName, why); }
 
 template <typename T, typename S, int kTokensHere>
 int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
     const dim3 grid((unsigned)((r.num_tokens + kTokensHere - 1) / kTokensHere));
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, st, r, c); };
-    if (pairs) go(kv_append_kernel<T, S, kSide, kTokensHere>);
-    else if (r.rotary % 16 == 0) go(kv_append_kernel<T, S, kChunksApart, kTokensHere>);
-    else go(kv_append_kernel<T, S, kApart, kTokensHere>);
-    return (int)hipGetLastError();
+    const auto go = [&](auto kernel) { return start(kernel, grid, kBlock, st, r, c); };
+    if (pairs) return go(kv_append_kernel<T, S, kSide, kTokensHere>);
+    if (r.rotary % 16 == 0) return go(kv_append_kernel<T, S, kChunksApart, kTokensHere>);
+    return go(kv_append_kernel<T, S, kApart, kTokensHere>);
 }
 
 // Tokens share a workgroup's start-up where that still fills the card.
@@ -287,6 +298,8 @@ extern "C" int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows,
     const hipStream_t st = (hipStream_t)stream;
     const bool pairs = w.interleaved != 0;
     if (cache->dtype == GFD_E4M3)
-        return w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(r, c, pairs, st) : launch<Fp16, E4m3>(r, c, pairs, st);
-    return w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(r, c, pairs, st) : launch<Fp16, Fp16>(r, c, pairs, st);
+        return launched(kName, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(r, c, pairs, st)
+                                                   : launch<Fp16, E4m3>(r, c, pairs, st));
+    return launched(kName, w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(r, c, pairs, st)
+                                               : launch<Fp16, Fp16>(r, c, pairs, st));
 }

@@ -9,9 +9,7 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <cstdio>
 
-#include "capi_error.h"
 #include "gfd_capi.h"
 #include "paged_attention.h"
 
@@ -175,9 +173,8 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
 
 template <typename T, int D, int kRows, int kPart>
 int launch_join(const Call& a, const Cache& c, const Stage& own, hipStream_t st) {
-    hipLaunchKernelGGL((join_kernel<T, D, kRows, kPart>), dim3((unsigned)(own.blocks * a.kv_heads), kRows / kPart),
-                       dim3(kJoinBlock), 0, st, a, c, own);
-    return (int)hipGetLastError();
+    return start(join_kernel<T, D, kRows, kPart>, dim3((unsigned)(own.blocks * a.kv_heads), kRows / kPart), kJoinBlock, st,
+                 a, c, own);
 }
 template <typename T, int D>
 int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
@@ -203,13 +200,6 @@ int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st
     if (rc || p.slots == 1) return rc;
     return dim == 64 ? launch_join<T, 64>(a, c, p, st) : dim == 128 ? launch_join<T, 128>(a, c, p, st)
                                                                    : launch_join<T, 256>(a, c, p, st);
-}
-
-int refuse(const char* name, const char* why) {
-    static thread_local char text[192];
-    snprintf(text, sizeof(text), "%s: %s", name, why);
-    gfd_internal_set_error(text);
-    return (int)hipErrorInvalidValue;
 }
 
 const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len) {
@@ -238,15 +228,15 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
 
 int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* call, const int* prefix_table,
               int prefix_len, void* workspace, size_t workspace_bytes, int* error_flag, void* stream) {
-    if (const char* why = check_call(cache, call, prefix_len)) return refuse(name, why);
+    if (const char* why = check_call(cache, call, prefix_len)) return refused(name, why);
     const gfd_attention& w = *call;
     if (w.batch == 0 || w.num_tokens == 0 || w.max_q_len == 0) return 0;
-    if (!w.q || !w.out || !w.q_start || !w.kv_len) return refuse(name, "q, out, q_start or kv_len is missing");
-    if (!w.block_table && w.max_kv_len > prefix_len) return refuse(name, "block_table is missing");
-    if (!prefix_table && prefix_len > 0) return refuse(name, "prefix_table is missing");
+    if (!w.q || !w.out || !w.q_start || !w.kv_len) return refused(name, "q, out, q_start or kv_len is missing");
+    if (!w.block_table && w.max_kv_len > prefix_len) return refused(name, "block_table is missing");
+    if (!prefix_table && prefix_len > 0) return refused(name, "prefix_table is missing");
     const Plan p = make_plan(*cache, w, prefix_len);
     if (p.bytes && (!workspace || workspace_bytes < (size_t)p.bytes || (uintptr_t)workspace % 16 != 0))
-        return refuse(name, "workspace is missing, not 16-byte aligned or smaller than gfd_attention_workspace_bytes says");
+        return refused(name, "workspace is missing, not 16-byte aligned or smaller than gfd_attention_workspace_bytes says");
     const int64_t rows = (int64_t)w.num_tokens * w.num_q_heads;
     float* const part_o = p.bytes ? (float*)workspace : nullptr;
     float* const part_ml = p.bytes ? part_o + p.slots * rows * cache->head_dim : nullptr;
@@ -266,10 +256,10 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
                  (f32x2*)part_ml, part_o, (int*)splits};
     const hipStream_t st = (hipStream_t)stream;
     if (cache->dtype == GFD_E4M3)
-        return w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(a, c, p, cache->head_dim, st)
-                                   : launch<Fp16, E4m3>(a, c, p, cache->head_dim, st);
-    return w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(a, c, p, cache->head_dim, st)
-                               : launch<Fp16, Fp16>(a, c, p, cache->head_dim, st);
+        return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(a, c, p, cache->head_dim, st)
+                                                  : launch<Fp16, E4m3>(a, c, p, cache->head_dim, st));
+    return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(a, c, p, cache->head_dim, st)
+                                              : launch<Fp16, Fp16>(a, c, p, cache->head_dim, st));
 }
 
 }  // namespace
@@ -279,7 +269,7 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
 extern "C" int64_t gfd_attention_workspace_bytes(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len) {
     using namespace gfd::kv;
     if (const char* why = check_call(cache, call, prefix_len)) {
-        refuse("gfd_attention_workspace_bytes", why);
+        refused("gfd_attention_workspace_bytes", why);
         return -1;
     }
     return make_plan(*cache, *call, prefix_len).bytes;

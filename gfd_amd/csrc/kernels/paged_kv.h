@@ -72,6 +72,18 @@ struct Cache {
     float k_scale, v_scale;  // 1 unless the type is E4M3
 };
 
+// Launches, and returns this launch's own status: the last error of the thread may be an earlier call's.
+template <typename... P>
+int start(void (*kernel)(P...), dim3 grid, int threads, hipStream_t st, const P&... args) {
+    void* pointers[] = {const_cast<P*>(&args)...};
+    const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3((unsigned)threads), pointers, 0, st);
+    if (e != hipSuccess) (void)hipGetLastError();  // it is returned, and is no later call's
+    return (int)e;
+}
+// The text behind gfd_last_error() for a refused call, or one whose launch failed with rc; returns the call's result.
+int refused(const char* name, const char* why);
+int launched(const char* name, int rc);
+
 // An argument that a kernel for the cache relies on, or NULL if all hold.
 const char* check_cache(const gfd_kv_cache* c);
 Cache make_cache(const gfd_kv_cache& c);
