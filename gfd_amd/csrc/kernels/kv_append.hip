@@ -280,6 +280,8 @@ extern "C" int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows,
     if (w.dtype != GFD_BF16 && w.dtype != GFD_FP16) return refuse("rows are neither GFD_BF16 nor GFD_FP16");
     if (cache->dtype != GFD_E4M3 && cache->dtype != w.dtype) return refuse("the cache's type is neither the rows' nor GFD_E4M3");
     if (w.num_tokens < 0) return refuse("negative num_tokens");
+    if (((int64_t)w.num_tokens + kTokens - 1) / kTokens * kBlock >= kGridThreads)
+        return refuse("more work than one launch takes");
     if (w.rotary_dim < 0 || w.rotary_dim > cache->head_dim || w.rotary_dim % 2 != 0)
         return refuse("rotary_dim is odd or outside 0..head_dim");
     if ((w.q != nullptr) != (w.q_out != nullptr)) return refuse("q and q_out go together");

@@ -91,7 +91,7 @@ struct Plan {
     int rows;                     // of an own-keys block
     Stage prefix, own;
     int slots;      // partial results per row
-    int64_t items;  // workgroups of the largest launch
+    int64_t threads;  // of the largest launch, at most
     int64_t bytes;  // of workspace
 };
 
@@ -165,7 +165,9 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.own.first_slot = p.prefix.splits;
     }
     p.slots = p.own.first_slot + p.own.splits;
-    p.items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
+    // Turns of 8 workgroups are filled up.  The join, where there is one, has as many threads at most.
+    const int64_t items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
+    p.threads = (items + 16) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
     if (p.slots > 1)
         p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4 + p.own.blocks * heads * 4;
     return p;
@@ -221,7 +223,7 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
         return "rows' pointers or strides are not multiples of 16 bytes";
     const int64_t pages = ((int64_t)std::max(w.max_kv_len - prefix_len, 0) + cache->page_size - 1) / cache->page_size;
     if (w.table_stride < pages) return "block_table's rows are shorter than max_kv_len needs";
-    if ((int64_t)w.num_tokens * w.num_q_heads > (1 << 30) || make_plan(*cache, w, prefix_len).items > (1 << 28))
+    if ((int64_t)w.num_tokens * w.num_q_heads > (1 << 30) || make_plan(*cache, w, prefix_len).threads >= kGridThreads)
         return "more work than one launch takes";
     return nullptr;
 }

@@ -72,6 +72,8 @@ struct Cache {
     float k_scale, v_scale;  // 1 unless the type is E4M3
 };
 
+// A launch has fewer threads along a grid than this.
+constexpr int64_t kGridThreads = 1ll << 32;
 // Launches, and returns this launch's own status: the last error of the thread may be an earlier call's.
 template <typename... P>
 int start(void (*kernel)(P...), dim3 grid, int threads, hipStream_t st, const P&... args) {

@@ -518,7 +518,10 @@ int gfd_sg_poller_run(void* queue, void* sg_queue, const gfd_device_sg_entry* d_
  * them by attention.  Every pointer is device memory.  Calls run on `stream`
  * (NULL: the default stream) of the current device, allocate nothing, do not
  * synchronise, and can be captured into a graph.  A refused call launches
- * nothing, and gfd_last_error() says why. ---- */
+ * nothing, and gfd_last_error() says why, as it does where a launch fails.
+ * Refused are also sizes past one launch, which has fewer than 2^32 threads:
+ * for kv_append 2^26 - 3 tokens, for attention about 2^24 workgroups (of a
+ * sequence's rows, a head of the cache and a range of keys) or 2^30 rows. ---- */
 enum { GFD_BF16 = 0, GFD_FP16 = 1, GFD_E4M3 = 2 };  /* element types; E4M3: 8-bit floats (OCP e4m3fn) */
 
 /* Keys and values in pages.  Slot s of page p, head h starts at element

@@ -7,7 +7,7 @@ import pytest
 import gfd_amd
 import paged_kv_ref as ref
 from paged_kv_ref import BF16
-from test_gpu_paged_kv import Attend, up
+from test_gpu_paged_kv import Attend, close, up
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,27 @@ def test_append_after_a_failed_call(fail_elsewhere):
                                             num_tokens=3, dtype=BF16))
     gfd_amd.synchronize()
     assert (words.download().view(np.uint16) == 0x3F80).sum() == 3 * 2 * 256
+
+
+def test_the_largest_batch_is_one_launch():
+    """2^24 - 24 workgroups of 256 threads, all but a few of sequences without tokens."""
+    rng = np.random.default_rng(97)
+    batch, kv = (1 << 21) - 3, 200
+    pages = ref.Pages(rng, [kv], 256, 8, 64, BF16, spare=0)
+    pages.table = np.zeros((batch, 1), np.int32)
+    a = Attend(rng, pages, [1] * 3, [kv] * 3, 8, BF16)
+    starts = np.zeros(batch + 1, np.int32)
+    lengths = np.zeros(batch, np.int32)
+    for i, b in enumerate((0, batch // 2, batch - 1)):  # the sequences with a token
+        starts[b + 1:] = i + 1
+        lengths[b] = kv
+    keep = up(starts), up(lengths)
+    a.call.q_start, a.call.kv_len, a.call.batch = keep[0].ptr, keep[1].ptr, batch
+    assert gfd_amd.attention_workspace_bytes(a.cache, a.call) == 0
+    want, want_lse, tol, tol_lse = ref.attention64(a.q, pages, [(0, kv - 1, 0, kv)] * 3, BF16, float(np.float32(a.scale)))
+    out, lse = a.run()
+    close(out, want, tol, "out")
+    close(lse, want_lse, tol_lse, "lse")
+    a.call.batch = batch + 1
+    with pytest.raises(gfd_amd.GfdError, match="more work than one launch takes"):
+        a.launch()

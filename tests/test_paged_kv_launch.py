@@ -18,3 +18,36 @@ def test_a_failed_launch_leaves_its_text_and_no_earlier_one():
             gfd_amd.kv_append(cache(), rows(num_tokens=-1))
         with pytest.raises(gfd_amd.GfdError, match=name + ": the launch failed: "):
             run()
+
+
+# A launch has fewer than 2^32 threads along its grid: the largest call that is taken, and the next one.
+
+@needs_no_gpu
+def test_the_largest_append():
+    largest = 4 * ((1 << 24) - 1)  # four tokens a workgroup of 256
+    with pytest.raises(gfd_amd.GfdError, match="the launch failed"):
+        gfd_amd.kv_append(cache(), rows(num_tokens=largest))
+    for tokens in (largest + 1, 0x7FFFFFFF):
+        with pytest.raises(gfd_amd.GfdError, match="gfd_kv_append: more work than one launch takes"):
+            gfd_amd.kv_append(cache(), rows(num_tokens=tokens))
+
+
+@needs_no_gpu
+@pytest.mark.parametrize("prefix", [0, 160])
+@pytest.mark.parametrize("sizes,largest", [(dict(max_kv_len=1000), (1 << 24) // 8 - 3),  # few rows: 256 threads a head and sequence
+                                           # two blocks of 128 rows more: 64 tokens of 4 heads
+                                           (dict(max_kv_len=1000, max_q_len=500), (1 << 24) // 8 - 5)])
+def test_the_largest_batch(sizes, largest, prefix):
+    """Two rounds of 8 workgroups may be filled up: so many sequences are one launch, and the next is refused."""
+    for batch, why in ((largest - 40 * bool(prefix), "the launch failed"), (largest + 1, "more work than one launch takes")):
+        c = call(batch=batch, num_tokens=64, **sizes)
+        with pytest.raises(gfd_amd.GfdError, match=why):
+            if prefix:
+                gfd_amd.shared_prefix_attention(cache(), c, 1 << 20, prefix, 1 << 20, 1 << 60)
+            else:
+                gfd_amd.paged_attention(cache(), c, 1 << 20, 1 << 60)
+
+
+def test_a_workspace_is_stated_only_for_calls_that_are_taken():
+    with pytest.raises(gfd_amd.GfdError, match="more work than one launch takes"):
+        gfd_amd.attention_workspace_bytes(cache(), call(batch=1 << 21, num_tokens=64, max_kv_len=1000))
