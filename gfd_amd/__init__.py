@@ -873,7 +873,8 @@ def kv_append(cache, rows, error_flag=None, stream=None):
 def attention_workspace_bytes(cache, call, prefix_len=0):
     """Device bytes that paged_attention() (prefix_len 0) or
     shared_prefix_attention() needs for `call` (Attention).  Depends on every
-    size of the call: keep the largest of those that a program makes."""
+    size of the call and is not the largest for the largest batch: keep the
+    largest of those that a program makes, or ask for each."""
     n = lib().gfd_attention_workspace_bytes(cache, call, prefix_len)
     if n < 0:
         _check(-1, "gfd_attention_workspace_bytes")

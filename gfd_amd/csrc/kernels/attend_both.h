@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call
     const Stage none{0, 0, 0, 0, 1, 0, 0};
     if (turn >= prefix_turns) {
         const int item = (turn - prefix_turns) * 8 + xcd;
-        if (item < own.blocks * own.splits * a.kv_heads) attend_rows<T, S, D, R, 4>(a, c, none, own, item, lds.rows);
+        if (item < own.blocks * own.splits * a.kv_heads) attend_rows<T, S, D, R, 4, false>(a, c, none, own, item, lds.rows);
     } else {
         attend_tiles<T, S, D, 4, kScores>(a, c, prefix, none, turn * 8 + xcd, lds.tiles);
     }

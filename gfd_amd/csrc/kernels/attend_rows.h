@@ -25,6 +25,7 @@
 // 64 ragged contexts of up to 8192: 161 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
 // capped: 61 us, 4.8 TB/s.  700 keys of one token: 7.4 us and 3.4 to join, a chain of loads
 // (lengths, pages, keys) and a launch each.  Many short contexts take a wave each: 128 of 128 keys in 16 us, 4.2 TB/s.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_attention.h"
@@ -148,7 +149,7 @@ template <typename T, typename S, int D, int R, int kWaves>
 struct RowsLds {
     using K = RowsKernel<T, S, D, R>;
     i32x4 rows[16 * R];
-    int64_t offsets[kWaves == 1 ? kRowsShort : kRowsMaxChunk];
+    int64_t offsets[kWaves == 1 ? kRowsShort : kRowsPiece];
     union {
         int samples[kSamples + 1];
         float merge[kWaves == 1 ? 1 : kWaves / 2][kWaves == 1 ? 1 : R * K::kAcc + 2 * R][64];
@@ -158,8 +159,8 @@ struct RowsLds {
     int any_bad;
 };
 
-// kWaves 1: ranges of at most kRowsShort keys.
-template <typename T, typename S, int D, int R, int kWaves>
+// kWaves 1: ranges of at most kRowsShort keys.  kPieces: ranges of more than kRowsPiece keys.
+template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
 __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int item,
                                             RowsLds<T, S, D, R, kWaves>& lds) {
     using K = RowsKernel<T, S, D, R>;
@@ -188,12 +189,14 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     }
     if (tid == 0) lds.any_bad = 0;
     __syncthreads();
-    Row row[R];
-    for (int i = 0; i < R; i++) {
+    const auto read_row = [&](int i) {
         const i32x4 x = lds.rows[16 * i + col];
-        row[i] = Row{x[0], x[1], x[2], x[3]};
-        range_add(g, row[i]);
-    }
+        return Row{x[0], x[1], x[2], x[3]};
+    };
+    Row row[R];
+    for (int i = 0; i < R; i++) range_add(g, row[i] = read_row(i));
+    // With pieces it is read again where it is used: registers are short.
+    const auto row_at = [&](int i) { return kPieces ? read_row(i) : row[i]; };
     g.lo = lanes_min(g.lo);
     g.hi = -lanes_min(-g.hi);
     g.all_lo = -lanes_min(-g.all_lo);
@@ -207,11 +210,19 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     const int c0 = max(base, g.lo), c1 = min(base + st.chunk, g.hi);
     const int64_t head = kv_head * c.head_stride;
     const int tiles = c1 > c0 ? (c1 - c0 + kRowsTile - 1) / kRowsTile : 0;
-    for (int n = tid; n < tiles * kRowsTile; n += kThreads) {
-        const int64_t o = c0 + n < c1 ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
-        if (o < 0 && c0 + n < c1) lds.any_bad = 1;
-        lds.offsets[n] = o;
-    }
+    // kPieces: a range is walked in pieces, whose keys' offsets are in LDS.
+    constexpr int kPieceTiles = (kWaves == 1 ? kRowsShort : kRowsPiece) / kRowsTile;
+    static_assert(kPieceTiles % kWaves == 0, "all waves end a piece together");
+    const auto look_up = [&](int piece) {
+        const int n0 = c0 + piece * kPieceTiles * kRowsTile;
+        const int most = (kPieces ? min(tiles - piece * kPieceTiles, kPieceTiles) : tiles) * kRowsTile;
+        for (int n = tid; n < most; n += kThreads) {
+            const int64_t o = n0 + n < c1 ? key_offset(c, k.table, n0 + n, head, a.error) : -1;
+            if (o < 0 && n0 + n < c1) lds.any_bad = 1;
+            lds.offsets[n] = o;
+        }
+    };
+    look_up(0);
 
     // The rows' operand, zero where there is no row.
     u32x4 q[K::kLdsRows ? 1 : R][K::kSteps];
@@ -219,18 +230,18 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     float slope[R];  // in the scores' units
     for (int i = 0; i < R; i++) {
         const int h = head_of(a, k, 16 * i + col, kv_head);
-        const uint16_t* p = a.q + row[i].t * a.q_stride + (int64_t)h * D;
+        const uint16_t* p = a.q + row_at(i).t * a.q_stride + (int64_t)h * D;
         for (int s = 0; s < K::kSteps; s++) {
             if (K::kLdsRows && wave != (i * K::kSteps + s) % kWaves) continue;
-            const u32x4 x = row[i].t >= 0 ? *(const u32x4*)(p + K::step_dim(s, quarter)) : u32x4{0, 0, 0, 0};
+            const u32x4 x = row_at(i).t >= 0 ? *(const u32x4*)(p + K::step_dim(s, quarter)) : u32x4{0, 0, 0, 0};
             if constexpr (K::kLdsRows) lds.queries[i * K::kSteps + s][lane] = x;
             else q[i][s] = x;
         }
-        slope[i] = a.slopes && row[i].t >= 0 ? a.slopes[h] * (kLog2e / factor) : 0.f;
+        slope[i] = a.slopes && row_at(i).t >= 0 ? a.slopes[h] * (kLog2e / factor) : 0.f;
     }
 
     __syncthreads();
-    const bool bad = lds.any_bad != 0;
+    bool bad = lds.any_bad != 0;
     float m[R], sum[R];
     f32x4 o[R][K::kDims];
     for (int i = 0; i < R; i++) {
@@ -249,13 +260,22 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     for (int tile = wave; tile < tiles; tile += kWaves) {
         const int n0 = c0 + tile * kRowsTile;
         const bool more = tile + kWaves < tiles;
-        const int64_t* next = lds.offsets + (tile + kWaves) * kRowsTile;
+        // A piece's last tiles, one a wave, with another piece behind it: all waves are here.
+        const bool turn = kPieces && tile % kPieceTiles >= kPieceTiles - kWaves &&
+                          tile / kPieceTiles * kPieceTiles + kPieceTiles < tiles;
+        const int64_t* next = lds.offsets + (kPieces ? (tile + kWaves) % kPieceTiles : tile + kWaves) * kRowsTile;
         if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
         K::store_keys(t, my_keys, lane);
         // Other lanes of the wave read them: its LDS accesses are in order, the compiler has to keep them so.
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (turn) {
+            __syncthreads();
+            look_up(tile / kPieceTiles + 1);
+            __syncthreads();
+            bad = lds.any_bad != 0;
+        }
         if (more) K::load_keys(t, c, next, lane);
         f32x4 x[R][2];
 #pragma unroll
@@ -297,14 +317,14 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
                 for (int j = 0; j < 8; j++) {
                     const int n = n0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
                     x[i][j >> 2][j & 3] =
-                        __builtin_fmaf(-slope[i], fabsf((float)(row[i].pos - n)), x[i][j >> 2][j & 3]);
+                        __builtin_fmaf(-slope[i], fabsf((float)(row_at(i).pos - n)), x[i][j >> 2][j & 3]);
                 }
             }
             if (!whole) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int n = n0 + 16 * (j >> 2) + 4 * quarter + (j & 3);
-                    const bool on = n >= row[i].lo && n < row[i].hi && ((valid >> j) & 1);
+                    const bool on = n >= row_at(i).lo && n < row_at(i).hi && ((valid >> j) & 1);
                     if (!on) x[i][j >> 2][j & 3] = -INFINITY;
                 }
             }
@@ -366,10 +386,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     // The infinities and NaN that were left out, key by key.  Where the product had some in, they add nothing new.
     if (any_odd) {
 #pragma unroll 1
-        for (int tile = wave; tile < tiles; tile += kWaves)
+        for (int n0 = c0 + wave * kRowsTile; n0 < c1; n0 += kWaves * kRowsTile)
 #pragma unroll 1
-            for (int n = tile * kRowsTile; n < (tile + 1) * kRowsTile; n++) {
-                const int64_t at = lds.offsets[n];
+            for (int n = n0; n < min(n0 + kRowsTile, c1); n++) {
+                const int64_t at = key_offset(c, k.table, n, head, nullptr);
                 const uint8_t* from = c.v + (at < 0 ? 0 : at) + 4 * quarter * K::kDims * K::kSize;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -380,7 +400,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
                         const float x = T::unpack(pair & ~only_finite<T>(pair))[d & 1];
 #pragma unroll
                         for (int i = 0; i < R; i++)
-                            o[i][d][r] += at >= 0 && c0 + n >= row[i].lo && c0 + n < row[i].hi ? x : 0.f;
+                            o[i][d][r] += at >= 0 && n >= row_at(i).lo && n < row_at(i).hi ? x : 0.f;
                     }
                 }
             }
@@ -421,11 +441,11 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     if (wave != 0) return;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        if (row[i].t < 0) continue;
+        if (row_at(i).t < 0) continue;
         const int h = head_of(a, k, 16 * i + col, kv_head);
         if (st.direct && splits == 1) {
             const float w = sum[i] == 0.f ? 0.f : c.v_scale / sum[i];
-            uint16_t* out = a.out + row[i].t * a.out_stride + (int64_t)h * D + 4 * quarter * K::kDims;
+            uint16_t* out = a.out + row_at(i).t * a.out_stride + (int64_t)h * D + 4 * quarter * K::kDims;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -435,10 +455,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
                     *(u32x2*)(out + r * K::kDims + d) = sum[i] == 0.f ? u32x2{0, 0} : y;
                 }
             if (a.lse && quarter == 0)
-                a.lse[(int64_t)row[i].t * a.q_heads + h] =
+                a.lse[(int64_t)row_at(i).t * a.q_heads + h] =
                     sum[i] == 0.f ? -INFINITY : (m[i] * factor + shift + __builtin_amdgcn_logf(sum[i])) * kLn2;
         } else {
-            const int64_t at = slot_of(a, st.first_slot + split, row[i].t, h);
+            const int64_t at = slot_of(a, st.first_slot + split, row_at(i).t, h);
             if (quarter == 0) a.part_ml[at] = f32x2{m[i] * factor + shift, sum[i]};
             float* out = a.part_o + at * D + 4 * quarter * K::kDims;
             if (sum[i] == 0.f) continue;  // its weight is zero and it is not read
@@ -452,11 +472,11 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     }
 }
 
-template <typename T, typename S, int D, int R, int kWaves>
+template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
 __global__ __launch_bounds__(64 * kWaves, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(
     Call a, Cache c, Stage prefix, Stage own) {
     __shared__ RowsLds<T, S, D, R, kWaves> lds;
-    attend_rows<T, S, D, R, kWaves>(a, c, prefix, own, (int)blockIdx.x, lds);
+    attend_rows<T, S, D, R, kWaves, kPieces>(a, c, prefix, own, (int)blockIdx.x, lds);
 }
 
 template <typename T, typename S>
@@ -466,8 +486,10 @@ int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage&
     const auto go = [&](auto kernel) { return start(kernel, grid, 64 * waves, st, a, c, prefix, own); };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (waves == 1) return wide ? go(attend_rows_kernel<T, S, D, 2, 1>) : go(attend_rows_kernel<T, S, D, 1, 1>);
-        return wide ? go(attend_rows_kernel<T, S, D, 2, 4>) : go(attend_rows_kernel<T, S, D, 1, 4>);
+        if (waves == 1) return wide ? go(attend_rows_kernel<T, S, D, 2, 1, false>) : go(attend_rows_kernel<T, S, D, 1, 1, false>);
+        if (std::max(prefix.chunk, own.chunk) > kRowsPiece)
+            return wide ? go(attend_rows_kernel<T, S, D, 2, 4, true>) : go(attend_rows_kernel<T, S, D, 1, 4, true>);
+        return wide ? go(attend_rows_kernel<T, S, D, 2, 4, false>) : go(attend_rows_kernel<T, S, D, 1, 4, false>);
     };
     if (dim == 64) return pick(std::integral_constant<int, 64>());
     if (dim == 128) return pick(std::integral_constant<int, 128>());

@@ -356,8 +356,8 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
     return w & ~(bad * 0xFFFFu);
 }
 
-// Few rows (attend_rows.h): a range has at most so many keys.
-constexpr int kRowsMaxChunk = 1024;
+// Few rows (attend_rows.h): a workgroup has the offsets of so many keys at a time.
+constexpr int kRowsPiece = 1024;
 constexpr int kRowsShort = 128;  // with one wave
 template <typename T, typename S>
 int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,

@@ -101,7 +101,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // lengths spread best over kRounds rounds of them (64 of up to 8192 keys: ranges of 1024 163 us, of 512 173),
 // but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
 // below one round the shortest range, a tile per wave, counts.
-constexpr int kRound = 512, kRounds = 4, kMinChunk = 128, kGoodChunk = 512;
+// Past kMostRounds ranges grow instead, walked in pieces: a full card gains nothing from more of them, and what they
+// leave to be joined would grow with the context (512 of 131072 keys: 1.1 GB in ranges of one piece, 17 MB so).
+// 64 of up to 32768: 616 us, in ranges of one piece 634; 512 of up to 4096, whole 515, 520.
+constexpr int kRound = 512, kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512;
 // From so many workgroups on (one round of four waves), short contexts get a wave each: of four waves most would
 // find no tile or one, and what takes the time is a workgroup's start (91 times 12 heads of 256 dims and 27 keys:
 // 46 us, with one wave 17; 70 times 8 heads of 128 dims and 128 keys: 15.2, 12.7).
@@ -118,7 +121,9 @@ void split(Stage* st, int64_t items, int64_t keys, bool few) {
             return ceil_div(ceil_div(keys * items, groups), kMinChunk) * kMinChunk;
         };
         const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(kRound)));
-        st->chunk = (int)std::min<int64_t>(kRowsMaxChunk, std::max(least, chunk_for(kRound * kRounds)));
+        const int64_t spread = std::min<int64_t>(kRowsPiece, std::max(least, chunk_for(kRound * kRounds)));
+        const int64_t whole = std::max<int64_t>(1, ceil_div(keys, kMinChunk)) * kMinChunk;
+        st->chunk = (int)std::min(whole, std::max(spread, chunk_for(kRound * kMostRounds)));
     } else {
         const int64_t fill = st->prefix ? kCus : 2 * kCus;
         const int64_t parts = items * 2 > kCus ? 1 : fill / std::max<int64_t>(items, 1);
@@ -194,6 +199,10 @@ int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st
     int rc;
     if (p.own_waves) {  // both stages have blocks of the same rows
         rc = launch_tiles<T, S>(a, c, p.prefix, p.own, dim, p.own_waves, st);
+    } else if (p.prefix_waves && p.own.chunk > kRowsPiece) {  // a batch that fills the card without the prefix
+        const Stage none{0, 0, 0, 0, 1, 0, 0};
+        rc = launch_tiles<T, S>(a, c, p.prefix, none, dim, p.prefix_waves, st);
+        if (!rc) rc = launch_rows<T, S>(a, c, none, p.own, dim, p.rows == 32, p.few_waves, st);
     } else if (p.prefix_waves) {
         rc = launch_both<T, S>(a, c, p.prefix, p.own, dim, p.rows == 32, st);
     } else {

@@ -608,10 +608,15 @@ typedef struct gfd_attention {
 
 /* Workspace that the next two need for such a call (prefix_len 0: the first);
  * -1: the call would be refused.  It holds what ranges of keys leave to be
- * joined, and depends on every size of the call (a batch that fills the card
- * by itself needs none), so a program keeps the largest of its calls' values;
- * a call that is given less is refused.  16-byte aligned; what it holds before
- * and after a call does not matter, but calls that may run at the same time need one each. */
+ * joined.  It depends on every size of the call and is not the largest for the
+ * largest batch (one that fills the card without ranges needs none), so a
+ * program keeps the largest of its calls' values, or asks for each call; a
+ * call that is given less is refused.  It is never more than
+ *   4 (head_dim + 2) num_q_heads num_tokens n + 4 num_heads (batch + num_tokens num_q_heads / num_heads / 128)
+ * with n = 1 + 8192 / (batch num_heads) ranges a row, and 1 + 256 / num_heads
+ * more with a prefix (1 + 8192 / num_heads up to 32 rows of a head in all).
+ * 16-byte aligned; what it holds before and after a call does not matter, but
+ * calls that may run at the same time need one each. */
 int64_t gfd_attention_workspace_bytes(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len);
 int gfd_paged_attention(const gfd_kv_cache* cache, const gfd_attention* call, void* workspace,
                         size_t workspace_bytes, int* error_flag, void* stream);
