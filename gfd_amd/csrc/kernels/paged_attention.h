@@ -65,7 +65,7 @@ struct Row {
 
 // Tokens of sequence b that the call covers.
 struct Sequence {
-    int first, q_len, rows_q, kv_len;  // rows_q: at most max_q_len
+    int first, q_len, rows_q, kv_len;  // rows_q: at most max_q_len; kv_len as given: positions count from it
     bool cut;
 };
 
@@ -74,7 +74,7 @@ __device__ __forceinline__ Sequence sequence(const Call& a, int start, int end, 
     s.first = min(max(start, 0), a.num_tokens);
     s.q_len = min(max(end, s.first), a.num_tokens) - s.first;
     s.rows_q = min(s.q_len, a.max_q_len);
-    s.kv_len = max(min(kv_len, a.max_kv_len), 0);
+    s.kv_len = max(kv_len, 0);
     s.cut = s.q_len > a.max_q_len || kv_len > a.max_kv_len;
     return s;
 }
@@ -87,8 +87,8 @@ __device__ __forceinline__ Row make_row(const Call& a, const Sequence& s, int i,
     r.t = s.first + i;
     r.pos = s.kv_len - s.q_len + i;
     r.lo = a.doc_start ? max(a.doc_start[r.t], 0) : 0;
-    if (a.window > 0) r.lo = max(r.lo, r.pos - a.window + 1);
-    r.hi = min(s.kv_len, a.prefix_end ? max(r.pos + 1, a.prefix_end[r.t]) : r.pos + 1);
+    if (a.window > 0 && r.pos >= a.window) r.lo = max(r.lo, r.pos - a.window + 1);
+    r.hi = min(min(s.kv_len, a.max_kv_len), a.prefix_end ? max(r.pos + 1, a.prefix_end[r.t]) : r.pos + 1);
     if (prefix) {
         r.hi = min(r.hi, a.prefix_len);
     } else {

@@ -262,7 +262,7 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     const float factor = (cap_small ? 2.f * w.softcap : raw) * kLog2e, shift = cap_small ? w.softcap * kLog2e : 0.f;
     const Call a{(const uint16_t*)w.q, (uint16_t*)w.out, w.lse, w.q_stride, w.out_stride, w.q_start, w.kv_len,
                  w.block_table, w.table_stride, prefix_table, prefix_len, w.doc_start, w.prefix_end, w.slopes, factor, shift,
-                 cap_in, cap_out, cap_small, std::min(w.window, 1 << 30), w.batch, w.num_tokens, w.max_q_len, w.max_kv_len,
+                 cap_in, cap_out, cap_small, w.window, w.batch, w.num_tokens, w.max_q_len, w.max_kv_len,
                  w.num_q_heads, cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
     const hipStream_t st = (hipStream_t)stream;

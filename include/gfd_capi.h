@@ -543,7 +543,8 @@ typedef struct gfd_kv_cache {
 /* Bits of *error_flag (device int, zeroed by the caller; NULL: not reported). */
 enum {
     GFD_KV_ERR_PAGE = 1,   /* a slot or page outside the cache: not written, read as nothing */
-    GFD_KV_ERR_LENGTH = 2  /* a length past the maximum that the call stated: cut there */
+    GFD_KV_ERR_LENGTH = 2  /* a length past the maximum that the call stated: keys past max_kv_len count as nothing
+                              (positions stay kv_len's), out and lse of tokens past max_q_len are not written */
 };
 
 /* The tokens of one step: rows of num_q_heads (k, v: the cache's num_heads)
