@@ -227,6 +227,9 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
     if (prefix_len < 0 || prefix_len > (1 << 30)) return "prefix_len out of range";
     if (!(w.softcap >= 0.f) || w.softcap > 3.4e38f) return "softcap is negative or not finite";
     if (!(w.scale > 0.f) || w.scale > 3.4e38f) return "scale is not positive and finite";
+    // Scores are kept in units of the product with the stored keys: the factor between must not leave 32 bits.
+    const double raw = (double)w.scale * (cache->dtype == GFD_E4M3 ? cache->k_scale : 1.f);
+    if (raw < 0x1p-100 || raw > 0x1p100) return "scale times k_scale is outside 2^-100 to 2^100";
     if (w.window < 0) return "negative window";
     if ((w.q_stride | w.out_stride) % 8 != 0 || ((uintptr_t)w.q | (uintptr_t)w.out) % 16 != 0)
         return "rows' pointers or strides are not multiples of 16 bytes";

@@ -583,6 +583,7 @@ int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows, int* error
  *   hi = min(kv_len[b], max(p + 1, prefix_end[token]))   (prefix_end NULL: p + 1)
  * with the score
  *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;  s -= slopes[head] |p - j| if slopes
+ * (scale, times the k_scale of an 8-bit cache, is within 2^-100 to 2^100)
  * (a cap of any size: off by 2^-22 of the cap up to 64 and of the score above, so one far above the scores changes nothing)
  * out = sum of softmax(s) v (zeros where nothing is visible), lse = the
  * natural logarithm of the sum of exp(s) (-inf there; NULL: not wanted).

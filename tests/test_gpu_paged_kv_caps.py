@@ -87,3 +87,10 @@ def test_caps_of_every_type(q, kv, d, dtype, cache, softcap):
 @pytest.mark.parametrize("q,kv", [([1, 1], [40, 3]), ([40], [40])], ids=["few", "many"])
 def test_the_smallest_cap_leaves_the_mean(q, kv):
     check(72, q, kv, 1e-40)
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("q,kv", [([1, 1], [40, 3]), ([40], [40])], ids=["few", "many"])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -60])
+def test_the_smallest_scales(q, kv, scale, slopes):
+    check(73, q, kv, 1e4, slopes=slopes, scale=scale)
