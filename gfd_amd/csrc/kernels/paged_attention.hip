@@ -97,35 +97,44 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Few rows: two workgroups of a range each fit a CU, kRound the card.  Sequences of very different
+// Workgroups of four waves that fit a CU: two, but one of 256 dims, whose outputs take the registers of two waves a
+// SIMD (not so for up to 16 rows of an 8-bit cache).
+constexpr int kCus = 256;
+int fit_cu(int dim, bool few, int rows, int dtype) {
+    return dim != 256 || (few && rows == 16 && dtype == GFD_E4M3) ? 2 : 1;
+}
+// Few rows: a round is what fits the card at once.  Sequences of very different
 // lengths spread best over kRounds rounds of them (64 of up to 8192 keys: ranges of 1024 163 us, of 512 173),
 // but a range of a few hundred keys is half start-up (8 of 8192: ranges of 256 64 us, of 512 57), and
-// below one round the shortest range, a tile per wave, counts.
+// below one round the shortest range, a tile per wave, counts.  256 dims: one sequence of 8000 keys 24.6 us, with
+// rounds of two workgroups a CU 33.7; two times 5 tokens 36.4, 48.6; 8 sequences of 3000 54, 49.
 // Past kMostRounds ranges grow instead, walked in pieces: a full card gains nothing from more of them, and what they
 // leave to be joined would grow with the context (512 of 131072 keys: 1.1 GB in ranges of one piece, 17 MB so).
 // 64 of up to 32768: 616 us, in ranges of one piece 634; 512 of up to 4096, whole 515, 520.
-constexpr int kRound = 512, kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512;
-// From so many workgroups on (one round of four waves), short contexts get a wave each: of four waves most would
+constexpr int kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512;
+// From so many workgroups on (two a CU), short contexts get a wave each: of four waves most would
 // find no tile or one, and what takes the time is a workgroup's start (91 times 12 heads of 256 dims and 27 keys:
 // 46 us, with one wave 17; 70 times 8 heads of 128 dims and 128 keys: 15.2, 12.7).
 constexpr int kOneWave = 512;
 // Many rows: what ranges leave has to be joined, so blocks are split only where they leave half of the CUs empty,
-// and not below 4 tiles.  Then two workgroups a CU (4 times 60 tokens over 4000 keys: 33 us, with one 36; 1000
+// and not below 4 tiles.  Then as many workgroups as fit a CU (4 times 60 tokens over 4000 keys: 33 us, with one 36; 1000
 // tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
-// of the CUs one (64 requests on 32768 shared keys: 92 us, with two 101).
-constexpr int kCus = 256, kTilesMinChunk = 256;
+// of the CUs one (64 requests on 32768 shared keys: 92 us, with two 101).  256 dims: 100 tokens over 4196 keys 54 us,
+// with two workgroups a CU 69; 512 over 2048 84, 98; a prefix of 32768 for 64 requests 160, with two 183.
+constexpr int kTilesMinChunk = 256;
 
-void split(Stage* st, int64_t items, int64_t keys, bool few) {
+void split(Stage* st, int64_t items, int64_t keys, bool few, int fit) {
     if (few) {
+        const int64_t round = (int64_t)fit * kCus;
         const auto chunk_for = [&](int64_t groups) {
             return ceil_div(ceil_div(keys * items, groups), kMinChunk) * kMinChunk;
         };
-        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(kRound)));
-        const int64_t spread = std::min<int64_t>(kRowsPiece, std::max(least, chunk_for(kRound * kRounds)));
+        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(round)));
+        const int64_t spread = std::min<int64_t>(kRowsPiece, std::max(least, chunk_for(round * kRounds)));
         const int64_t whole = std::max<int64_t>(1, ceil_div(keys, kMinChunk)) * kMinChunk;
-        st->chunk = (int)std::min(whole, std::max(spread, chunk_for(kRound * kMostRounds)));
+        st->chunk = (int)std::min(whole, std::max(spread, chunk_for(round * kMostRounds)));
     } else {
-        const int64_t fill = st->prefix ? kCus : 2 * kCus;
+        const int64_t fill = st->prefix ? kCus : fit * kCus;
         const int64_t parts = items * 2 > kCus ? 1 : fill / std::max<int64_t>(items, 1);
         st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
     }
@@ -154,7 +163,8 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.rows = 32 * p.own_waves;
         p.own.blocks = (int)std::min<int64_t>(w.batch * ceil_div(seq_rows, p.rows), all_rows / p.rows + w.batch);
     }
-    split(&p.own, p.own.blocks * heads, keys, !p.own_waves);
+    const auto fit = [&](bool few) { return fit_cu(cache.head_dim, few, p.rows, cache.dtype); };
+    split(&p.own, p.own.blocks * heads, keys, !p.own_waves, fit(!p.own_waves));
     p.few_waves = 4;
     if (!p.own_waves && !prefix_len && keys <= kRowsShort && p.own.blocks * heads >= kOneWave) {
         p.few_waves = 1;
@@ -166,7 +176,7 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.prefix.prefix = 1;
         p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : 4;
         p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
-        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves);
+        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves));
         p.own.first_slot = p.prefix.splits;
     }
     p.slots = p.own.first_slot + p.own.splits;

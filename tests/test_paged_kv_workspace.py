@@ -50,3 +50,12 @@ def test_no_size_needs_more_than_the_bound():
         extra = rng.choice([{}, dict(window=int(2 ** rng.uniform(0, 14)))])
         n = need(batch, q, kv, heads * group, heads, dim, prefix, tokens, **extra)
         assert n <= bound(batch, q, heads * group, heads, dim, prefix, tokens), (batch, q, kv, heads, group, dim, prefix, tokens)
+
+
+@pytest.mark.parametrize("q_len,kv,rows", [(100, 4196, 128), (1, 8000, 16)])
+def test_ranges_of_256_dims_fill_the_card_once(q_len, kv, rows):
+    """One workgroup of 256 dims fits a CU, two of 128: ranges times blocks times heads are at most as many."""
+    for dim, fit in ((128, 2), (256, 1)):
+        blocks = -(-q_len * 4 // rows)
+        ranges = need(1, q_len, kv, dim=dim) // (4 * (dim + 2) * 32 * q_len)
+        assert 128 * fit < ranges * blocks * 8 <= 256 * fit
