@@ -1,8 +1,8 @@
 #pragma once
 // A shared prefix of many rows and what follows it with few, in one launch: the
 // prefix is bound by the matrix products and leaves half of each CU, which the rest, bound by the cache's bytes,
-// fills as it comes (64 requests on 32768 shared keys, when both were slower: 92 us, in two launches 107; 17 times 4
-// drafted tokens on 5001 shared 8-bit keys: 31 us, 44).  The prefix goes first: its workgroups are the long ones, and
+// fills as it comes (64 requests on 32768 shared keys: 91 us, in two launches 106; 17 times 4
+// drafted tokens on 5001 shared 8-bit keys: 30 us, 40).  The prefix goes first: its workgroups are the long ones, and
 // taking the two kinds by turns left one of them a CU (128 us).  Of 256 dims one workgroup fits a CU, and the rest
 // follows the prefix on the CUs that end first: it is as good as two launches (64 requests on 32768: 160 us, 156; 200 on
 // 16384: 345, 368; 17 times 4 tokens on 5001 in 8 bits: 61, 61).

@@ -21,9 +21,9 @@
 // undo it, a reload waits for every load: two waves a SIMD without spills take 165 us
 // where three with eight of them take 187.
 //
-// 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 371 us, 5.8 TB/s (a large read: 6.2).
-// 64 ragged contexts of up to 8192: 161 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
-// capped: 61 us, 4.8 TB/s.  700 keys of one token: 7.4 us and 3.4 to join, a chain of loads
+// 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 361 us, 5.9 TB/s (a large read: 6.2).
+// 64 ragged contexts of up to 8192: 160 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
+// capped: 60 us, 4.9 TB/s.  700 keys of one token: 7.6 us and 3.9 to join, a chain of loads
 // (lengths, pages, keys) and a launch each.  Many short contexts take a wave each: 128 of 128 keys in 16 us, 4.2 TB/s.
 #include <algorithm>
 #include <type_traits>

@@ -15,11 +15,13 @@
 // Chunks of 16 bytes are swapped by row, so that neither read finds two rows in a bank
 // (with a swap by 8 rows, 43% of the LDS's cycles were conflicts).
 //
-// 4096 tokens over 16384 keys, 32 heads of 128 in bf16: 945 us, 1020 TFLOP/s, where a library product of
-// 8192^3 reaches 1186 (the card's power holds both: 1.9 GHz with the matrix pipes at 45%,
-// and 1.6 to 1.9 GHz at 70%).  8192 packed tokens with capped scores: 211 us, 485 TFLOP/s; a cap costs
-// two more transcendental instructions a score, and the longest document's blocks end last.
-// 7 ragged prompts of 64 dims with a bias: 55 us, the 30 tiles of the longest one by 4 waves.
+// 4096 tokens over 16384 keys, 32 heads of 128 in bf16: 925 us, 1040 TFLOP/s, where a library product of
+// 8192^3 reaches 1186 (the card's power holds both: 1.9 GHz with the matrix pipes at 46%,
+// and 1.6 to 1.9 GHz at 70%).  8192 packed tokens with capped scores: 210 us, 485 TFLOP/s; a cap costs
+// two more transcendental instructions a score, and the longest document's blocks end last: with 1.5 waves a SIMD on
+// average neither pipe is full (20% and 31%), a wave waits 36% of its time for results.
+// 7 ragged prompts of 64 dims with a bias: 57 us, the 30 tiles of the longest one by 4 waves, one a SIMD, which waits
+// 47% of its time: a tile's scores, maximum, exponents and values follow one another, and nothing else is there.
 // Tried and slower: half of the waves a product behind the others (1130 us for 1096), tiles of 32 keys with
 // three under way (2048 tokens 85 us for 74), two groups of 4 waves to a block (packed tokens 263 us for 223).
 #include <type_traits>

@@ -324,7 +324,7 @@ template <>
 struct Mma<Fp16> {
     // This type holds 2^-14 to 2^16 in full, below in steps of 2^-24.  Weights use its upper end, so that those of
     // many keys far below a maximum are not lost: down to 2^-29 of the largest they are rounded relatively, and what a
-    // key loses below that is 2^-40 of the largest, or 2^-39 where scores may pass the maximum by 2^1.
+    // key loses below that is 2^-40 of the largest (2^-28 and 2^-39 where scores may pass the maximum by 2^1).
     // The small slack costs a few rescalings more: 7 ragged prompts of 64 dims 61 us, with 2^8 and no offset 59.5.
     static constexpr float kRaise = 15.f, kSlack = 1.f;
     static constexpr uint32_t kNear = 0x04000400u;

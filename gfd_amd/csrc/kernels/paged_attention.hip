@@ -117,9 +117,9 @@ constexpr int kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512;
 // 46 us, with one wave 17; 70 times 8 heads of 128 dims and 128 keys: 15.2, 12.7).
 constexpr int kOneWave = 512;
 // Many rows: what ranges leave has to be joined, so blocks are split only where they leave half of the CUs empty,
-// and not below 4 tiles.  Then as many workgroups as fit a CU (4 times 60 tokens over 4000 keys: 33 us, with one 36; 1000
+// and not below 4 tiles.  Then as many workgroups as fit a CU (4 times 60 tokens over 4000 keys: 31 us, with one 35; 1000
 // tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
-// of the CUs one (64 requests on 32768 shared keys: 92 us, with two 101).  256 dims: 100 tokens over 4196 keys 54 us,
+// of the CUs one (64 requests on 32768 shared keys: 91 us, with two 103).  256 dims: 100 tokens over 4196 keys 54 us,
 // with two workgroups a CU 69; 512 over 2048 84, 98; a prefix of 32768 for 64 requests 160, with two 183.
 constexpr int kTilesMinChunk = 256;
 
