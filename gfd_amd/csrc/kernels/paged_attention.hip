@@ -245,7 +245,9 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
         return "rows' pointers or strides are not multiples of 16 bytes";
     const int64_t pages = ((int64_t)std::max(w.max_kv_len - prefix_len, 0) + cache->page_size - 1) / cache->page_size;
     if (w.table_stride < pages) return "block_table's rows are shorter than max_kv_len needs";
-    if ((int64_t)w.num_tokens * w.num_q_heads > (1 << 30) || make_plan(*cache, w, prefix_len).threads >= kGridThreads)
+    // The first two keep the plan's products within 64 bits: a workgroup has a wave at least.
+    if ((int64_t)w.num_tokens * w.num_q_heads > (1 << 30) || (int64_t)w.batch * cache->num_heads >= kGridThreads / 64 ||
+        make_plan(*cache, w, prefix_len).threads >= kGridThreads)
         return "more work than one launch takes";
     return nullptr;
 }

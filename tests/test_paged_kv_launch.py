@@ -51,3 +51,13 @@ def test_the_largest_batch(sizes, largest, prefix):
 def test_a_workspace_is_stated_only_for_calls_that_are_taken():
     with pytest.raises(gfd_amd.GfdError, match="more work than one launch takes"):
         gfd_amd.attention_workspace_bytes(cache(), call(batch=1 << 21, num_tokens=64, max_kv_len=1000))
+
+
+@pytest.mark.parametrize("batch,heads", [(1 << 24, 65535), (1 << 24, 1 << 14), (1 << 20, 1 << 12), (1 << 24, 255), (1 << 11, 65535)])
+@pytest.mark.parametrize("kv", [1, 129, 1 << 30])
+@pytest.mark.parametrize("prefix,max_q", [(0, 1), (160, 1), (1 << 30, 1), (0, 1 << 24), (1 << 20, 500)])
+def test_products_of_the_largest_sizes_do_not_wrap(batch, heads, kv, prefix, max_q):
+    c = cache(num_heads=heads)
+    k = call(batch=batch, num_tokens=1, max_q_len=max_q, max_kv_len=kv, num_q_heads=heads, table_stride=1 << 27)
+    with pytest.raises(gfd_amd.GfdError, match="more work than one launch takes"):
+        gfd_amd.attention_workspace_bytes(c, k, prefix)
