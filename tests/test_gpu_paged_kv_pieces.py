@@ -30,7 +30,7 @@ def batch_of(rng, batch, q, hq, hk, d, dtype, cache, lengths, **kw):
     return pages, kv, lambda: Attend(rng, pages, [q] * batch, kv, hq, dtype, **kw)
 
 
-EDGES = [KV, 1, 1023, 1024, 1025, 1151, 1152, 1153, 2047, 2048, 2049, 2176, 2177, 2432, 2433, 3071, 3072, 3073, 3999]
+EDGES = [KV, 1, 1023, 1024, 1025, 1151, 1152, 1153, 2047, 2048, 2049, 2176, 2177, 2432, 2433, 3328, 3329, 3456, 3999]
 
 
 @pytest.mark.parametrize("batch", [1100, 2400, 5000])  # ranges of 1152 and 2432 keys, and whole contexts
