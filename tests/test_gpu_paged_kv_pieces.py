@@ -104,3 +104,31 @@ def test_a_prefix_before_ranges_of_several_pieces(batch):
     assert a.errors() == 0 and np.isfinite(out).all()
     close(out[:12], want, tol, "out")
     close(lse[:12], want_lse, tol_lse, "lse")
+
+
+@pytest.mark.parametrize("batch", [1, 9])
+def test_a_shared_prefix_in_pieces(batch):
+    """A prefix of 140800 keys whose table names the same ten pages again and again, with 64 heads: its ranges are of
+    more than a piece where few rows share it."""
+    rng = np.random.default_rng(94)
+    heads, d, page, times = 64, 64, 64, 220
+    period = 10 * page
+    prefix = period * times
+    pages = ref.Pages(rng, [1] * batch, page, heads, d, BF16, prefix=period)
+    pages.prefix_table = np.tile(pages.prefix_table, times)
+    a = Attend(rng, pages, [1] * batch, [prefix + 1] * batch, heads, BF16, prefix=prefix)
+    out, lse = a.run()
+    assert a.errors() == 0
+    for t in range(batch):
+        for h in range(0, heads, 7):
+            k, v = pages.k[t][:, h], pages.v[t][:, h]  # a period and the token's own key
+            s = k @ a.q[t, h] * float(np.float32(a.scale))
+            w = np.exp(s - s.max()) * np.r_[np.full(period, times), 1]
+            w, total = w / w.sum(), s.max() + np.log(w.sum())
+            # Scores: d + 8 steps of 2^-24 of their magnitudes, twice in a weight; sums over all keys in any order, one
+            # step for each of a wave's; weights and output rounded once.
+            err = (d + 8) * ref.F32 * (np.abs(k) @ np.abs(a.q[t, h]) * a.scale).max()
+            rel = 2 * err + (64 + 2 * 1152) * ref.F32
+            tol = 2.0 ** -8 * np.abs(w @ v) + (1.01 * 2.0 ** -8 + 1.01 * rel) * (w @ np.abs(v)) + 1e-30
+            close(out[t, h], w @ v, tol, "out")
+            assert abs(lse[t, h] - total) <= err + (16 + 2 * 1152) * ref.F32 * (1 + abs(total))
