@@ -19,7 +19,9 @@ __all__ = [
     "DescriptorQueue", "zero_copy_gather_tokens", "zero_copy_gather", "GfdError",
     "HOST_DEFAULT", "HOST_COHERENT", "HOST_NONCOHERENT", "HOST_NUMA_USER", "QUEUE_SIZE",
     "BF16", "FP16", "E4M3", "KVCache", "KVRows", "Attention", "kv_append", "paged_attention",
-    "shared_prefix_attention", "attention_workspace_bytes",
+    "shared_prefix_attention", "attention_workspace_bytes", "KV4Cache", "RotaryAxes", "KVRead", "kv_read", "KVPool",
+    "KVFork", "KVCompact", "PAGE_COPY_DTYPE", "kv_copy_pages", "kv_pool_workspace_bytes", "kv_fork", "kv_free",
+    "kv_compact",
 ]
 
 HOST_DEFAULT, HOST_COHERENT, HOST_NONCOHERENT, HOST_NUMA_USER = 0, 1, 2, 4
@@ -73,7 +75,7 @@ class DeviceSGEntry(ctypes.Structure):
 
 # Element types of the paged cache's operators, and the bits of their error word.
 BF16, FP16, E4M3 = 0, 1, 2
-KV_ERR_PAGE, KV_ERR_LENGTH = 1, 2
+KV_ERR_PAGE, KV_ERR_LENGTH, KV_ERR_AXIS, KV_ERR_ROW, KV_ERR_FULL, KV_ERR_REFS = 1, 2, 4, 8, 16, 32
 
 
 class KVCache(ctypes.Structure):
@@ -106,6 +108,60 @@ class Attention(ctypes.Structure):
                 ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int),
                 ("batch", ctypes.c_int), ("num_tokens", ctypes.c_int), ("max_q_len", ctypes.c_int),
                 ("max_kv_len", ctypes.c_int), ("num_q_heads", ctypes.c_int), ("dtype", ctypes.c_int)]
+
+
+class KV4Cache(ctypes.Structure):
+    """gfd_kv4_cache: keys and values in pages of 4-bit numbers with a scale per
+    32 of them (device pointers, strides in bytes).  Takes KVCache's place in
+    every function of the paged cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("page_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("scale_page_stride", ctypes.c_int64), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("num_heads", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class RotaryAxes(ctypes.Structure):
+    """gfd_rotary_axes: positions with several axes for kv_append()."""
+
+    _fields_ = [("positions", ctypes.c_void_p), ("axis", ctypes.c_void_p), ("axis_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("num_axes", ctypes.c_int), ("float_positions", ctypes.c_int)]
+
+
+class KVRead(ctypes.Structure):
+    """gfd_kv_read_rows: the tokens that kv_read() takes out of a cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_int64),
+                ("v_stride", ctypes.c_int64), ("slots", ctypes.c_void_p), ("num_tokens", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
+# gfd_kv_page_copy
+PAGE_COPY_DTYPE = np.dtype([("src", np.int32), ("dst", np.int32), ("slots", np.int32), ("reserved", np.int32)])
+
+
+class KVPool(ctypes.Structure):
+    """gfd_kv_pool: how many table entries name each page of a cache."""
+
+    _fields_ = [("refs", ctypes.c_void_p), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int)]
+
+
+class KVFork(ctypes.Structure):
+    """gfd_kv_fork_call: sequences that go on from others, begin or grow."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("child_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("child_stride", ctypes.c_int64), ("rows", ctypes.c_int), ("child_rows", ctypes.c_int),
+                ("parent", ctypes.c_void_p), ("child", ctypes.c_void_p), ("len", ctypes.c_void_p),
+                ("capacity", ctypes.c_void_p), ("copies", ctypes.c_void_p), ("num", ctypes.c_int)]
+
+
+class KVCompact(ctypes.Structure):
+    """gfd_kv_compact_call: a cache's tables before and after its pages are brought together."""
+
+    _fields_ = [("new_refs", ctypes.c_void_p), ("table", ctypes.c_void_p), ("new_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("new_stride", ctypes.c_int64), ("len", ctypes.c_void_p),
+                ("rows", ctypes.c_int), ("page_map", ctypes.c_void_p), ("copies", ctypes.c_void_p),
+                ("num_copies", ctypes.c_void_p)]
 
 
 DEVICE_SG_ENTRY_DTYPE = np.dtype([("src", np.uint64), ("dst", np.uint64), ("size", np.uint32), ("tag", np.uint32)])
@@ -266,6 +322,23 @@ def _declare(L):
         "gfd_paged_attention": ([ctypes.POINTER(KVCache), ctypes.POINTER(Attention), vp, c_sz, vp, vp], c_int),
         "gfd_shared_prefix_attention": ([ctypes.POINTER(KVCache), ctypes.POINTER(Attention), vp, c_int, vp, c_sz, vp,
                                          vp], c_int),
+        "gfd_kv_append_axes": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), ctypes.POINTER(RotaryAxes), vp, vp],
+                               c_int),
+        "gfd_kv4_append": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(KVRows), ctypes.POINTER(RotaryAxes), vp, vp],
+                           c_int),
+        "gfd_kv_read": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVRead), vp, vp], c_int),
+        "gfd_kv4_read": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(KVRead), vp, vp], c_int),
+        "gfd_kv4_attention_workspace_bytes": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(Attention), c_int],
+                                              ctypes.c_int64),
+        "gfd_kv4_attention": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(Attention), vp, c_sz, vp, vp], c_int),
+        "gfd_kv4_shared_prefix_attention": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(Attention), vp, c_int, vp, c_sz,
+                                             vp, vp], c_int),
+        "gfd_kv_copy_pages": ([ctypes.POINTER(KVCache), ctypes.POINTER(KVCache), vp, c_int, vp, vp, vp], c_int),
+        "gfd_kv4_copy_pages": ([ctypes.POINTER(KV4Cache), ctypes.POINTER(KV4Cache), vp, c_int, vp, vp, vp], c_int),
+        "gfd_kv_pool_workspace_bytes": ([ctypes.POINTER(KVPool), c_int], ctypes.c_int64),
+        "gfd_kv_fork": ([ctypes.POINTER(KVPool), ctypes.POINTER(KVFork), vp, c_sz, vp, vp], c_int),
+        "gfd_kv_free": ([ctypes.POINTER(KVPool), vp, ctypes.c_int64, c_int, vp, vp, c_int, vp, vp], c_int),
+        "gfd_kv_compact": ([ctypes.POINTER(KVPool), ctypes.POINTER(KVCompact), vp, c_sz, vp, vp], c_int),
         "gfd_bench_sg_session": ([vp, vp, c_u32, c_u32, c_int, c_int, pd], c_int),
     }
     for name, (args, res) in sig.items():
@@ -861,13 +934,35 @@ SgWarpSpecSession = SGWarpSpecSession
 
 # ------------------------------------------------ operators on the paged cache
 
-def kv_append(cache, rows, error_flag=None, stream=None):
-    """Rotate the queries and keys of `rows` (KVRows) to their positions and
-    append the keys and values to `cache` (KVCache).  error_flag: device int
-    that takes KV_ERR_* bits.  See gfd_kv_append in include/gfd_capi.h."""
-    rc = lib().gfd_kv_append(cache, rows, error_flag, stream)
+def _call(name, *args):
+    rc = getattr(lib(), name)(*args)
     if rc:
-        _check(rc, "gfd_kv_append")
+        _check(rc, name)
+
+
+def _bytes(name, *args):
+    n = getattr(lib(), name)(*args)
+    if n < 0:
+        _check(-1, name)
+    return n
+
+
+def kv_append(cache, rows, error_flag=None, stream=None, axes=None):
+    """Rotate the queries and keys of `rows` (KVRows) to their positions, or to
+    those of `axes` (RotaryAxes), and append the keys and values to `cache`
+    (KVCache or KV4Cache).  error_flag: device int that takes KV_ERR_* bits.  See gfd_kv_append,
+    gfd_kv_append_axes and gfd_kv4_append in include/gfd_capi.h."""
+    if isinstance(cache, KV4Cache):
+        _call("gfd_kv4_append", cache, rows, axes, error_flag, stream)
+    elif axes is not None:
+        _call("gfd_kv_append_axes", cache, rows, axes, error_flag, stream)
+    else:
+        _call("gfd_kv_append", cache, rows, error_flag, stream)
+
+
+def kv_read(cache, rows, error_flag=None, stream=None):
+    """Keys and values of slots of `cache` as rows (`rows`: KVRead); see gfd_kv_read in include/gfd_capi.h."""
+    _call("gfd_kv4_read" if isinstance(cache, KV4Cache) else "gfd_kv_read", cache, rows, error_flag, stream)
 
 
 def attention_workspace_bytes(cache, call, prefix_len=0):
@@ -875,27 +970,51 @@ def attention_workspace_bytes(cache, call, prefix_len=0):
     shared_prefix_attention() needs for `call` (Attention).  Depends on every
     size of the call and is not the largest for the largest batch: keep the
     largest of those that a program makes, or ask for each."""
-    n = lib().gfd_attention_workspace_bytes(cache, call, prefix_len)
-    if n < 0:
-        _check(-1, "gfd_attention_workspace_bytes")
-    return n
+    return _bytes("gfd_kv4_attention_workspace_bytes" if isinstance(cache, KV4Cache) else
+                  "gfd_attention_workspace_bytes", cache, call, prefix_len)
 
 
 def paged_attention(cache, call, workspace=None, workspace_bytes=0, error_flag=None, stream=None):
-    """Attention of `call` (Attention) over `cache` (KVCache); see gfd_paged_attention in include/gfd_capi.h."""
-    rc = lib().gfd_paged_attention(cache, call, workspace, workspace_bytes, error_flag, stream)
-    if rc:
-        _check(rc, "gfd_paged_attention")
+    """Attention of `call` (Attention) over `cache` (KVCache or KV4Cache); see
+    gfd_paged_attention and gfd_kv4_attention in include/gfd_capi.h."""
+    _call("gfd_kv4_attention" if isinstance(cache, KV4Cache) else "gfd_paged_attention", cache, call, workspace,
+          workspace_bytes, error_flag, stream)
 
 
 def shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace=None, workspace_bytes=0, error_flag=None,
                             stream=None):
     """paged_attention() of sequences whose first prefix_len keys are the same
     ones, in the pages of prefix_table; they are read once for all."""
-    rc = lib().gfd_shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace, workspace_bytes,
-                                           error_flag, stream)
-    if rc:
-        _check(rc, "gfd_shared_prefix_attention")
+    _call("gfd_kv4_shared_prefix_attention" if isinstance(cache, KV4Cache) else "gfd_shared_prefix_attention", cache,
+          call, prefix_table, prefix_len, workspace, workspace_bytes, error_flag, stream)
+
+
+def kv_copy_pages(dst, src, copies, max_copies, count=None, error_flag=None, stream=None):
+    """Copy pages of cache `src` to pages of `dst` (both KVCache or both KV4Cache, perhaps the same).  copies: device array
+    of PAGE_COPY_DTYPE, of which *count (device int; None: all) are done.  See gfd_kv_copy_pages in include/gfd_capi.h."""
+    _call("gfd_kv4_copy_pages" if isinstance(dst, KV4Cache) else "gfd_kv_copy_pages", dst, src, copies, max_copies,
+          count, error_flag, stream)
+
+
+def kv_pool_workspace_bytes(pool, num=0):
+    """Device bytes that kv_fork() of up to `num` items and kv_compact() need for `pool` (KVPool)."""
+    return _bytes("gfd_kv_pool_workspace_bytes", pool, num)
+
+
+def kv_fork(pool, call, workspace, workspace_bytes, error_flag=None, stream=None):
+    """Sequences that go on from others, begin or grow (`call`: KVFork): their tables and the counts of `pool` (KVPool).
+    What is then to be copied in each layer's cache is in call.copies.  See gfd_kv_fork in include/gfd_capi.h."""
+    _call("gfd_kv_fork", pool, call, workspace, workspace_bytes, error_flag, stream)
+
+
+def kv_free(pool, table, table_stride, rows, row, length, num, error_flag=None, stream=None):
+    """Let go of the pages of length[i] tokens of row[i] of a table (device arrays, num items)."""
+    _call("gfd_kv_free", pool, table, table_stride, rows, row, length, num, error_flag, stream)
+
+
+def kv_compact(pool, call, workspace, workspace_bytes, error_flag=None, stream=None):
+    """Bring the used pages of `pool` to its front (`call`: KVCompact); see gfd_kv_compact in include/gfd_capi.h."""
+    _call("gfd_kv_compact", pool, call, workspace, workspace_bytes, error_flag, stream)
 
 
 def build(verbose=False):

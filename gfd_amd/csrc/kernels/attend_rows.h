@@ -40,18 +40,20 @@ struct Words {
     uint32_t w[N];
 };
 
-template <int N>  // words
-__device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
-    Words<N> r;
-    if constexpr (N == 1) {
+template <int kBytes>
+__device__ __forceinline__ Words<(kBytes + 3) / 4> load_words(const uint8_t* p) {
+    Words<(kBytes + 3) / 4> r;
+    if constexpr (kBytes == 2) {
+        r.w[0] = __builtin_nontemporal_load((const uint16_t*)p);
+    } else if constexpr (kBytes == 4) {
         r.w[0] = __builtin_nontemporal_load((const uint32_t*)p);
-    } else if constexpr (N == 2) {
+    } else if constexpr (kBytes == 8) {
         const u32x2 x = __builtin_nontemporal_load((const u32x2*)p);
         r.w[0] = x[0];
         r.w[1] = x[1];
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
+        for (int i = 0; i < kBytes / 4; i += 4) {
             const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + 4 * i));
 #pragma unroll
             for (int j = 0; j < 4; j++) r.w[i + j] = x[j];
@@ -62,24 +64,34 @@ __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
 
 template <typename T, typename S, int D, int R>
 struct RowsKernel {
-    static constexpr int kSize = S::kBytes;
+    static constexpr int kBits = S::kBits;
     static constexpr int kDims = D / 16;                   // a lane's dims of a value row
     static constexpr int kSteps = D / 32;                  // products per 16 keys
-    static constexpr int kKeyChunks = D * kSize / 16;      // of 16 bytes a key
+    static constexpr int kKeyChunks = D * kBits / 128;     // of 16 bytes a key
     static constexpr int kKeyLoads = kRowsTile * kKeyChunks / 64;
-    static constexpr int kValWords = kDims * kSize / 4;
+    static constexpr int kValBytes = kDims * kBits / 8;
+    static constexpr int kValWords = (kValBytes + 3) / 4;
     static constexpr int kAcc = kDims * 4;                 // a lane's outputs per 16 rows
     // 32 rows of 128 dims and more: with the rows' operand in registers too, a lane would need more than it has.
     static constexpr bool kLdsRows = (R == 2 && D >= 128) || D == 256;
+    // 4-bit keys: a lane has the scales of one group of dims, or two, of a key of each 16.
+    static constexpr int kKeyScales = kBits == 4 ? 2 * (D == 256 ? 2 : 1) : 0;
 
+    // A lane's dims of one key's values: of 4 bits all of one group.
+    struct Value : Words<kValWords> {
+        uint32_t scale;  // 4 bits: the byte
+    };
     struct Tile {
         u32x4 k[kKeyLoads];
-        Words<kValWords> v[8];
+        uint32_t k_scale[kKeyScales + 1];
+        Value v[8];
     };
 
-    // Dims of product step s and quarter g start here: a chunk of 16 bytes is one step's, or two steps'.
+    // Dims of product step s and quarter g start here: what a lane reads of a key at once, 16 bytes (8 of 64 4-bit dims),
+    // is 1 step's, 2 or 4 steps'.
+    static constexpr int kStepsPerChunk = kBits == 16 ? 1 : kBits == 8 || D == 64 ? 2 : 4;
     static __device__ __forceinline__ int step_dim(int s, int g) {
-        return kSize == 2 ? 32 * s + 8 * g : 64 * (s / 2) + 16 * g + 8 * (s % 2);
+        return 32 * (s / kStepsPerChunk * kStepsPerChunk) + 8 * kStepsPerChunk * g + 8 * (s % kStepsPerChunk);
     }
     // Where a key's chunk lies in the wave's LDS: neighbours are spread over the banks.
     static __device__ __forceinline__ int key_at(int key, int chunk) {
@@ -94,7 +106,16 @@ struct RowsKernel {
         for (int i = 0; i < kKeyLoads; i++) {
             const int n = i * 64 + lane;
             const int64_t o = off[n / kKeyChunks];
-            t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + (o < 0 ? 0 : o) + n % kKeyChunks * 16));
+            t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + row_offset<S>(c, o < 0 ? 0 : o) + n % kKeyChunks * 16));
+        }
+        if constexpr (kBits == 4) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int64_t o = off[16 * h + (lane & 15)];
+                const uint8_t* p = c.k_scales + scales_offset(c, o < 0 ? 0 : o) + (D == 64 ? lane >> 5 : lane >> 4);
+#pragma unroll
+                for (int n = 0; n < kKeyScales / 2; n++) t.k_scale[h * (kKeyScales / 2) + n] = p[4 * n];
+            }
         }
     }
     static __device__ __forceinline__ void store_keys(const Tile& t, u32x4* lds, int lane) {
@@ -110,35 +131,71 @@ struct RowsKernel {
         for (int j = 0; j < 8; j++) {
             const int64_t o = off[16 * (j >> 2) + 4 * (lane >> 4) + (j & 3)];
             valid |= (o >= 0) << j;
-            t.v[j] = load_words<kValWords>(c.v + (o < 0 ? 0 : o) + (lane & 15) * kDims * kSize);
+            t.v[j] = load_value(c, o < 0 ? 0 : o, lane & 15);
         }
         return valid;
     }
+    // The dims of a row that lane n of its 16 has.
+    static __device__ __forceinline__ Value load_value(const Cache& c, int64_t place, int n) {
+        Value v;
+        (Words<kValWords>&)v = load_words<kValBytes>(c.v + row_offset<S>(c, place) + n * kValBytes);
+        if constexpr (kBits == 4) v.scale = c.v_scales[scales_offset(c, place) + n * kDims / kGroup4];
+        return v;
+    }
 
-    // Keys' operands of step s (two steps for 8-bit keys) for 16 keys from first on.
-    static constexpr int kStepsPerChunk = kSize == 2 ? 1 : 2;
-    static __device__ __forceinline__ void key_frags(const u32x4* lds, int first, int s, int lane,
+    // Keys' operands of step s (and the others of its chunk) for 16 keys from first on.
+    static __device__ __forceinline__ void key_frags(const u32x4* lds, const uint32_t* scales, int first, int s, int lane,
                                                      u32x4 (&f)[kStepsPerChunk]) {
-        const u32x4 x = lds[key_at(first + (lane & 15), s / kStepsPerChunk * 4 + (lane >> 4))];
-        if constexpr (kSize == 2) {
-            f[0] = x;
-        } else {
+        const int key = first + (lane & 15), n = s / kStepsPerChunk;
+        if constexpr (kBits == 16) {
+            f[0] = lds[key_at(key, n * 4 + (lane >> 4))];
+        } else if constexpr (kBits == 8) {
+            const u32x4 x = lds[key_at(key, n * 4 + (lane >> 4))];
 #pragma unroll
             for (int i = 0; i < 2; i++)
                 f[i] = u32x4{Mma<T>::widen_lo(x[2 * i]), Mma<T>::widen_hi(x[2 * i]), Mma<T>::widen_lo(x[2 * i + 1]),
                              Mma<T>::widen_hi(x[2 * i + 1])};
+        } else {
+            const float scale = scale_of<T>(scales[first / 16 * (kKeyScales / 2) + n]);
+            uint32_t w[kStepsPerChunk];
+            if constexpr (D == 64) {
+                const u32x2 x = ((const u32x2*)(lds + key_at(key, lane >> 5)))[(lane >> 4) & 1];
+                w[0] = x[0], w[1] = x[1];
+            } else {
+                const u32x4 x = lds[key_at(key, n * 4 + (lane >> 4))];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = x[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kStepsPerChunk; i++) f[i] = widen4<T>(w[i], scale);
         }
     }
     // Word i of a value row in 16-bit pairs.
-    static __device__ __forceinline__ uint32_t value_pair(const Words<kValWords>& v, int i) {
-        if constexpr (kSize == 2) return v.w[i];
-        else return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
+    static __device__ __forceinline__ uint32_t value_pair(const Value& v, int i) {
+        if constexpr (kBits == 16) return v.w[i];
+        else if constexpr (kBits == 8) return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
+        else return widen4<T>(v.w[i / 4], i % 4, scale_of<T>(v.scale));
     }
-    // A word as it lies in the cache, infinities and NaN made zero.
-    static __device__ __forceinline__ uint32_t only_finite_word(uint32_t w) {
-        if constexpr (kSize == 2) return only_finite<T>(w);
-        const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // e4m3: all ones but the sign
-        return w & ~((nan >> 7) * 0xFFu);
+    // Values as they lie in the cache, all of them made zero, or the infinities and NaN.
+    static __device__ __forceinline__ void keep(Value& v, bool there) {
+#pragma unroll
+        for (int i = 0; i < kValWords; i++) v.w[i] = there ? v.w[i] : 0u;
+        if constexpr (kBits == 4) v.scale = there ? v.scale : 0u;
+    }
+    static __device__ __forceinline__ void keep_finite(Value& v) {
+        if constexpr (kBits == 4) {
+            keep(v, v.scale <= (uint32_t)ScaleRange<T>::kMost);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kValWords; i++) {
+                if constexpr (kBits == 16) {
+                    v.w[i] = only_finite<T>(v.w[i]);
+                } else {
+                    const uint32_t nan = ((v.w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // e4m3: all ones but the sign
+                    v.w[i] &= ~((nan >> 7) * 0xFFu);
+                }
+            }
+        }
     }
     static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b, int odd) {
         return __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
@@ -217,7 +274,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         const int n0 = c0 + piece * kPieceTiles * kRowsTile;
         const int most = (kPieces ? min(tiles - piece * kPieceTiles, kPieceTiles) : tiles) * kRowsTile;
         for (int n = tid; n < most; n += kThreads) {
-            const int64_t o = n0 + n < c1 ? key_offset(c, k.table, n0 + n, head, a.error) : -1;
+            const int64_t o = n0 + n < c1 ? key_place<S>(c, k.table, n0 + n, head, a.error) : -1;
             if (o < 0 && n0 + n < c1) lds.any_bad = 1;
             lds.offsets[n] = o;
         }
@@ -266,6 +323,9 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         const int64_t* next = lds.offsets + (kPieces ? (tile + kWaves) % kPieceTiles : tile + kWaves) * kRowsTile;
         if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
         K::store_keys(t, my_keys, lane);
+        uint32_t k_scale[K::kKeyScales + 1];
+#pragma unroll
+        for (int i = 0; i < K::kKeyScales; i++) k_scale[i] = t.k_scale[i];
         // Other lanes of the wave read them: its LDS accesses are in order, the compiler has to keep them so.
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -283,8 +343,8 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 #pragma unroll
         for (int s = 0; s < K::kSteps; s += K::kStepsPerChunk) {
             u32x4 k0[K::kStepsPerChunk], k1[K::kStepsPerChunk];
-            K::key_frags(my_keys, 0, s, lane, k0);
-            K::key_frags(my_keys, 16, s, lane, k1);
+            K::key_frags(my_keys, k_scale, 0, s, lane, k0);
+            K::key_frags(my_keys, k_scale, 16, s, lane, k1);
 #pragma unroll
             for (int j = 0; j < K::kStepsPerChunk; j++)
 #pragma unroll
@@ -358,17 +418,14 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             uint32_t odd = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-#pragma unroll
-                for (int i = 0; i < K::kValWords; i++) t.v[j].w[i] = (valid >> j) & 1 ? t.v[j].w[i] : 0u;
+                K::keep(t.v[j], (valid >> j) & 1);
 #pragma unroll
                 for (int i = 0; i < K::kDims / 2; i++) odd |= not_finite<T>(K::value_pair(t.v[j], i));
             }
             if (__any(odd != 0)) {
                 any_odd = true;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int i = 0; i < K::kValWords; i++) t.v[j].w[i] = K::only_finite_word(t.v[j].w[i]);
+                for (int j = 0; j < 8; j++) K::keep_finite(t.v[j]);
             }
         }
 #pragma unroll
@@ -389,11 +446,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         for (int n0 = c0 + wave * kRowsTile; n0 < c1; n0 += kWaves * kRowsTile)
 #pragma unroll 1
             for (int n = n0; n < min(n0 + kRowsTile, c1); n++) {
-                const int64_t at = key_offset(c, k.table, n, head, nullptr);
-                const uint8_t* from = c.v + (at < 0 ? 0 : at) + 4 * quarter * K::kDims * K::kSize;
+                const int64_t at = key_place<S>(c, k.table, n, head, nullptr);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const auto v = load_words<K::kValWords>(from + r * K::kDims * K::kSize);
+                    const auto v = K::load_value(c, at < 0 ? 0 : at, 4 * quarter + r);
 #pragma unroll
                     for (int d = 0; d < K::kDims; d++) {
                         const uint32_t pair = K::value_pair(v, d / 2);
@@ -473,7 +529,7 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 }
 
 template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
-__global__ __launch_bounds__(64 * kWaves, D == 256 && (R == 2 || S::kBytes == 2) ? 1 : 2) void attend_rows_kernel(
+__global__ __launch_bounds__(64 * kWaves, D == 256 && (R == 2 || S::kBits == 16) ? 1 : 2) void attend_rows_kernel(
     Call a, Cache c, Stage prefix, Stage own) {
     __shared__ RowsLds<T, S, D, R, kWaves> lds;
     attend_rows<T, S, D, R, kWaves, kPieces>(a, c, prefix, own, (int)blockIdx.x, lds);

@@ -40,10 +40,11 @@ struct TilesKernel {
     static constexpr int kChunks = D / 8;  // of 8 elements a row
     static constexpr int kUnits = kTile * kChunks / kThreads;
     static_assert(kUnits >= 1, "a thread moves a chunk at least");
-    static constexpr int kUnitWords = 2 * S::kBytes;
+    static constexpr int kUnitWords = S::kBits / 4;
 
     struct Staged {
         uint32_t k[kUnits][kUnitWords], v[kUnits][kUnitWords];
+        uint32_t k_scale[S::kBits == 4 ? kUnits : 1], v_scale[S::kBits == 4 ? kUnits : 1];  // 4 bits: of the chunks' groups
     };
     // A thread moves the same chunk of every kStride-th row.
     static constexpr int kStride = kThreads / kChunks;
@@ -55,12 +56,18 @@ struct TilesKernel {
     static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 
     // kc and vc: the thread's chunk of the cache's first row.
-    static __device__ __forceinline__ void load(Staged& g, const uint8_t* kc, const uint8_t* vc, const int64_t* off,
-                                                int tid) {
+    static __device__ __forceinline__ void load(Staged& g, const Cache& c, const uint8_t* kc, const uint8_t* vc,
+                                                const int64_t* off, int tid) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int64_t o = off[tid / kChunks + u * kStride];
-            if constexpr (S::kBytes == 2) {
+            const int64_t place = off[tid / kChunks + u * kStride], o = row_offset<S>(c, place);
+            if constexpr (S::kBits == 4) {
+                const int64_t at = scales_offset(c, place) + tid % kChunks * 8 / kGroup4;
+                g.k[u][0] = *(const uint32_t*)(kc + o);
+                g.v[u][0] = *(const uint32_t*)(vc + o);
+                g.k_scale[u] = c.k_scales[at];
+                g.v_scale[u] = c.v_scales[at];
+            } else if constexpr (S::kBits == 16) {
                 const u32x4 k = *(const u32x4*)(kc + o), v = *(const u32x4*)(vc + o);
 #pragma unroll
                 for (int i = 0; i < 4; i++) g.k[u][i] = k[i], g.v[u][i] = v[i];
@@ -71,8 +78,9 @@ struct TilesKernel {
             }
         }
     }
-    static __device__ __forceinline__ u32x4 widened(const uint32_t (&w)[kUnitWords]) {
-        if constexpr (S::kBytes == 2) return u32x4{w[0], w[1], w[2], w[3]};
+    static __device__ __forceinline__ u32x4 widened(const uint32_t (&w)[kUnitWords], uint32_t scale) {
+        if constexpr (S::kBits == 4) return widen4<T>(w[0], scale_of<T>(scale));
+        else if constexpr (S::kBits == 16) return u32x4{w[0], w[1], w[2], w[3]};
         else return u32x4{Mma<T>::widen_lo(w[0]), Mma<T>::widen_hi(w[0]), Mma<T>::widen_lo(w[1]), Mma<T>::widen_hi(w[1])};
     }
     // Values of keys that are not there (there: not NULL if there may be such) become zeros; keys may be anything,
@@ -84,8 +92,8 @@ struct TilesKernel {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             const int row = tid / kChunks + u * kStride;
-            v[u] = widened(g.v[u]);
-            *(u32x4*)(kb + row * D + (chunk ^ swap_k(row)) * 8) = widened(g.k[u]);
+            v[u] = widened(g.v[u], g.v_scale[S::kBits == 4 ? u : 0]);
+            *(u32x4*)(kb + row * D + (chunk ^ swap_k(row)) * 8) = widened(g.k[u], g.k_scale[S::kBits == 4 ? u : 0]);
         }
         if (there) {
 #pragma unroll
@@ -124,7 +132,7 @@ struct TilesLds {
     };
     u32x4 values[2][K::kTile * D / 8];
     i32x4 rows[K::kRows];
-    int64_t offsets[4][K::kTile];  // of keys, 0 where none is
+    int64_t offsets[4][K::kTile];  // where keys lie, 0 where none is
     int there[4][K::kTile];
     int bad[8], odd[8], ranges[4][W];
 };
@@ -136,7 +144,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     constexpr int kTile = K::kTile, kRows = K::kRows;
     // Tiles under way: two where the registers hold them (4096 tokens over 16384 keys, 8 waves: 948 us, with one 1056).
     // 4 waves that move 128 dims of 16 bits hold one.
-    constexpr int kAhead = W == 8 || D == 64 || S::kBytes == 1 || (D == 256 && kScores != kBiased) ? 2 : 1;
+    constexpr int kAhead = W == 8 || D == 64 || S::kBits < 16 || (D == 256 && kScores != kBiased) ? 2 : 1;
     auto &keys_lds = lds.keys, &values_lds = lds.values;
     auto &rows = lds.rows;
     auto &offsets = lds.offsets;
@@ -250,13 +258,13 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     const auto whole = [&](const Range& x, int n0) { return x.all_lo <= n0 && n0 + kTile <= min(x.all_hi, c1); };
     for (int n = tid; n < 3 * kTile; n += K::kThreads) {
         const bool in = c0 + n < c1;
-        const int64_t at = in ? key_offset(c, k.table, c0 + n, head, a.error) : -1;
+        const int64_t at = in ? key_place<S>(c, k.table, c0 + n, head, a.error) : -1;
         if (in && at < 0) bad[n / kTile] = 1;
         offsets[n / kTile][n % kTile] = max(at, (int64_t)0);
         there[n / kTile][n % kTile] = at >= 0;
     }
-    const uint8_t* const kc = c.k + tid % K::kChunks * 8 * S::kBytes;
-    const uint8_t* const vc = c.v + tid % K::kChunks * 8 * S::kBytes;
+    const uint8_t* const kc = c.k + tid % K::kChunks * S::kBits;
+    const uint8_t* const vc = c.v + tid % K::kChunks * S::kBits;
     const auto place = [&](const typename K::Staged& x, int t) {  // tile t to LDS
         const int n0 = c0 + t * kTile;
         const bool full = n0 + kTile <= c1 && !bad[t & 7];
@@ -266,8 +274,8 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     };
     __syncthreads();
     if (tiles > 0) {
-        K::load(staged[0], kc, vc, offsets[0], tid);
-        if constexpr (kAhead == 2) K::load(staged[1], kc, vc, offsets[1], tid);
+        K::load(staged[0], c, kc, vc, offsets[0], tid);
+        if constexpr (kAhead == 2) K::load(staged[1], c, kc, vc, offsets[1], tid);
         place(staged[0], 0);
     }
     __syncthreads();
@@ -291,7 +299,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
         const auto page_of = [&](int n) { return c.page.div((uint32_t)min(n, c1 - 1)); };
         int id_look = 0;
         if (wave == 0) id_look = k.table[page_of(n_look)];
-        K::load(later, kc, vc, offsets[(t + kAhead) & 3], tid);
+        K::load(later, c, kc, vc, offsets[(t + kAhead) & 3], tid);
 
         if (odd[t & 7]) {
             // Of keys that some rows see and others do not, infinities and NaN reach only the rows
@@ -452,7 +460,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
                     bad[(t + 3) & 7] = 1;
                     if (a.error) atomicOr(a.error, GFD_KV_ERR_PAGE);
                 } else {
-                    at = id_look * c.page_stride + (int64_t)((uint32_t)n_look - page_of(n_look) * c.page.d) * c.slot_stride + head;
+                    at = place_of<S>(c, id_look, (uint32_t)n_look - page_of(n_look) * c.page.d, head);
                 }
             }
             if (lane < kTile) {

@@ -13,7 +13,7 @@
 
 #include "capi_error.h"
 #include "gfd_capi.h"
-#include "paged_kv.h"
+#include "kv_rows.h"
 
 namespace gfd {
 namespace kv {
@@ -34,11 +34,73 @@ const char* check_cache(const gfd_kv_cache* c) {
     return nullptr;
 }
 
+const char* check_cache(const gfd_kv4_cache* c) {
+    if (!c || !c->k || !c->v || !c->k_scales || !c->v_scales) return "no cache";
+    if (c->num_pages < 1 || c->page_size < 1 || c->page_size > 65536 || c->num_heads < 1 || c->num_heads > 65535)
+        return "cache sizes out of range";
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return "head_dim is not 64, 128 or 256";
+    if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 != 0 || (c->page_stride | c->slot_stride | c->head_stride) % 16 != 0)
+        return "cache pointers or strides are not multiples of 16 bytes";
+    const int64_t most = 0x7FFFFFFF;
+    for (const int64_t stride : {c->page_stride, c->slot_stride, c->head_stride, c->scale_page_stride}) {
+        if (stride < 0) return "negative cache stride";
+        if (stride > most) return "cache stride over 2^31 - 1";
+    }
+    if ((c->page_size - 1) * c->slot_stride + (c->num_heads - 1) * c->head_stride + c->head_dim / 2 > most + 1)
+        return "a page's rows do not end within 2^31 bytes";
+    return nullptr;
+}
+
+Cache make_cache(const gfd_kv4_cache& c) {
+    return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride, c.slot_stride, c.head_stride, c.num_pages,
+                 make_divider((uint32_t)c.page_size), 1.f, 1.f, (uint8_t*)c.k_scales, (uint8_t*)c.v_scales,
+                 c.scale_page_stride};
+}
+
 Cache make_cache(const gfd_kv_cache& c) {
     const int64_t size = c.dtype == GFD_E4M3 ? 1 : 2;
     const bool scaled = c.dtype == GFD_E4M3;
     return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride * size, c.slot_stride * size, c.head_stride * size,
-                 c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f};
+                 c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f,
+                 nullptr, nullptr, 0};
+}
+
+const char* check_rows(const gfd_kv_rows* rows, int head_dim, const gfd_rotary_axes* axes) {
+    if (!rows) return "no rows";
+    const gfd_kv_rows& w = *rows;
+    if (w.dtype != GFD_BF16 && w.dtype != GFD_FP16) return "rows are neither GFD_BF16 nor GFD_FP16";
+    if (w.num_tokens < 0) return "negative num_tokens";
+    if (((int64_t)w.num_tokens + kAppendTokens - 1) / kAppendTokens * kAppendBlock >= kGridThreads)
+        return "more work than one launch takes";
+    if (w.rotary_dim < 0 || w.rotary_dim > head_dim || w.rotary_dim % 2 != 0)
+        return "rotary_dim is odd or outside 0..head_dim";
+    if ((w.q != nullptr) != (w.q_out != nullptr)) return "q and q_out go together";
+    if (w.q && (w.num_q_heads < 1 || w.num_q_heads > 65535)) return "num_q_heads out of range";
+    if (((w.q ? w.q_stride | w.q_out_stride : 0) | w.k_stride | w.v_stride) % 8 != 0 ||
+        ((uintptr_t)w.q | (uintptr_t)w.q_out | (uintptr_t)w.k | (uintptr_t)w.v) % 16 != 0)
+        return "rows' pointers or strides are not multiples of 16 bytes";
+    if (axes && (axes->num_axes < 1 || axes->num_axes > 256)) return "num_axes is outside 1..256";
+    if (w.num_tokens == 0) return nullptr;
+    if (!w.k || !w.v || !w.slots || (w.rotary_dim && (!(axes ? axes->positions : w.positions) || !w.inv_freq)))
+        return "k, v, slots, positions or inv_freq is missing";
+    if (axes && w.rotary_dim && !axes->axis) return "axis is missing";
+    return nullptr;
+}
+
+Rows make_rows(const gfd_kv_rows& w, int num_heads, int head_dim, const gfd_rotary_axes* axes, float k_div, float v_div,
+               int* error) {
+    Rows r{(const uint16_t*)w.q, (const uint16_t*)w.k, (const uint16_t*)w.v, (uint16_t*)w.q_out, w.q_stride, w.k_stride,
+           w.v_stride, w.q_out_stride, w.positions, w.slots, w.inv_freq, w.num_tokens, w.q ? w.num_q_heads : 0,
+           num_heads, head_dim, w.rotary_dim, k_div, v_div, error, nullptr, nullptr, 0, 0, 0, 0};
+    if (axes) {
+        r.axes_positions = axes->positions;
+        r.axis = axes->axis;
+        r.axis_stride = axes->axis_stride;
+        r.token_stride = axes->token_stride;
+        r.num_axes = axes->num_axes;
+        r.float_positions = axes->float_positions;
+    }
+    return r;
 }
 
 int refused(const char* name, const char* why) {
@@ -59,21 +121,7 @@ int launched(const char* name, int rc) {
 
 namespace {
 
-struct Rows {
-    const uint16_t* q;
-    const uint16_t* k;
-    const uint16_t* v;
-    uint16_t* q_out;
-    int64_t q_stride, k_stride, v_stride, q_out_stride;
-    const int* positions;
-    const int64_t* slots;
-    const float* inv_freq;
-    int num_tokens, q_heads, kv_heads, dim, rotary;
-    float k_div, v_div;  // stored = x / div
-    int* error;
-};
-
-constexpr int kBlock = 256, kTokens = 4;
+constexpr int kBlock = kAppendBlock, kTokens = kAppendTokens;
 
 // Eight values to the stored type.
 template <typename T>
@@ -99,19 +147,6 @@ struct Store<E4m3> {
         *(u32x2*)p = u32x2{w[0], w[1]};
     }
 };
-
-template <typename T>
-__device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const f32x2 y = T::unpack(w[i]);
-        x[2 * i] = y[0];
-        x[2 * i + 1] = y[1];
-    }
-}
-
-// How the rotated pairs lie: side by side, a half apart in whole chunks of 8, or a half apart.
-enum { kSide, kChunksApart, kApart };
 
 // A workgroup takes kTokensHere tokens: their turns go to LDS, then each thread takes 16 values of a
 // head at a time, two chunks of 16 bytes.  A pair's two chunks are taken together; where
@@ -162,7 +197,7 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
 
     for (int n = tid; n < tokens * half; n += kBlock) {
         const int t = n / half, i = n - t * half;
-        const double whole = (double)r.positions[t0 + t] * ((double)r.inv_freq[i] * 0.15915494309189533577);
+        const double whole = position_of(r, t0 + t, i) * ((double)r.inv_freq[i] * 0.15915494309189533577);
         float s, co;
         sincospif((float)(2.0 * (whole - rint(whole))), &s, &co);
         turns[t][i] = f32x2{co, s};
@@ -250,9 +285,6 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
     }
 }
 
-constexpr char kName[] = "gfd_kv_append";
-int refuse(const char* why) { return refused(kName, why); }
-
 template <typename T, typename S, int kTokensHere>
 int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
     const dim3 grid((unsigned)((r.num_tokens + kTokensHere - 1) / kTokensHere));
@@ -268,40 +300,34 @@ int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
     return r.num_tokens >= 2048 * kTokens ? launch<T, S, kTokens>(r, c, pairs, st) : launch<T, S, 1>(r, c, pairs, st);
 }
 
+int append(const char* name, const gfd_kv_cache* cache, const gfd_kv_rows* rows, const gfd_rotary_axes* axes,
+           int* error_flag, void* stream) {
+    if (const char* why = check_cache(cache)) return refused(name, why);
+    if (const char* why = check_rows(rows, cache->head_dim, axes)) return refused(name, why);
+    const gfd_kv_rows& w = *rows;
+    if (cache->dtype != GFD_E4M3 && cache->dtype != w.dtype)
+        return refused(name, "the cache's type is neither the rows' nor GFD_E4M3");
+    if (w.num_tokens == 0) return 0;
+    const Rows r = make_rows(w, cache->num_heads, cache->head_dim, axes, cache->k_scale, cache->v_scale, error_flag);
+    const Cache c = make_cache(*cache);
+    const hipStream_t st = (hipStream_t)stream;
+    const bool pairs = w.interleaved != 0;
+    if (cache->dtype == GFD_E4M3)
+        return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(r, c, pairs, st)
+                                                  : launch<Fp16, E4m3>(r, c, pairs, st));
+    return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(r, c, pairs, st)
+                                              : launch<Fp16, Fp16>(r, c, pairs, st));
+}
+
 }  // namespace
 }  // namespace kv
 }  // namespace gfd
 
 extern "C" int gfd_kv_append(const gfd_kv_cache* cache, const gfd_kv_rows* rows, int* error_flag, void* stream) {
-    using namespace gfd::kv;
-    if (const char* why = check_cache(cache)) return refuse(why);
-    if (!rows) return refuse("no rows");
-    const gfd_kv_rows& w = *rows;
-    if (w.dtype != GFD_BF16 && w.dtype != GFD_FP16) return refuse("rows are neither GFD_BF16 nor GFD_FP16");
-    if (cache->dtype != GFD_E4M3 && cache->dtype != w.dtype) return refuse("the cache's type is neither the rows' nor GFD_E4M3");
-    if (w.num_tokens < 0) return refuse("negative num_tokens");
-    if (((int64_t)w.num_tokens + kTokens - 1) / kTokens * kBlock >= kGridThreads)
-        return refuse("more work than one launch takes");
-    if (w.rotary_dim < 0 || w.rotary_dim > cache->head_dim || w.rotary_dim % 2 != 0)
-        return refuse("rotary_dim is odd or outside 0..head_dim");
-    if ((w.q != nullptr) != (w.q_out != nullptr)) return refuse("q and q_out go together");
-    if (w.q && (w.num_q_heads < 1 || w.num_q_heads > 65535)) return refuse("num_q_heads out of range");
-    if (((w.q ? w.q_stride | w.q_out_stride : 0) | w.k_stride | w.v_stride) % 8 != 0 ||
-        ((uintptr_t)w.q | (uintptr_t)w.q_out | (uintptr_t)w.k | (uintptr_t)w.v) % 16 != 0)
-        return refuse("rows' pointers or strides are not multiples of 16 bytes");
-    if (w.num_tokens == 0) return 0;
-    if (!w.k || !w.v || !w.slots || (w.rotary_dim && (!w.positions || !w.inv_freq)))
-        return refuse("k, v, slots, positions or inv_freq is missing");
-    const Rows r{(const uint16_t*)w.q, (const uint16_t*)w.k, (const uint16_t*)w.v, (uint16_t*)w.q_out, w.q_stride,
-                 w.k_stride, w.v_stride, w.q_out_stride, w.positions, w.slots, w.inv_freq, w.num_tokens,
-                 w.q ? w.num_q_heads : 0, cache->num_heads, cache->head_dim, w.rotary_dim, cache->k_scale,
-                 cache->v_scale, error_flag};
-    const Cache c = make_cache(*cache);
-    const hipStream_t st = (hipStream_t)stream;
-    const bool pairs = w.interleaved != 0;
-    if (cache->dtype == GFD_E4M3)
-        return launched(kName, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(r, c, pairs, st)
-                                                   : launch<Fp16, E4m3>(r, c, pairs, st));
-    return launched(kName, w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(r, c, pairs, st)
-                                               : launch<Fp16, Fp16>(r, c, pairs, st));
+    return gfd::kv::append("gfd_kv_append", cache, rows, nullptr, error_flag, stream);
+}
+
+extern "C" int gfd_kv_append_axes(const gfd_kv_cache* cache, const gfd_kv_rows* rows, const gfd_rotary_axes* axes,
+                                  int* error_flag, void* stream) {
+    return gfd::kv::append("gfd_kv_append_axes", cache, rows, axes, error_flag, stream);
 }

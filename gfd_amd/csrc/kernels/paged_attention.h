@@ -223,15 +223,16 @@ __device__ __forceinline__ int head_of(const Call& a, const Block& k, int r, int
     return kv_head * (int)a.group.d + (int)(n - a.group.div(n) * a.group.d);
 }
 
-// Byte offset of a key, -1 where its page is none of the cache's.
-__device__ __forceinline__ int64_t key_offset(const Cache& c, const int* table, int n, int64_t head, int* error) {
+// Where a key lies, -1 where its page is none of the cache's.
+template <typename S>
+__device__ __forceinline__ int64_t key_place(const Cache& c, const int* table, int n, int64_t head, int* error) {
     const uint32_t page = c.page.div((uint32_t)n);
     const int id = table[page];
     if (id < 0 || id >= c.num_pages) {
         if (error) atomicOr(error, GFD_KV_ERR_PAGE);
         return -1;
     }
-    return id * c.page_stride + (int64_t)((uint32_t)n - page * c.page.d) * c.slot_stride + head;
+    return place_of<S>(c, id, (uint32_t)n - page * c.page.d, head);
 }
 
 __device__ __forceinline__ int64_t slot_of(const Call& a, int slot, int t, int h) {

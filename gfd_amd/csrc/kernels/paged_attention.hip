@@ -84,6 +84,20 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
     }
 }
 
+// A 4-bit cache's form, as the plan and the checks take it.
+constexpr int kE2m1 = -1;
+gfd_kv_cache form_of(const gfd_kv4_cache& c) {
+    gfd_kv_cache f{};
+    f.num_pages = c.num_pages;
+    f.page_size = c.page_size;
+    f.num_heads = c.num_heads;
+    f.head_dim = c.head_dim;
+    f.dtype = kE2m1;
+    f.k_scale = f.v_scale = 1.f;
+    return f;
+}
+gfd_kv_cache form_of(const gfd_kv_cache& c) { return c; }
+
 // How a call is cut into row blocks and key ranges.
 struct Plan {
     int prefix_waves, own_waves;  // of a block of 32 rows a wave; 0: few rows (attend_rows.h)
@@ -101,7 +115,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // SIMD (not so for up to 16 rows of an 8-bit cache).
 constexpr int kCus = 256;
 int fit_cu(int dim, bool few, int rows, int dtype) {
-    return dim != 256 || (few && rows == 16 && dtype == GFD_E4M3) ? 2 : 1;
+    return dim != 256 || (few && rows == 16 && (dtype == GFD_E4M3 || dtype == kE2m1)) ? 2 : 1;
 }
 // Few rows: a round is what fits the card at once.  Sequences of very different
 // lengths spread best over kRounds rounds of them (64 of up to 8192 keys: ranges of 1024 163 us, of 512 173),
@@ -223,12 +237,14 @@ int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st
                                                                    : launch_join<T, 256>(a, c, p, st);
 }
 
-const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len) {
-    if (const char* why = check_cache(cache)) return why;
+template <typename C>
+const char* check_call(const C* of, const gfd_attention* call, int prefix_len) {
+    if (const char* why = check_cache(of)) return why;
+    const gfd_kv_cache form = form_of(*of), *const cache = &form;
     if (!call) return "no call";
     const gfd_attention& w = *call;
     if (w.dtype != GFD_BF16 && w.dtype != GFD_FP16) return "q is neither GFD_BF16 nor GFD_FP16";
-    if (cache->dtype != GFD_E4M3 && cache->dtype != w.dtype) return "the cache's type is neither q's nor GFD_E4M3";
+    if (cache->dtype != GFD_E4M3 && cache->dtype != kE2m1 && cache->dtype != w.dtype) return "the cache's type is neither q's nor GFD_E4M3";
     if (w.num_q_heads < 1 || w.num_q_heads > 65535 || w.num_q_heads % cache->num_heads != 0)
         return "num_q_heads is no multiple of the cache's heads";
     if (w.batch < 0 || w.num_tokens < 0 || w.max_q_len < 0 || w.max_kv_len < 0 || w.max_kv_len > (1 << 30) ||
@@ -252,9 +268,11 @@ const char* check_call(const gfd_kv_cache* cache, const gfd_attention* call, int
     return nullptr;
 }
 
-int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* call, const int* prefix_table,
-              int prefix_len, void* workspace, size_t workspace_bytes, int* error_flag, void* stream) {
-    if (const char* why = check_call(cache, call, prefix_len)) return refused(name, why);
+template <typename C>
+int attention(const char* name, const C* of, const gfd_attention* call, const int* prefix_table, int prefix_len,
+              void* workspace, size_t workspace_bytes, int* error_flag, void* stream) {
+    if (const char* why = check_call(of, call, prefix_len)) return refused(name, why);
+    const gfd_kv_cache form = form_of(*of), *const cache = &form;
     const gfd_attention& w = *call;
     if (w.batch == 0 || w.num_tokens == 0 || w.max_q_len == 0) return 0;
     if (!w.q || !w.out || !w.q_start || !w.kv_len) return refused(name, "q, out, q_start or kv_len is missing");
@@ -262,12 +280,13 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
     if (!prefix_table && prefix_len > 0) return refused(name, "prefix_table is missing");
     const Plan p = make_plan(*cache, w, prefix_len);
     if (p.bytes && (!workspace || workspace_bytes < (size_t)p.bytes || (uintptr_t)workspace % 16 != 0))
-        return refused(name, "workspace is missing, not 16-byte aligned or smaller than gfd_attention_workspace_bytes says");
+        return refused(name, "workspace is missing, not 16-byte aligned or smaller than "
+                             "gfd_attention_workspace_bytes (4 bits: gfd_kv4_attention_workspace_bytes) says");
     const int64_t rows = (int64_t)w.num_tokens * w.num_q_heads;
     float* const part_o = p.bytes ? (float*)workspace : nullptr;
     float* const part_ml = p.bytes ? part_o + p.slots * rows * cache->head_dim : nullptr;
     float* const splits = p.bytes ? part_ml + p.slots * rows * 2 : nullptr;
-    const Cache c = make_cache(*cache);
+    const Cache c = make_cache(*of);
     const float raw = w.scale * c.k_scale;
     // Of a cap past what 32 bits hold of it, the quotients' ends: scores far below it stay as they are, others are +-cap_out.
     const auto held = [](double x) { return (float)std::min(x, 3.4028234e38); };
@@ -281,6 +300,9 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
                  w.num_q_heads, cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
     const hipStream_t st = (hipStream_t)stream;
+    if (cache->dtype == kE2m1)
+        return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E2m1>(a, c, p, cache->head_dim, st)
+                                                  : launch<Fp16, E2m1>(a, c, p, cache->head_dim, st));
     if (cache->dtype == GFD_E4M3)
         return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(a, c, p, cache->head_dim, st)
                                                   : launch<Fp16, E4m3>(a, c, p, cache->head_dim, st));
@@ -288,17 +310,21 @@ int attention(const char* name, const gfd_kv_cache* cache, const gfd_attention* 
                                               : launch<Fp16, Fp16>(a, c, p, cache->head_dim, st));
 }
 
+template <typename C>
+int64_t workspace_bytes(const char* name, const C* cache, const gfd_attention* call, int prefix_len) {
+    if (const char* why = check_call(cache, call, prefix_len)) {
+        refused(name, why);
+        return -1;
+    }
+    return make_plan(form_of(*cache), *call, prefix_len).bytes;
+}
+
 }  // namespace
 }  // namespace kv
 }  // namespace gfd
 
 extern "C" int64_t gfd_attention_workspace_bytes(const gfd_kv_cache* cache, const gfd_attention* call, int prefix_len) {
-    using namespace gfd::kv;
-    if (const char* why = check_call(cache, call, prefix_len)) {
-        refused("gfd_attention_workspace_bytes", why);
-        return -1;
-    }
-    return make_plan(*cache, *call, prefix_len).bytes;
+    return gfd::kv::workspace_bytes("gfd_attention_workspace_bytes", cache, call, prefix_len);
 }
 
 extern "C" int gfd_paged_attention(const gfd_kv_cache* cache, const gfd_attention* call, void* workspace,
@@ -311,5 +337,23 @@ extern "C" int gfd_shared_prefix_attention(const gfd_kv_cache* cache, const gfd_
                                            const int* prefix_table, int prefix_len, void* workspace,
                                            size_t workspace_bytes, int* error_flag, void* stream) {
     return gfd::kv::attention("gfd_shared_prefix_attention", cache, call, prefix_table, prefix_len, workspace,
+                              workspace_bytes, error_flag, stream);
+}
+
+extern "C" int64_t gfd_kv4_attention_workspace_bytes(const gfd_kv4_cache* cache, const gfd_attention* call,
+                                                     int prefix_len) {
+    return gfd::kv::workspace_bytes("gfd_kv4_attention_workspace_bytes", cache, call, prefix_len);
+}
+
+extern "C" int gfd_kv4_attention(const gfd_kv4_cache* cache, const gfd_attention* call, void* workspace,
+                                 size_t workspace_bytes, int* error_flag, void* stream) {
+    return gfd::kv::attention("gfd_kv4_attention", cache, call, nullptr, 0, workspace, workspace_bytes, error_flag,
+                              stream);
+}
+
+extern "C" int gfd_kv4_shared_prefix_attention(const gfd_kv4_cache* cache, const gfd_attention* call,
+                                               const int* prefix_table, int prefix_len, void* workspace,
+                                               size_t workspace_bytes, int* error_flag, void* stream) {
+    return gfd::kv::attention("gfd_kv4_shared_prefix_attention", cache, call, prefix_table, prefix_len, workspace,
                               workspace_bytes, error_flag, stream);
 }

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "gfd_capi.h"
 
@@ -22,7 +23,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // Element types: how a 32-bit word holds them.
 struct Bf16 {
-    static constexpr int kBytes = 2;
+    static constexpr int kBits = 16;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {  // nearest even
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
     }
@@ -31,7 +32,7 @@ struct Bf16 {
     }
 };
 struct Fp16 {
-    static constexpr int kBytes = 2;
+    static constexpr int kBits = 16;
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2));
     }
@@ -40,8 +41,58 @@ struct Fp16 {
     }
 };
 struct E4m3 {
-    static constexpr int kBytes = 1;
+    static constexpr int kBits = 8;
 };
+// 4-bit floats, kGroup4 of them with a power of two, whose exponent is a byte (255: NaN).
+struct E2m1 {
+    static constexpr int kBits = 4;
+};
+constexpr int kGroup4 = 32;
+constexpr int kScaleNan = 255;
+// The scales that an append writes: 6 times the largest is finite in the rows' type (8 times it would not be), half of
+// the least is the least that the type tells from zero (bf16: its least of full precision).
+template <typename T>
+struct ScaleRange;
+template <>
+struct ScaleRange<Bf16> {
+    static constexpr int kLeast = 1, kMost = 252;
+};
+template <>
+struct ScaleRange<Fp16> {
+    static constexpr int kLeast = 104, kMost = 140;
+};
+// A scale as the conversions take it.  One beyond what an append writes would leave some numbers of its group infinite and
+// others not: it is read as NaN, so that a group's numbers are finite all together or not at all.
+template <typename T>
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return __uint_as_float((byte > (uint32_t)ScaleRange<T>::kMost ? (uint32_t)kScaleNan : byte) << 23);
+}
+// Two numbers, byte `byte` of w, as a pair of T: the first in the low half of the byte and of the pair.
+template <typename T>
+__device__ __forceinline__ uint32_t widen4(uint32_t w, int byte, float scale) {
+    static_assert(std::is_same<T, Bf16>::value || std::is_same<T, Fp16>::value, "rows are bf16 or fp16");
+    if constexpr (std::is_same<T, Bf16>::value) {
+        const auto at = [&](auto b) {
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, decltype(b)::value));
+        };
+        return byte == 0   ? at(std::integral_constant<int, 0>())
+               : byte == 1 ? at(std::integral_constant<int, 1>())
+               : byte == 2 ? at(std::integral_constant<int, 2>())
+                           : at(std::integral_constant<int, 3>());
+    } else {
+        const auto at = [&](auto b) {
+            return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, decltype(b)::value));
+        };
+        return byte == 0   ? at(std::integral_constant<int, 0>())
+               : byte == 1 ? at(std::integral_constant<int, 1>())
+               : byte == 2 ? at(std::integral_constant<int, 2>())
+                           : at(std::integral_constant<int, 3>());
+    }
+}
+template <typename T>
+__device__ __forceinline__ u32x4 widen4(uint32_t w, float scale) {  // all eight
+    return u32x4{widen4<T>(w, 0, scale), widen4<T>(w, 1, scale), widen4<T>(w, 2, scale), widen4<T>(w, 3, scale)};
+}
 
 // n / d for 0 <= n < 2^31 by a multiplication: floor(n * mul / 2^(32 + shift))
 // with mul = ceil(2^(32 + shift) / d), shift = ceil(log2 d) - 1 (d = 1: n
@@ -70,7 +121,28 @@ struct Cache {
     int num_pages;
     Divider page;
     float k_scale, v_scale;  // 1 unless the type is E4M3
+    // Of 4-bit numbers: the scales, whose offset within a page is a 16th of the numbers'.
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    int64_t scale_page_stride;
 };
+
+// Where a row (slot and head of a page) of a cache of type S lies, as a number that is not negative: its byte offset, or
+// for 4-bit numbers, whose scales lie elsewhere, the page and the offset within it.
+template <typename S>
+__device__ __forceinline__ int64_t place_of(const Cache& c, int page, uint32_t slot, int64_t head) {
+    const int64_t in = slot * c.slot_stride + head;
+    if constexpr (S::kBits == 4) return (int64_t)page << 32 | in;
+    else return page * c.page_stride + in;
+}
+template <typename S>
+__device__ __forceinline__ int64_t row_offset(const Cache& c, int64_t place) {
+    if constexpr (S::kBits == 4) return (int64_t)(int)(place >> 32) * c.page_stride + (uint32_t)place;
+    else return place;
+}
+__device__ __forceinline__ int64_t scales_offset(const Cache& c, int64_t place) {
+    return (int64_t)(int)(place >> 32) * c.scale_page_stride + ((uint32_t)place >> 4);
+}
 
 // A launch has fewer threads along a grid than this.
 constexpr int64_t kGridThreads = 1ll << 32;
@@ -88,7 +160,9 @@ int launched(const char* name, int rc);
 
 // An argument that a kernel for the cache relies on, or NULL if all hold.
 const char* check_cache(const gfd_kv_cache* c);
+const char* check_cache(const gfd_kv4_cache* c);
 Cache make_cache(const gfd_kv_cache& c);
+Cache make_cache(const gfd_kv4_cache& c);
 
 }  // namespace kv
 }  // namespace gfd

@@ -631,6 +631,164 @@ int gfd_shared_prefix_attention(const gfd_kv_cache* cache, const gfd_attention* 
                                 int prefix_len, void* workspace, size_t workspace_bytes, int* error_flag,
                                 void* stream);
 
+/* ---- the paged cache in 4 bits, positions of several axes, and the cache's
+ * pages.  What is said above of every call of the paged cache's operators holds for these. ---- */
+
+/* A cache of 4-bit floats (OCP e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) with a power of two per 32 of them (OCP e8m0: 2^(byte - 127), 255: NaN).
+ * The numbers of slot s of page p, head h start at byte
+ *   p * page_stride + s * slot_stride + h * head_stride of k and of v:
+ * head_dim / 2 contiguous bytes, element 2 i in the low half of byte i.  Their
+ * head_dim / 32 scales start at byte
+ *   p * scale_page_stride + (s * slot_stride + h * head_stride) / 16 of k_scales and of v_scales,
+ * so scales lie as the numbers do, in the page's own block or in one apart: a page of
+ * 16 tokens of 8 heads of 128 is 16 KiB of numbers and 1 KiB of scales, in one piece for the
+ * gather if the strides say so.  k, v, page_stride, slot_stride and head_stride
+ * are multiples of 16; the strides are at most 2^31 - 1, and a page's rows
+ * end within 2^31 bytes of its first.  head_dim: 64, 128 or 256; page_size: 1 to 65536. */
+typedef struct gfd_kv4_cache {
+    void* k;
+    void* v;
+    void* k_scales;
+    void* v_scales;
+    int64_t page_stride, slot_stride, head_stride, scale_page_stride;  /* bytes */
+    int num_pages, page_size, num_heads, head_dim;
+} gfd_kv4_cache;
+
+/* More bits of *error_flag. */
+enum {
+    GFD_KV_ERR_AXIS = 4,  /* a pair of an axis that is none: it is not rotated */
+    GFD_KV_ERR_ROW = 8,   /* a row of a table that is none, or too short for its length: skipped */
+    GFD_KV_ERR_FULL = 16, /* no free page was left: entries of -1 */
+    GFD_KV_ERR_REFS = 32  /* a page freed more often than it was held: its count stays 0 */
+};
+
+/* Positions with several axes (time, height, width of images and video): pair i
+ * of a head turns by its own axis's position, positions[axis[i] * axis_stride +
+ * token * token_stride] * inv_freq[i].  gfd_kv_rows's positions are not read then. */
+typedef struct gfd_rotary_axes {
+    const void* positions;     /* int, or float with float_positions (finite) */
+    const uint8_t* axis;       /* [rotary_dim / 2] */
+    int64_t axis_stride, token_stride;  /* elements */
+    int num_axes;              /* 1 to 256 */
+    int float_positions;
+} gfd_rotary_axes;
+
+/* gfd_kv_append with such positions (axes NULL: gfd_kv_append itself). */
+int gfd_kv_append_axes(const gfd_kv_cache* cache, const gfd_kv_rows* rows, const gfd_rotary_axes* axes,
+                       int* error_flag, void* stream);
+/* The same into a 4-bit cache (axes NULL: the rows' positions).  A group's
+ * scale is the least power of two of which its largest magnitude is at most seven,
+ * its numbers are the nearest multiples, ties to even, of magnitudes up to 6 (what lies between 6 and 7 is off by no more
+ * than elsewhere between 4 and 6).  Scales are kept to 2^-126 .. 2^125 (bf16 rows) or 2^-23 ..
+ * 2^13 (fp16 rows), so that what is read back is a finite number of the rows' type: larger magnitudes
+ * are saturated.  A group that holds an infinity or a NaN reads as NaN. */
+int gfd_kv4_append(const gfd_kv4_cache* cache, const gfd_kv_rows* rows, const gfd_rotary_axes* axes,
+                   int* error_flag, void* stream);
+
+/* Tokens' keys and values back out of the cache, as rows of num_heads heads of head_dim
+ * elements (GFD_BF16 or GFD_FP16; a 16-bit cache's own type): row t is slot
+ * slots[t], times the scale in 32 bits, rounded to the type.  A slot that is
+ * negative leaves its row as it is; one outside the cache too, and is reported. */
+typedef struct gfd_kv_read_rows {
+    void* k;                   /* NULL: not wanted */
+    void* v;
+    int64_t k_stride, v_stride;  /* elements, multiples of 8 */
+    const int64_t* slots;
+    int num_tokens;
+    int dtype;
+} gfd_kv_read_rows;
+int gfd_kv_read(const gfd_kv_cache* cache, const gfd_kv_read_rows* rows, int* error_flag, void* stream);
+int gfd_kv4_read(const gfd_kv4_cache* cache, const gfd_kv_read_rows* rows, int* error_flag, void* stream);
+
+/* gfd_attention_workspace_bytes, gfd_paged_attention and
+ * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type, exactly in
+ * bf16 but for magnitudes under 2^-126; in fp16 as that type holds them (steps of 2^-24, infinite
+ * from 65520 on): what rows of that type have appended is exact. */
+int64_t gfd_kv4_attention_workspace_bytes(const gfd_kv4_cache* cache, const gfd_attention* call, int prefix_len);
+int gfd_kv4_attention(const gfd_kv4_cache* cache, const gfd_attention* call, void* workspace, size_t workspace_bytes,
+                      int* error_flag, void* stream);
+int gfd_kv4_shared_prefix_attention(const gfd_kv4_cache* cache, const gfd_attention* call, const int* prefix_table,
+                                    int prefix_len, void* workspace, size_t workspace_bytes, int* error_flag,
+                                    void* stream);
+
+/* A copy of the first `slots` slots of page src (of one cache) to page dst (of
+ * the same or another); src or dst negative: none. */
+typedef struct gfd_kv_page_copy {
+    int src, dst, slots, reserved;
+} gfd_kv_page_copy;
+
+/* Copies pages, bit for bit.  Both caches have the same page_size, heads,
+ * head_dim, type and scales; strides and num_pages may differ.  copies is device memory
+ * ([max_copies], 16-byte aligned), of which *count (device int; NULL: max_copies) are done, so that it can
+ * be what gfd_kv_fork or gfd_kv_compact leave, once for each layer's cache.  Within a
+ * call no page is the destination of two copies, or of one and another's source. */
+int gfd_kv_copy_pages(const gfd_kv_cache* dst, const gfd_kv_cache* src, const gfd_kv_page_copy* copies,
+                      int max_copies, const int* count, int* error_flag, void* stream);
+int gfd_kv4_copy_pages(const gfd_kv4_cache* dst, const gfd_kv4_cache* src, const gfd_kv_page_copy* copies,
+                       int max_copies, const int* count, int* error_flag, void* stream);
+
+/* Who holds the pages: refs[p] table entries name page p, 0: it is free.  A
+ * program that keeps pages for itself counts them in refs. */
+typedef struct gfd_kv_pool {
+    int* refs;       /* [num_pages], device */
+    int num_pages;   /* up to 2^24 */
+    int page_size;   /* 1 to 65536 */
+} gfd_kv_pool;
+
+/* Sequences that go on from others, that begin, or that grow: for i < num
+ *   parent[i] >= 0: row child[i] of child_table begins with the first len[i] tokens of row parent[i]
+ *     of table.  Whole pages are shared (their refs grow by one); where len[i] ends within
+ *     a page, the child has a page of its own and copies[i] says what to copy to it;
+ *   parent[i] == -1: row child[i] keeps the pages that it has, for len[i] tokens (0: a new sequence; a row
+ *     that grows: the capacity that it was given before).
+ * Then it gets free pages up to capacity[i] tokens (NULL, or less than len[i]: len[i]), refs 1.
+ * The pages that the items need, in their order, are the free pages in theirs, lowest first:
+ * the same call gives the same tables.  A child[i] that is negative is skipped.  child_table may
+ * be table if no row is both a parent and a child; no row is a child twice.  Entries past a child's pages
+ * stay as they are.  A parent's entry that names no page is passed on as -1. */
+typedef struct gfd_kv_fork_call {
+    const int* table;        /* [rows][table_stride] */
+    int* child_table;        /* [child_rows][child_stride] */
+    int64_t table_stride, child_stride;
+    int rows, child_rows;
+    const int* parent;       /* [num] */
+    const int* child;
+    const int* len;
+    const int* capacity;
+    gfd_kv_page_copy* copies;  /* [num], all written; 16-byte aligned */
+    int num;                 /* up to 2^20 */
+} gfd_kv_fork_call;
+/* Workspace of gfd_kv_fork with up to num items and of gfd_kv_compact (any num); -1: refused.  16-byte aligned; what it
+ * holds before and after a call does not matter, but calls that may run at the same time need one each. */
+int64_t gfd_kv_pool_workspace_bytes(const gfd_kv_pool* pool, int num);
+int gfd_kv_fork(const gfd_kv_pool* pool, const gfd_kv_fork_call* call, void* workspace, size_t workspace_bytes,
+                int* error_flag, void* stream);
+
+/* Lets go of the pages of len[i] tokens of row row[i] of table, i < num: each entry's
+ * page has one less in refs.  Negative rows and entries are skipped; the table stays as it is. */
+int gfd_kv_free(const gfd_kv_pool* pool, const int* table, int64_t table_stride, int rows, const int* row,
+                const int* len, int num, int* error_flag, void* stream);
+
+/* Brings a cache's n used pages to its first n: the used pages from n on, in their order, go to the free
+ * ones before n.  copies ([num_pages / 2] at most) and *num_copies say what to copy,
+ * new_table and new_refs are the tables and counts after it (they may be table and
+ * pool->refs themselves), page_map (NULL: not wanted) where each page is then, -1 for
+ * free ones, for what else names pages.  Entries past a row's len stay as new_table has them. */
+typedef struct gfd_kv_compact_call {
+    int* new_refs;           /* [num_pages] */
+    const int* table;        /* [rows][table_stride] */
+    int* new_table;          /* [rows][new_stride] */
+    int64_t table_stride, new_stride;
+    const int* len;          /* [rows], tokens */
+    int rows;
+    int* page_map;           /* [num_pages] */
+    gfd_kv_page_copy* copies;
+    int* num_copies;
+} gfd_kv_compact_call;
+int gfd_kv_compact(const gfd_kv_pool* pool, const gfd_kv_compact_call* call, void* workspace, size_t workspace_bytes,
+                   int* error_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
