@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call
     const int xcd = (int)blockIdx.x & 7, turn = (int)blockIdx.x >> 3;
     const Stage none{0, 0, 0, 0, 1, 0, 0};
     if (turn >= prefix_turns) {
-        const int item = (turn - prefix_turns) * 8 + xcd;
+        const int item = rows_item<S>((turn - prefix_turns) * 8 + xcd, a.kv_heads);
         if (item < own.blocks * own.splits * a.kv_heads) attend_rows<T, S, D, R, 4, false>(a, c, none, own, item, lds.rows);
     } else {
         attend_tiles<T, S, D, 4, kScores>(a, c, prefix, none, turn * 8 + xcd, lds.tiles);
@@ -36,7 +36,7 @@ int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage&
                 hipStream_t st) {
     const Stage none{0, 0, 0, 0, 1, 0, 0};
     const int prefix_turns = (int)(tiles_groups(a, prefix, none) / 8),
-              own_turns = (int)(((int64_t)own.blocks * own.splits * a.kv_heads + 7) / 8);
+              own_turns = (int)((rows_groups<S>((int64_t)own.blocks * own.splits, a.kv_heads) + 7) / 8);
     const auto go = [&](auto kernel) {
         return start(kernel, dim3((unsigned)(8 * (prefix_turns + own_turns))), 256, st, a, c, prefix, own, prefix_turns);
     };

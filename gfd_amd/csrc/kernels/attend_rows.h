@@ -23,7 +23,8 @@
 //
 // 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 361 us, 5.9 TB/s (a large read: 6.2).
 // 64 ragged contexts of up to 8192: 160 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
-// capped: 60 us, 4.9 TB/s.  700 keys of one token: 7.6 us and 3.9 to join, a chain of loads
+// capped: 60 us, 4.9 TB/s.  4-bit keys of 128 dims: 64 x 8192 of them in 120 us, 4.7 TB/s, 64 ragged contexts of up to 16384 in
+// 97, where the loads alone take 105 of the 120 and the conversions, products and exponents alone 102.  700 keys of one token: 7.6 us and 3.9 to join, a chain of loads
 // (lengths, pages, keys) and a launch each.  Many short contexts take a wave each: 128 of 128 keys in 16 us, 4.2 TB/s.
 #include <algorithm>
 #include <type_traits>
@@ -62,42 +63,51 @@ __device__ __forceinline__ Words<(kBytes + 3) / 4> load_words(const uint8_t* p) 
     return r;
 }
 
-template <typename T, typename S, int D, int R>
-struct RowsKernel {
-    static constexpr int kBits = S::kBits;
+// What 16-bit, 8-bit and 4-bit caches share.
+template <typename T, typename S, int D, int R, int kStepsPerChunk>
+struct RowsShape {
     static constexpr int kDims = D / 16;                   // a lane's dims of a value row
     static constexpr int kSteps = D / 32;                  // products per 16 keys
-    static constexpr int kKeyChunks = D * kBits / 128;     // of 16 bytes a key
-    static constexpr int kKeyLoads = kRowsTile * kKeyChunks / 64;
-    static constexpr int kValBytes = kDims * kBits / 8;
-    static constexpr int kValWords = (kValBytes + 3) / 4;
     static constexpr int kAcc = kDims * 4;                 // a lane's outputs per 16 rows
-    // 32 rows of 128 dims and more: with the rows' operand in registers too, a lane would need more than it has.
-    static constexpr bool kLdsRows = (R == 2 && D >= 128) || D == 256;
-    // 4-bit keys: a lane has the scales of one group of dims, or two, of a key of each 16.
-    static constexpr int kKeyScales = kBits == 4 ? 2 * (D == 256 ? 2 : 1) : 0;
-
-    // A lane's dims of one key's values: of 4 bits all of one group.
-    struct Value : Words<kValWords> {
-        uint32_t scale;  // 4 bits: the byte
-    };
-    struct Tile {
-        u32x4 k[kKeyLoads];
-        uint32_t k_scale[kKeyScales + 1];
-        Value v[8];
-    };
+    // 32 rows of 128 dims and more: with the rows' operand in registers too, a lane would need more than it has.  4 bits: so
+    // that four waves fit a SIMD (64 x 8192 keys 121 us, with three 127).
+    static constexpr bool kLdsRows = (R == 2 && D >= 128) || D == 256 || (S::kBits == 4 && D == 128);
 
     // Dims of product step s and quarter g start here: what a lane reads of a key at once, 16 bytes (8 of 64 4-bit dims),
     // is 1 step's, 2 or 4 steps'.
-    static constexpr int kStepsPerChunk = kBits == 16 ? 1 : kBits == 8 || D == 64 ? 2 : 4;
     static __device__ __forceinline__ int step_dim(int s, int g) {
         return 32 * (s / kStepsPerChunk * kStepsPerChunk) + 8 * kStepsPerChunk * g + 8 * (s % kStepsPerChunk);
     }
     // Where a key's chunk lies in the wave's LDS: neighbours are spread over the banks.
+    template <int kKeyChunks>
     static __device__ __forceinline__ int key_at(int key, int chunk) {
         constexpr int kPerTurn = kKeyChunks >= 16 ? 1 : 16 / kKeyChunks;  // keys that span the banks
         return key * kKeyChunks + (chunk ^ ((key / kPerTurn) & (kKeyChunks >= 16 ? 15 : kKeyChunks - 1)));
     }
+    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b, int odd) {
+        return __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
+    }
+};
+
+template <typename T, typename S, int D, int R>
+struct RowsKernel : RowsShape<T, S, D, R, S::kBits == 16 ? 1 : 2> {
+    using Shape = RowsShape<T, S, D, R, S::kBits == 16 ? 1 : 2>;
+    using Shape::kDims;
+    static constexpr int kBits = S::kBits;
+    static constexpr int kKeyChunks = D * kBits / 128;     // of 16 bytes a key
+    static constexpr int kKeyLoads = kRowsTile * kKeyChunks / 64;
+    static constexpr int kValBytes = kDims * kBits / 8;
+    static constexpr int kValWords = kValBytes / 4;
+    static constexpr int kStepsPerChunk = kBits == 16 ? 1 : 2;
+
+    using Value = Words<kValWords>;  // a lane's dims of one key's values
+    using Values = Value[8];
+    struct Tile {
+        u32x4 k[kKeyLoads];
+        Values v;
+        int valid;  // bit j: value j is there
+    };
+    using Lds = u32x4[kRowsTile * kKeyChunks];  // of a wave
 
     // A load takes whole keys, as many as 1024 bytes hold: the cache's bytes are not used again, and
     // whole rows at a time come faster than the operand's own 64-byte pieces of 16 keys.
@@ -106,111 +116,224 @@ struct RowsKernel {
         for (int i = 0; i < kKeyLoads; i++) {
             const int n = i * 64 + lane;
             const int64_t o = off[n / kKeyChunks];
-            t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + row_offset<S>(c, o < 0 ? 0 : o) + n % kKeyChunks * 16));
-        }
-        if constexpr (kBits == 4) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int64_t o = off[16 * h + (lane & 15)];
-                const uint8_t* p = c.k_scales + scales_offset(c, o < 0 ? 0 : o) + (D == 64 ? lane >> 5 : lane >> 4);
-#pragma unroll
-                for (int n = 0; n < kKeyScales / 2; n++) t.k_scale[h * (kKeyScales / 2) + n] = p[4 * n];
-            }
+            t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + (o < 0 ? 0 : o) + n % kKeyChunks * 16));
         }
     }
-    static __device__ __forceinline__ void store_keys(const Tile& t, u32x4* lds, int lane) {
+    static __device__ __forceinline__ void store(const Tile& t, Lds& lds, int lane) {
 #pragma unroll
         for (int i = 0; i < kKeyLoads; i++) {
             const int n = i * 64 + lane;
-            lds[key_at(n / kKeyChunks, n % kKeyChunks)] = t.k[i];
+            lds[Shape::template key_at<kKeyChunks>(n / kKeyChunks, n % kKeyChunks)] = t.k[i];
         }
     }
-    static __device__ __forceinline__ int load_values(Tile& t, const Cache& c, const int64_t* off, int lane) {
-        int valid = 0;
+    static __device__ __forceinline__ void load_values(Tile& t, const Cache& c, const int64_t* off, int lane) {
+        t.valid = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int64_t o = off[16 * (j >> 2) + 4 * (lane >> 4) + (j & 3)];
-            valid |= (o >= 0) << j;
-            t.v[j] = load_value(c, o < 0 ? 0 : o, lane & 15);
+            t.valid |= (o >= 0) << j;
+            t.v[j] = value(c, o < 0 ? 0 : o, lane & 15);
         }
-        return valid;
     }
     // The dims of a row that lane n of its 16 has.
-    static __device__ __forceinline__ Value load_value(const Cache& c, int64_t place, int n) {
-        Value v;
-        (Words<kValWords>&)v = load_words<kValBytes>(c.v + row_offset<S>(c, place) + n * kValBytes);
-        if constexpr (kBits == 4) v.scale = c.v_scales[scales_offset(c, place) + n * kDims / kGroup4];
-        return v;
+    static __device__ __forceinline__ Value value(const Cache& c, int64_t place, int n) {
+        return load_words<kValBytes>(c.v + place + n * kValBytes);
     }
 
-    // Keys' operands of step s (and the others of its chunk) for 16 keys from first on.
-    static __device__ __forceinline__ void key_frags(const u32x4* lds, const uint32_t* scales, int first, int s, int lane,
+    // Keys' operands of step s (two steps for 8-bit keys) for 16 keys from first on.
+    static __device__ __forceinline__ void key_frags(const Lds& lds, int first, int s, int lane,
                                                      u32x4 (&f)[kStepsPerChunk]) {
-        const int key = first + (lane & 15), n = s / kStepsPerChunk;
+        const u32x4 x = lds[Shape::template key_at<kKeyChunks>(first + (lane & 15), s / kStepsPerChunk * 4 + (lane >> 4))];
         if constexpr (kBits == 16) {
-            f[0] = lds[key_at(key, n * 4 + (lane >> 4))];
-        } else if constexpr (kBits == 8) {
-            const u32x4 x = lds[key_at(key, n * 4 + (lane >> 4))];
+            f[0] = x;
+        } else {
 #pragma unroll
             for (int i = 0; i < 2; i++)
                 f[i] = u32x4{Mma<T>::widen_lo(x[2 * i]), Mma<T>::widen_hi(x[2 * i]), Mma<T>::widen_lo(x[2 * i + 1]),
                              Mma<T>::widen_hi(x[2 * i + 1])};
-        } else {
-            const float scale = scale_of<T>(scales[first / 16 * (kKeyScales / 2) + n]);
-            uint32_t w[kStepsPerChunk];
-            if constexpr (D == 64) {
-                const u32x2 x = ((const u32x2*)(lds + key_at(key, lane >> 5)))[(lane >> 4) & 1];
-                w[0] = x[0], w[1] = x[1];
-            } else {
-                const u32x4 x = lds[key_at(key, n * 4 + (lane >> 4))];
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = x[i];
-            }
-#pragma unroll
-            for (int i = 0; i < kStepsPerChunk; i++) f[i] = widen4<T>(w[i], scale);
         }
     }
     // Word i of a value row in 16-bit pairs.
     static __device__ __forceinline__ uint32_t value_pair(const Value& v, int i) {
         if constexpr (kBits == 16) return v.w[i];
-        else if constexpr (kBits == 8) return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
-        else return widen4<T>(v.w[i / 4], i % 4, scale_of<T>(v.scale));
+        else return (i & 1) ? Mma<T>::widen_hi(v.w[i / 2]) : Mma<T>::widen_lo(v.w[i / 2]);
     }
     // Values as they lie in the cache, all of them made zero, or the infinities and NaN.
     static __device__ __forceinline__ void keep(Value& v, bool there) {
 #pragma unroll
         for (int i = 0; i < kValWords; i++) v.w[i] = there ? v.w[i] : 0u;
-        if constexpr (kBits == 4) v.scale = there ? v.scale : 0u;
     }
     static __device__ __forceinline__ void keep_finite(Value& v) {
-        if constexpr (kBits == 4) {
-            keep(v, v.scale <= (uint32_t)ScaleRange<T>::kMost);
-        } else {
 #pragma unroll
-            for (int i = 0; i < kValWords; i++) {
-                if constexpr (kBits == 16) {
-                    v.w[i] = only_finite<T>(v.w[i]);
-                } else {
-                    const uint32_t nan = ((v.w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // e4m3: all ones but the sign
-                    v.w[i] &= ~((nan >> 7) * 0xFFu);
-                }
+        for (int i = 0; i < kValWords; i++) {
+            if constexpr (kBits == 16) {
+                v.w[i] = only_finite<T>(v.w[i]);
+            } else {
+                const uint32_t nan = ((v.w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;  // e4m3: all ones but the sign
+                v.w[i] &= ~((nan >> 7) * 0xFFu);
             }
         }
     }
-    static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b, int odd) {
-        return __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
+};
+
+// 4-bit numbers.  A tile of 128 dims is 2 KiB of keys and as much of values, and 256 bytes of scales: loads of a lane's own
+// pieces would be many for few bytes, so whole rows of keys, of values and the scales (a key's by a lane, a value's by
+// another) pass through the wave's LDS.  They are all under way during the tile before (two tiles under way were no
+// faster: what bounds is half the bytes, half the instructions that widen them).
+template <typename T, int D, int R>
+struct RowsKernel<T, E2m1, D, R> : RowsShape<T, E2m1, D, R, D == 64 ? 2 : 4> {
+    using Shape = RowsShape<T, E2m1, D, R, D == 64 ? 2 : 4>;
+    using Shape::kDims;
+    static constexpr int kBits = 4;
+    static constexpr int kKeyChunks = D / 32;  // of 16 bytes a row, and its scales
+    static constexpr int kKeyLoads = kRowsTile * kKeyChunks / 64;
+    static constexpr int kValBytes = kDims / 2;
+    static constexpr int kValWords = (kValBytes + 3) / 4;
+    static constexpr int kStepsPerChunk = D == 64 ? 2 : 4;
+
+    struct Value {  // a lane's dims of one key's values, all of one group
+        uint32_t w[kValWords];
+        float scale;
+    };
+    using Values = Value[8];
+    struct Tile {
+        u32x4 k[kKeyLoads], v[kKeyLoads];
+        uint32_t scales[(kKeyChunks + 3) / 4];
+        int valid;  // bit j: value j is there
+    };
+    struct Lds {
+        u32x4 keys[kRowsTile * kKeyChunks], values[kRowsTile * kKeyChunks];
+        uint8_t scales[2][kKeyChunks][kRowsTile];  // of keys and of values
+    };
+
+    // there: a bit for each key.
+    static __device__ __forceinline__ void load(Tile& t, const Cache& c, const Place4* off, uint32_t there, int lane) {
+        const uint32_t w = there >> 4 * (lane >> 4);
+        t.valid = (w & 15) | (w >> 12 & 0xF0);
+        int64_t o[kKeyLoads];
+#pragma unroll
+        for (int i = 0; i < kKeyLoads; i++) {
+            const int n = i * 64 + lane;
+            o[i] = off[n / kKeyChunks].row + n % kKeyChunks * 16;
+        }
+        if (c.heads_inner) {  // a line has neighbouring heads' rows too: it is to stay until they are read
+            asm volatile("");  // the two kinds of loads are not to become one
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; i++) {
+                t.k[i] = *(const u32x4*)(c.k + o[i]);
+                t.v[i] = *(const u32x4*)(c.v + o[i]);
+            }
+            asm volatile("");
+        } else {
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; i++) {
+                t.k[i] = __builtin_nontemporal_load((const u32x4*)(c.k + o[i]));
+                t.v[i] = __builtin_nontemporal_load((const u32x4*)(c.v + o[i]));
+            }
+        }
+        load_scales(t.scales, (lane < 32 ? c.k_scales : c.v_scales) + off[lane & 31].scales);
     }
+    // They lie at any address.
+    static __device__ __forceinline__ void load_scales(uint32_t (&s)[(kKeyChunks + 3) / 4], const uint8_t* p) {
+        if constexpr (D == 64) {
+            uint16_t x;
+            __builtin_memcpy(&x, p, 2);
+            s[0] = x;
+        } else {
+            __builtin_memcpy(s, p, kKeyChunks);
+        }
+    }
+    // A value row's place: the four that a lane's quarters read at once lie side by side, and so do the four that
+    // are stored at once.
+    static __device__ __forceinline__ int value_at(int key) {
+        const int quarter = (key >> 2) & 3, r = key & 3;
+        return ((key & 16) + 4 * r + ((quarter + r) & 3)) * kKeyChunks;
+    }
+    static __device__ __forceinline__ void store(const Tile& t, Lds& lds, int lane) {
+#pragma unroll
+        for (int i = 0; i < kKeyLoads; i++) {
+            const int n = i * 64 + lane;
+            lds.keys[Shape::template key_at<kKeyChunks>(n / kKeyChunks, n % kKeyChunks)] = t.k[i];
+            lds.values[value_at(n / kKeyChunks) + n % kKeyChunks] = t.v[i];
+        }
+#pragma unroll
+        for (int g = 0; g < kKeyChunks; g += 4) {
+            const uint32_t w = read_scales<T>(t.scales[g / 4]);
+#pragma unroll
+            for (int b = 0; b < (D == 64 ? 2 : 4); b++) lds.scales[lane >> 5][g + b][lane & 31] = (uint8_t)(w >> 8 * b);
+        }
+    }
+
+    static __device__ __forceinline__ void key_frags(const Lds& lds, int first, int s, int lane,
+                                                     u32x4 (&f)[kStepsPerChunk]) {
+        const int key = first + (lane & 15), chunk = D == 64 ? lane >> 5 : s / 4 * 4 + (lane >> 4);
+        const float scale = __uint_as_float((uint32_t)lds.scales[0][chunk][key] << 23);
+        const u32x4* const x = lds.keys + Shape::template key_at<kKeyChunks>(key, chunk);
+        uint32_t w[kStepsPerChunk];
+        if constexpr (D == 64) {
+            const u32x2 y = ((const u32x2*)x)[(lane >> 4) & 1];
+            w[0] = y[0], w[1] = y[1];
+        } else {
+            const u32x4 y = *x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = y[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kStepsPerChunk; i++) f[i] = widen4<T>(w[i], scale);
+    }
+    static __device__ __forceinline__ void values(const Lds& lds, int lane, Values& v) {
+        const int quarter = lane >> 4, n = lane & 15;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t scales = *(const uint32_t*)&lds.scales[1][n * kDims / kGroup4][16 * h + 4 * quarter];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                Value& x = v[4 * h + r];
+                const uint8_t* p = (const uint8_t*)(lds.values + value_at(16 * h + 4 * quarter + r)) + n * kValBytes;
+                if constexpr (kValBytes == 2) {
+                    x.w[0] = *(const uint16_t*)p;
+                } else if constexpr (kValBytes == 4) {
+                    x.w[0] = *(const uint32_t*)p;
+                } else {
+                    const u32x2 y = *(const u32x2*)p;
+                    x.w[0] = y[0], x.w[1] = y[1];
+                }
+                x.scale = __uint_as_float((r == 3 ? scales >> 1 : scales << (23 - 8 * r)) & 0x7F800000u);
+            }
+        }
+    }
+    static __device__ __forceinline__ Value value(const Cache& c, const Place4& place, int n) {
+        Value x;
+        const auto w = load_words<kValBytes>(c.v + place.row + n * kValBytes);
+#pragma unroll
+        for (int i = 0; i < kValWords; i++) x.w[i] = w.w[i];
+        x.scale = scale_of<T>(c.v_scales[place.scales + n * kDims / kGroup4]);
+        return x;
+    }
+    static __device__ __forceinline__ uint32_t value_pair(const Value& v, int i) {
+        return widen4<T>(v.w[i / 4], i % 4, v.scale);
+    }
+    static __device__ __forceinline__ void keep(Value& v, bool there) {
+#pragma unroll
+        for (int i = 0; i < kValWords; i++) v.w[i] = there ? v.w[i] : 0u;
+        v.scale = there ? v.scale : 1.f;
+    }
+    static __device__ __forceinline__ void keep_finite(Value& v) { keep(v, __float_as_uint(v.scale) != (uint32_t)kScaleNan << 23); }
 };
 
 template <typename T, typename S, int D, int R, int kWaves>
 struct RowsLds {
     using K = RowsKernel<T, S, D, R>;
     i32x4 rows[16 * R];
-    int64_t offsets[kWaves == 1 ? kRowsShort : kRowsPiece];
+    // Of the range's keys, or a piece's.  4 bits: 0 where none is, and a bit each that says so; else -1.
+    static constexpr int kKeys = kWaves == 1 ? kRowsShort : kRowsPiece;
+    // The last tile is none.
+    Place<S> offsets[kKeys + (S::kBits == 4 ? kRowsTile : 0)];
+    uint32_t there[S::kBits == 4 ? kKeys / kRowsTile + 1 : 1];
     union {
         int samples[kSamples + 1];
         float merge[kWaves == 1 ? 1 : kWaves / 2][kWaves == 1 ? 1 : R * K::kAcc + 2 * R][64];
-        u32x4 keys[kWaves][kRowsTile * K::kKeyChunks];
+        typename K::Lds tiles[kWaves];
     };
     u32x4 queries[K::kLdsRows ? R * K::kSteps : 1][64];
     int any_bad;
@@ -245,6 +368,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         lds.rows[lane] = i32x4{r.t, r.pos, r.lo, r.hi};
     }
     if (tid == 0) lds.any_bad = 0;
+    if constexpr (K::kBits == 4) {
+        if (tid < kRowsTile) lds.offsets[lds.kKeys + tid] = Place4{0, 0};
+        if (tid == 0) lds.there[lds.kKeys / kRowsTile] = 0;
+    }
     __syncthreads();
     const auto read_row = [&](int i) {
         const i32x4 x = lds.rows[16 * i + col];
@@ -252,8 +379,8 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     };
     Row row[R];
     for (int i = 0; i < R; i++) range_add(g, row[i] = read_row(i));
-    // With pieces it is read again where it is used: registers are short.
-    const auto row_at = [&](int i) { return kPieces ? read_row(i) : row[i]; };
+    // With pieces, and 4 bits, it is read again where it is used: registers are short.
+    const auto row_at = [&](int i) { return kPieces || K::kBits == 4 ? read_row(i) : row[i]; };
     g.lo = lanes_min(g.lo);
     g.hi = -lanes_min(-g.hi);
     g.all_lo = -lanes_min(-g.all_lo);
@@ -274,8 +401,16 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         const int n0 = c0 + piece * kPieceTiles * kRowsTile;
         const int most = (kPieces ? min(tiles - piece * kPieceTiles, kPieceTiles) : tiles) * kRowsTile;
         for (int n = tid; n < most; n += kThreads) {
-            const int64_t o = n0 + n < c1 ? key_place<S>(c, k.table, n0 + n, head, a.error) : -1;
-            if (o < 0 && n0 + n < c1) lds.any_bad = 1;
+            Place<S> o;
+            const bool in = n0 + n < c1, there = in && key_place<S>(c, k.table, n0 + n, head, a.error, &o);
+            if (in && !there) lds.any_bad = 1;
+            if constexpr (K::kBits == 4) {
+                const uint64_t bits = __ballot(there);
+                if (!there) o = Place4{0, 0};
+                if (n % kRowsTile == 0) lds.there[n / kRowsTile] = (uint32_t)(bits >> (lane & 32));
+            } else {
+                if (!there) o = -1;
+            }
             lds.offsets[n] = o;
         }
     };
@@ -307,12 +442,14 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         for (int d = 0; d < K::kDims; d++) o[i][d] = f32x4{0, 0, 0, 0};
     }
     typename K::Tile t;
-    u32x4* const my_keys = lds.keys[wave];
-    int valid = 0;
+    typename K::Lds& my_tile = lds.tiles[wave];
     bool any_odd = false;
-    if (wave < tiles) {
+    if constexpr (K::kBits == 4) {
+        const int at = wave < tiles ? wave : lds.kKeys / kRowsTile;
+        K::load(t, c, lds.offsets + at * kRowsTile, lds.there[at], lane);
+    } else if (wave < tiles) {
         K::load_keys(t, c, lds.offsets + wave * kRowsTile, lane);
-        valid = K::load_values(t, c, lds.offsets + wave * kRowsTile, lane);
+        K::load_values(t, c, lds.offsets + wave * kRowsTile, lane);
     }
     for (int tile = wave; tile < tiles; tile += kWaves) {
         const int n0 = c0 + tile * kRowsTile;
@@ -320,12 +457,10 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         // A piece's last tiles, one a wave, with another piece behind it: all waves are here.
         const bool turn = kPieces && tile % kPieceTiles >= kPieceTiles - kWaves &&
                           tile / kPieceTiles * kPieceTiles + kPieceTiles < tiles;
-        const int64_t* next = lds.offsets + (kPieces ? (tile + kWaves) % kPieceTiles : tile + kWaves) * kRowsTile;
+        const int next = kPieces ? (tile + kWaves) % kPieceTiles : tile + kWaves;
         if constexpr (K::kLdsRows) asm volatile("" ::: "memory");  // read again for each tile
-        K::store_keys(t, my_keys, lane);
-        uint32_t k_scale[K::kKeyScales + 1];
-#pragma unroll
-        for (int i = 0; i < K::kKeyScales; i++) k_scale[i] = t.k_scale[i];
+        K::store(t, my_tile, lane);
+        const int valid = t.valid;
         // Other lanes of the wave read them: its LDS accesses are in order, the compiler has to keep them so.
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -336,25 +471,47 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             __syncthreads();
             bad = lds.any_bad != 0;
         }
-        if (more) K::load_keys(t, c, next, lane);
+        if constexpr (K::kBits == 4) {
+            // Whether or not there is such a tile, so that each wait is for the oldest loads only.
+            const int at = more ? next : lds.kKeys / kRowsTile;
+            K::load(t, c, lds.offsets + at * kRowsTile, lds.there[at], lane);
+        } else {
+            if (more) K::load_keys(t, c, lds.offsets + next * kRowsTile, lane);
+        }
         f32x4 x[R][2];
 #pragma unroll
         for (int i = 0; i < R; i++) x[i][0] = x[i][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < K::kSteps; s += K::kStepsPerChunk) {
-            u32x4 k0[K::kStepsPerChunk], k1[K::kStepsPerChunk];
-            K::key_frags(my_keys, k_scale, 0, s, lane, k0);
-            K::key_frags(my_keys, k_scale, 16, s, lane, k1);
+            const auto query = [&](int i, int j) {
+                if constexpr (K::kLdsRows) return lds.queries[i * K::kSteps + s + j][lane];
+                else return q[i][s + j];
+            };
+            if constexpr (K::kBits == 4 && D != 256) {
+                // 16 keys after the others: those of 32, widened, would take the registers of a wave.
 #pragma unroll
-            for (int j = 0; j < K::kStepsPerChunk; j++)
+                for (int h = 0; h < 2; h++) {
+                    u32x4 kf[K::kStepsPerChunk];
+                    K::key_frags(my_tile, 16 * h, s, lane, kf);
 #pragma unroll
-                for (int i = 0; i < R; i++) {
-                    u32x4 qf;
-                    if constexpr (K::kLdsRows) qf = lds.queries[i * K::kSteps + s + j][lane];
-                    else qf = q[i][s + j];
-                    x[i][0] = Mma<T>::m16(k0[j], qf, x[i][0]);
-                    x[i][1] = Mma<T>::m16(k1[j], qf, x[i][1]);
+                    for (int j = 0; j < K::kStepsPerChunk; j++)
+#pragma unroll
+                        for (int i = 0; i < R; i++) x[i][h] = Mma<T>::m16(kf[j], query(i, j), x[i][h]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+            } else {
+                u32x4 k0[K::kStepsPerChunk], k1[K::kStepsPerChunk];
+                K::key_frags(my_tile, 0, s, lane, k0);
+                K::key_frags(my_tile, 16, s, lane, k1);
+#pragma unroll
+                for (int j = 0; j < K::kStepsPerChunk; j++)
+#pragma unroll
+                    for (int i = 0; i < R; i++) {
+                        const u32x4 qf = query(i, j);
+                        x[i][0] = Mma<T>::m16(k0[j], qf, x[i][0]);
+                        x[i][1] = Mma<T>::m16(k1[j], qf, x[i][1]);
+                    }
+            }
         }
         const bool whole = !bad && g.all_lo <= n0 && n0 + kRowsTile <= min(g.all_hi, c1);
         u32x4 p[R];
@@ -411,6 +568,15 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
 #pragma unroll
             for (int j = 0; j < 4; j++) p[i][j] = T::pack(e[2 * j], e[2 * j + 1]);
         }
+        typename K::Values read;
+        auto& v = [&]() -> typename K::Values& {
+            if constexpr (K::kBits == 4) {
+                K::values(my_tile, lane, read);
+                return read;
+            } else {
+                return t.v;
+            }
+        }();
         if (!whole) {
             // Values of keys outside the range count as zeros.  Of keys that some rows see and
             // others do not, infinities and NaN reach only the rows that do: a weight of zero
@@ -418,14 +584,14 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             uint32_t odd = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                K::keep(t.v[j], (valid >> j) & 1);
+                K::keep(v[j], (valid >> j) & 1);
 #pragma unroll
-                for (int i = 0; i < K::kDims / 2; i++) odd |= not_finite<T>(K::value_pair(t.v[j], i));
+                for (int i = 0; i < K::kDims / 2; i++) odd |= not_finite<T>(K::value_pair(v[j], i));
             }
             if (__any(odd != 0)) {
                 any_odd = true;
 #pragma unroll
-                for (int j = 0; j < 8; j++) K::keep_finite(t.v[j]);
+                for (int j = 0; j < 8; j++) K::keep_finite(v[j]);
             }
         }
 #pragma unroll
@@ -433,11 +599,13 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
             u32x4 vf;
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                vf[j] = K::join(K::value_pair(t.v[2 * j], d / 2), K::value_pair(t.v[2 * j + 1], d / 2), d & 1);
+                vf[j] = K::join(K::value_pair(v[2 * j], d / 2), K::value_pair(v[2 * j + 1], d / 2), d & 1);
 #pragma unroll
             for (int i = 0; i < R; i++) o[i][d] = Mma<T>::m16(vf, p[i], o[i][d]);
         }
-        if (more) valid = K::load_values(t, c, next, lane);
+        if constexpr (K::kBits != 4) {
+            if (more) K::load_values(t, c, lds.offsets + next * kRowsTile, lane);
+        }
     }
 
     // The infinities and NaN that were left out, key by key.  Where the product had some in, they add nothing new.
@@ -446,17 +614,18 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
         for (int n0 = c0 + wave * kRowsTile; n0 < c1; n0 += kWaves * kRowsTile)
 #pragma unroll 1
             for (int n = n0; n < min(n0 + kRowsTile, c1); n++) {
-                const int64_t at = key_place<S>(c, k.table, n, head, nullptr);
+                Place<S> at{};
+                const bool there = key_place<S>(c, k.table, n, head, nullptr, &at);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const auto v = K::load_value(c, at < 0 ? 0 : at, 4 * quarter + r);
+                    const auto v = K::value(c, at, 4 * quarter + r);
 #pragma unroll
                     for (int d = 0; d < K::kDims; d++) {
                         const uint32_t pair = K::value_pair(v, d / 2);
                         const float x = T::unpack(pair & ~only_finite<T>(pair))[d & 1];
 #pragma unroll
                         for (int i = 0; i < R; i++)
-                            o[i][d][r] += at >= 0 && n >= row_at(i).lo && n < row_at(i).hi ? x : 0.f;
+                            o[i][d][r] += there && n >= row_at(i).lo && n < row_at(i).hi ? x : 0.f;
                     }
                 }
             }
@@ -528,17 +697,42 @@ __device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const
     }
 }
 
+// Waves that a SIMD is to hold.
+template <typename S, int D, int R, bool kPieces>
+constexpr int rows_waves() {
+    if (S::kBits == 4 && D != 256 && R == 1) return kPieces ? 3 : 4;  // with pieces a few registers more
+    return D == 256 && (R == 2 || S::kBits == 16) ? 1 : 2;
+}
+
+// Which of the items workgroup id takes, and how many workgroups so many items of all heads need.  Workgroups go to the 8
+// XCDs by turns.  A row of 4-bit numbers is half a line of an L2, or less, and its scales a small part of one: the heads of
+// a range stay on one XCD, which then fetches a line once (64 x 8192 keys,
+// heads inside slots: 209 us, so 166; what of it is read with loads that keep lines 143).  Ranges of one sequence are spread over
+// the XCDs, or the longest ones would be one XCD's (64 ragged contexts of up to 16384: 131 us, so 105).
+template <typename S>
+__device__ __forceinline__ int rows_item(int id, int heads) {
+    if constexpr (S::kBits != 4) return id;
+    const int turn = id >> 3, eight = turn / heads;
+    return (eight * 8 + ((id + eight + (eight >> 3)) & 7)) * heads + turn % heads;
+}
+template <typename S>
+int64_t rows_groups(int64_t ranges, int heads) {
+    return S::kBits == 4 ? (ranges + 7) / 8 * 8 * heads : ranges * heads;
+}
+
 template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
-__global__ __launch_bounds__(64 * kWaves, D == 256 && (R == 2 || S::kBits == 16) ? 1 : 2) void attend_rows_kernel(
+__global__ __launch_bounds__(64 * kWaves, (rows_waves<S, D, R, kPieces>())) void attend_rows_kernel(
     Call a, Cache c, Stage prefix, Stage own) {
     __shared__ RowsLds<T, S, D, R, kWaves> lds;
-    attend_rows<T, S, D, R, kWaves, kPieces>(a, c, prefix, own, (int)blockIdx.x, lds);
+    const int item = rows_item<S>((int)blockIdx.x, a.kv_heads);
+    if (S::kBits == 4 && item >= (prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads) return;
+    attend_rows<T, S, D, R, kWaves, kPieces>(a, c, prefix, own, item, lds);
 }
 
 template <typename T, typename S>
 int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st) {
-    const dim3 grid((unsigned)((prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads));
+    const dim3 grid((unsigned)rows_groups<S>((int64_t)prefix.blocks * prefix.splits + (int64_t)own.blocks * own.splits, a.kv_heads));
     const auto go = [&](auto kernel) { return start(kernel, grid, 64 * waves, st, a, c, prefix, own); };
     const auto pick = [&](auto d) {
         constexpr int D = decltype(d)::value;

@@ -57,12 +57,13 @@ struct TilesKernel {
 
     // kc and vc: the thread's chunk of the cache's first row.
     static __device__ __forceinline__ void load(Staged& g, const Cache& c, const uint8_t* kc, const uint8_t* vc,
-                                                const int64_t* off, int tid) {
+                                                const Place<S>* off, int tid) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
-            const int64_t place = off[tid / kChunks + u * kStride], o = row_offset<S>(c, place);
+            const Place<S> place = off[tid / kChunks + u * kStride];
+            const int64_t o = numbers_at(place);
             if constexpr (S::kBits == 4) {
-                const int64_t at = scales_offset(c, place) + tid % kChunks * 8 / kGroup4;
+                const int64_t at = place.scales + tid % kChunks * 8 / kGroup4;
                 g.k[u][0] = *(const uint32_t*)(kc + o);
                 g.v[u][0] = *(const uint32_t*)(vc + o);
                 g.k_scale[u] = c.k_scales[at];
@@ -132,7 +133,7 @@ struct TilesLds {
     };
     u32x4 values[2][K::kTile * D / 8];
     i32x4 rows[K::kRows];
-    int64_t offsets[4][K::kTile];  // where keys lie, 0 where none is
+    Place<S> offsets[4][K::kTile];  // where keys lie, 0 where none is
     int there[4][K::kTile];
     int bad[8], odd[8], ranges[4][W];
 };
@@ -258,10 +259,11 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
     const auto whole = [&](const Range& x, int n0) { return x.all_lo <= n0 && n0 + kTile <= min(x.all_hi, c1); };
     for (int n = tid; n < 3 * kTile; n += K::kThreads) {
         const bool in = c0 + n < c1;
-        const int64_t at = in ? key_place<S>(c, k.table, c0 + n, head, a.error) : -1;
-        if (in && at < 0) bad[n / kTile] = 1;
-        offsets[n / kTile][n % kTile] = max(at, (int64_t)0);
-        there[n / kTile][n % kTile] = at >= 0;
+        Place<S> at{};
+        const bool found = in && key_place<S>(c, k.table, c0 + n, head, a.error, &at);
+        if (in && !found) bad[n / kTile] = 1;
+        offsets[n / kTile][n % kTile] = at;
+        there[n / kTile][n % kTile] = found;
     }
     const uint8_t* const kc = c.k + tid % K::kChunks * S::kBits;
     const uint8_t* const vc = c.v + tid % K::kChunks * S::kBits;
@@ -454,18 +456,20 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
 
         if (more) place(next, t + 1);
         if (wave == 0) {
-            int64_t at = -1;
+            Place<S> at{};
+            bool found = false;
             if (n_look < c1) {
                 if (id_look < 0 || id_look >= c.num_pages) {
                     bad[(t + 3) & 7] = 1;
                     if (a.error) atomicOr(a.error, GFD_KV_ERR_PAGE);
                 } else {
                     at = place_of<S>(c, id_look, (uint32_t)n_look - page_of(n_look) * c.page.d, head);
+                    found = true;
                 }
             }
             if (lane < kTile) {
-                offsets[(t + 3) & 3][lane] = max(at, (int64_t)0);
-                there[(t + 3) & 3][lane] = at >= 0;
+                offsets[(t + 3) & 3][lane] = at;
+                there[(t + 3) & 3][lane] = found;
             }
         }
         if (tid == 0) bad[(t + 5) & 7] = odd[(t + 5) & 7] = 0;

@@ -54,7 +54,7 @@ const char* check_cache(const gfd_kv4_cache* c) {
 Cache make_cache(const gfd_kv4_cache& c) {
     return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride, c.slot_stride, c.head_stride, c.num_pages,
                  make_divider((uint32_t)c.page_size), 1.f, 1.f, (uint8_t*)c.k_scales, (uint8_t*)c.v_scales,
-                 c.scale_page_stride};
+                 c.scale_page_stride, c.head_stride <= c.slot_stride};
 }
 
 Cache make_cache(const gfd_kv_cache& c) {
@@ -62,7 +62,7 @@ Cache make_cache(const gfd_kv_cache& c) {
     const bool scaled = c.dtype == GFD_E4M3;
     return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride * size, c.slot_stride * size, c.head_stride * size,
                  c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f,
-                 nullptr, nullptr, 0};
+                 nullptr, nullptr, 0, 0};
 }
 
 const char* check_rows(const gfd_kv_rows* rows, int head_dim, const gfd_rotary_axes* axes) {
@@ -185,11 +185,8 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
             u.b = u.a + half;
         }
         const int64_t t = t0 + u.t;
-        const uint16_t* p = (u.kind == 0   ? r.q + t * r.q_stride
-                             : u.kind == 1 ? r.k + t * r.k_stride
-                                           : r.v + t * r.v_stride) + (int64_t)u.head * r.dim;
-        u.x = *(const u32x4*)(p + u.a);
-        u.y = *(const u32x4*)(p + u.b);
+        u.x = eight_of(r, u.kind, t, u.head * r.dim + u.a);
+        u.y = eight_of(r, u.kind, t, u.head * r.dim + u.b);
         return u;
     };
     Unit u;

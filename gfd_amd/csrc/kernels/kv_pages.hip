@@ -3,7 +3,7 @@
 //
 // refs[p] counts the table entries that name page p.  Which pages a call takes is
 // a rank among the free (or used) pages in their order, so a call's result is a function of its
-// inputs: a first launch counts each kChunk pages, a second one adds the counts up and
+// inputs: a first launch counts each chunk of pages, a second one adds the counts up and
 // gives every page its rank.  Nothing waits for another workgroup and no atomic's order is
 // used; refs only change by sums and by stores to pages that nothing else names.
 #include <hip/hip_runtime.h>
@@ -19,10 +19,10 @@ namespace kv {
 namespace {
 
 constexpr int kBlock = 256, kWaves = kBlock / 64;
-constexpr int kChunk = 4 * kBlock;  // pages a workgroup ranks, four a thread
+// Pages a workgroup ranks: kFew a thread in small pools, where one chain of loads after the other counts (256 sequences
+// forked in a pool of 12000 pages: 4.5 us, with 4 a thread 11), kMany in large ones, as every workgroup adds up all counts.
+constexpr int kFew = 1, kMany = 16, kSmallPool = 1 << 16;
 constexpr int kSamples = 1024;
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -57,13 +57,22 @@ struct Pool {
     Divider page;
 };
 
-// A thread's four pages of a chunk; what lies past the last page is `past`.
-__device__ __forceinline__ i32x4 four_refs(const Pool& pool, int first, int past) {
-    i32x4 x;
+// A thread's pages of a chunk; what lies past the last page is `past`.
+template <int kPer>
+struct Refs {
+    int page, x[kPer];
+    __device__ __forceinline__ Refs(const Pool& pool, int chunk, int past) {
+        page = (chunk * kBlock + (int)threadIdx.x) * kPer;
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = first + i < pool.num_pages ? pool.refs[first + i] : past;
-    return x;
-}
+        for (int i = 0; i < kPer; i++) x[i] = page + i < pool.num_pages ? pool.refs[page + i] : past;
+    }
+    __device__ __forceinline__ int free_pages() const {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) n += x[i] == 0;
+        return n;
+    }
+};
 
 // What the chunks before this one count together; *total of all.
 __device__ __forceinline__ int chunks_before(const int* counts, int chunks, int chunk, int* part, int* total) {
@@ -132,16 +141,15 @@ __device__ __forceinline__ Item item_of(const Fork& f, int i, int* error) {
     return x;
 }
 
-__device__ __forceinline__ int free_of(const i32x4& x) { return (x[0] == 0) + (x[1] == 0) + (x[2] == 0) + (x[3] == 0); }
-
 // A workgroup counts a chunk's free pages; the last one the pages that the items before each need.
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void fork_count_kernel(Fork f) {
     __shared__ int part[kWaves];
     __shared__ long long part64[kWaves];
     if ((int)blockIdx.x < f.pool.chunks) {
-        const i32x4 x = four_refs(f.pool, (int)blockIdx.x * kChunk + (int)threadIdx.x * 4, 1);
+        const Refs<kPer> r(f.pool, (int)blockIdx.x, 1);
         int total;
-        before(free_of(x), part, &total);
+        before(r.free_pages(), part, &total);
         if (threadIdx.x == 0) f.counts[blockIdx.x] = total;
         return;
     }
@@ -162,41 +170,41 @@ __global__ __launch_bounds__(kBlock) void fork_count_kernel(Fork f) {
 }
 
 // Gives a chunk's free pages to the items whose needs have their ranks.
+template <int kPer>
 __device__ __forceinline__ void give_pages(const Fork& f, int chunk, int* part, int* samples) {
+    const Refs<kPer> r(f.pool, chunk, 1);
+    const int needed = f.first[f.num], step = (f.num + kSamples - 1) / kSamples;
     int free_pages, total;
     const int base = chunks_before(f.counts, f.pool.chunks, chunk, part, &free_pages);
-    const int needed = f.first[f.num];
     if (base >= needed) return;
-    const int step = (f.num + kSamples - 1) / kSamples;
-    for (int i = (int)threadIdx.x; i <= kSamples; i += kBlock) samples[i] = f.first[min(i * step, f.num)];
-    const int page = chunk * kChunk + (int)threadIdx.x * 4;
-    const i32x4 x = four_refs(f.pool, page, 1);
-    int rank = base + before(free_of(x), part, &total);  // its barriers stand behind the samples too
-#pragma unroll 1
-    for (int n = 0; n < 4; n++) {
-        if (x[n] != 0) continue;
+    for (int i = (int)threadIdx.x; i <= kSamples && i * step < f.num + step; i += kBlock) samples[i] = f.first[min(i * step, f.num)];
+    int rank = base + before(r.free_pages(), part, &total);  // its barriers stand behind the samples too
+#pragma unroll
+    for (int n = 0; n < kPer; n++) {
+        if (r.x[n] != 0) continue;
         if (rank >= needed) return;
         // The item with first[i] <= rank < first[i + 1].
-        int lo = 0, hi = kSamples;
+        int lo = 0, hi = (f.num + step - 1) / step;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             if (samples[mid] <= rank) lo = mid; else hi = mid;
         }
+        int before_item = samples[lo];
         lo *= step;
         hi = min(lo + step, f.num);
         while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (f.first[mid] <= rank) lo = mid; else hi = mid;
+            const int mid = (lo + hi) / 2, at = f.first[mid];
+            if (at <= rank) lo = mid, before_item = at; else hi = mid;
         }
         const Item it = item_of(f, lo, nullptr);
-        const int j = it.from + (rank - f.first[lo]);
-        f.child_table[it.child * f.child_stride + j] = page + n;
-        f.refs[page + n] = 1;
+        const int j = it.from + (rank - before_item), page = r.page + n;
+        f.child_table[it.child * f.child_stride + j] = page;
+        f.refs[page] = 1;
         if (it.part && j == it.from) {
             const int src = f.table[it.parent * f.table_stride + j];
             const bool there = src >= 0 && src < f.pool.num_pages;
             if (!there) report(f.error, GFD_KV_ERR_PAGE);
-            f.copies[lo] = there ? gfd_kv_page_copy{src, page + n, it.part, 0} : gfd_kv_page_copy{-1, -1, 0, 0};
+            f.copies[lo] = there ? gfd_kv_page_copy{src, page, it.part, 0} : gfd_kv_page_copy{-1, -1, 0, 0};
         }
         rank++;
     }
@@ -210,6 +218,9 @@ __device__ __forceinline__ void share_pages(const Fork& f, int i, int turn, int 
         if (first_turn) f.copies[i] = gfd_kv_page_copy{-1, -1, 0, 0};
         return;
     }
+    const int first = f.first[i];
+    int free_pages;
+    chunks_before(f.counts, f.pool.chunks, 0, part, &free_pages);
     int* const to = f.child_table + x.child * f.child_stride;
     for (int j = turn * kBlock + (int)threadIdx.x; j < x.shared; j += turns * kBlock) {
         int id = f.table[x.parent * f.table_stride + j];
@@ -221,9 +232,6 @@ __device__ __forceinline__ void share_pages(const Fork& f, int i, int turn, int 
         }
         to[j] = id;
     }
-    int free_pages;
-    chunks_before(f.counts, f.pool.chunks, 0, part, &free_pages);
-    const int first = f.first[i];
     if (first_turn && (x.part == 0 || first >= free_pages)) f.copies[i] = gfd_kv_page_copy{-1, -1, 0, 0};
     const int lost = x.from + max(free_pages - first, 0);
     if (lost >= x.end) return;
@@ -232,10 +240,11 @@ __device__ __forceinline__ void share_pages(const Fork& f, int i, int turn, int 
 }
 
 // A few launches' latency for a few sequences; the tables' bytes for many.
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void fork_kernel(Fork f, int turns) {
     __shared__ int part[kWaves], samples[kSamples + 1];
     const int id = (int)blockIdx.x - f.pool.chunks;
-    if (id < 0) give_pages(f, (int)blockIdx.x, part, samples);
+    if (id < 0) give_pages<kPer>(f, (int)blockIdx.x, part, samples);
     else share_pages(f, id / turns, id % turns, turns, part);
 }
 
@@ -295,44 +304,45 @@ struct Compact {
     int* dst;
 };
 
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void compact_count_kernel(Compact f) {
     __shared__ int part[kWaves];
     int total;
-    const i32x4 x = four_refs(f.pool, (int)blockIdx.x * kChunk + (int)threadIdx.x * 4, 0);
-    before(4 - free_of(x), part, &total);
+    const Refs<kPer> r(f.pool, (int)blockIdx.x, 0);
+    before(kPer - r.free_pages(), part, &total);
     if (threadIdx.x == 0) f.counts[blockIdx.x] = total;
 }
 
 // Every page's rank among the used ones.  With n used pages, of which m lie before page n, the used page of rank k from
 // page n on is copy k - m's source, and the free page p before n, with k used ones before it, copy p - k's destination.
 // In place new_refs only gets what is there already: other workgroups still count.
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void compact_rank_kernel(Compact f) {
     __shared__ int part[kWaves];
-    int used, total, in_front;
-    const int chunk = (int)blockIdx.x, page = chunk * kChunk + (int)threadIdx.x * 4;
+    int used, total, in_front, all;
+    const int chunk = (int)blockIdx.x;
+    const Refs<kPer> r(f.pool, chunk, 0);
     const int base = chunks_before(f.counts, f.pool.chunks, chunk, part, &used);
-    const int edge = used / kChunk, edge_page = edge * kChunk + (int)threadIdx.x * 4;
-    const i32x4 at_edge = four_refs(f.pool, edge_page, 0);
+    const int edge = used / (kPer * kBlock);
+    const Refs<kPer> at_edge(f.pool, edge, 0);
     int mine = 0;
 #pragma unroll
-    for (int n = 0; n < 4; n++) mine += edge_page + n < used && at_edge[n] != 0;
+    for (int n = 0; n < kPer; n++) mine += at_edge.page + n < used && at_edge.x[n] != 0;
     before(mine, part, &in_front);
-    int all;
     in_front += chunks_before(f.counts, f.pool.chunks, edge, part, &all);
     if (chunk == 0 && threadIdx.x == 0) *f.num_copies = used - in_front;
-    const i32x4 x = four_refs(f.pool, page, 0);
-    int rank = base + before(4 - free_of(x), part, &total);
+    int rank = base + before(kPer - r.free_pages(), part, &total);
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-        const int p = page + n;
+    for (int n = 0; n < kPer; n++) {
+        const int p = r.page + n;
         if (p >= f.pool.num_pages) return;
         int to = -1;
-        if (x[n] != 0) {
+        if (r.x[n] != 0) {
             to = p;
             if (p >= used) {
                 const int i = rank - in_front;
                 f.src[i] = p;
-                f.src_refs[i] = x[n];
+                f.src_refs[i] = r.x[n];
                 to = -2 - i;
             }
             rank++;
@@ -340,7 +350,7 @@ __global__ __launch_bounds__(kBlock) void compact_rank_kernel(Compact f) {
             f.dst[p - rank] = p;
         }
         f.where[p] = to;
-        if (to == p || (x[n] == 0 && p >= used)) f.new_refs[p] = x[n];
+        if (to == p || (r.x[n] == 0 && p >= used)) f.new_refs[p] = r.x[n];
         if (f.page_map && to >= -1) f.page_map[p] = to;
     }
 }
@@ -404,31 +414,32 @@ __global__ __launch_bounds__(kBlock) void copy_pages_kernel(Copy f, int64_t grou
         }
         u32x4 k[kUnits], v[kUnits];
         uint8_t ks[kUnits], vs[kUnits];
-        int64_t to[kUnits];
+        Place<S> to[kUnits];
+        bool there[kUnits];
 #pragma unroll
         for (int n = 0; n < kUnits; n++) {
             const int at = unit + n * kBlock, row = at >> f.row_chunks, chunk = at & ((1 << f.row_chunks) - 1);
             const int outer = (int)f.inner.div((uint32_t)row), inner = row - outer * (int)f.inner.d;
             const int slot = f.heads_inner ? outer : inner, head = f.heads_inner ? inner : outer;
-            to[n] = -1;
-            if (row >= rows || slot >= p.slots) continue;
-            to[n] = place_of<S>(f.dst, p.dst, (uint32_t)slot, head * f.dst.head_stride) + 16 * chunk;
-            const int64_t from = place_of<S>(f.src, p.src, (uint32_t)slot, head * f.src.head_stride) + 16 * chunk;
-            k[n] = *(const u32x4*)(f.src.k + row_offset<S>(f.src, from));
-            v[n] = *(const u32x4*)(f.src.v + row_offset<S>(f.src, from));
+            there[n] = row < rows && slot < p.slots;
+            if (!there[n]) continue;
+            to[n] = place_of<S>(f.dst, p.dst, (uint32_t)slot, head * f.dst.head_stride + 16 * chunk);
+            const auto from = place_of<S>(f.src, p.src, (uint32_t)slot, head * f.src.head_stride + 16 * chunk);
+            k[n] = *(const u32x4*)(f.src.k + numbers_at(from));
+            v[n] = *(const u32x4*)(f.src.v + numbers_at(from));
             if constexpr (S::kBits == 4) {
-                ks[n] = f.src.k_scales[scales_offset(f.src, from)];
-                vs[n] = f.src.v_scales[scales_offset(f.src, from)];
+                ks[n] = f.src.k_scales[from.scales];
+                vs[n] = f.src.v_scales[from.scales];
             }
         }
 #pragma unroll
         for (int n = 0; n < kUnits; n++) {
-            if (to[n] < 0) continue;
-            *(u32x4*)(f.dst.k + row_offset<S>(f.dst, to[n])) = k[n];
-            *(u32x4*)(f.dst.v + row_offset<S>(f.dst, to[n])) = v[n];
+            if (!there[n]) continue;
+            *(u32x4*)(f.dst.k + numbers_at(to[n])) = k[n];
+            *(u32x4*)(f.dst.v + numbers_at(to[n])) = v[n];
             if constexpr (S::kBits == 4) {
-                f.dst.k_scales[scales_offset(f.dst, to[n])] = ks[n];
-                f.dst.v_scales[scales_offset(f.dst, to[n])] = vs[n];
+                f.dst.k_scales[to[n].scales] = ks[n];
+                f.dst.v_scales[to[n].scales] = vs[n];
             }
         }
     }
@@ -466,8 +477,16 @@ const char* check_pool(const gfd_kv_pool* pool) {
     return nullptr;
 }
 
+int chunks_of(const gfd_kv_pool& p) {
+    return (int)ceil_div(p.num_pages, kBlock * (p.num_pages <= kSmallPool ? kFew : kMany));
+}
 Pool make_pool(const gfd_kv_pool& p) {
-    return Pool{p.refs, p.num_pages, (int)ceil_div(p.num_pages, kChunk), make_divider((uint32_t)p.page_size)};
+    return Pool{p.refs, p.num_pages, chunks_of(p), make_divider((uint32_t)p.page_size)};
+}
+// f(pages a thread ranks), as a constant.
+template <typename F>
+int with_pages(const gfd_kv_pool& p, F f) {
+    return p.num_pages <= kSmallPool ? f(std::integral_constant<int, kFew>()) : f(std::integral_constant<int, kMany>());
 }
 
 constexpr int kMostItems = 1 << 20;
@@ -475,7 +494,7 @@ constexpr int kMostItems = 1 << 20;
 // Counts of chunks, then a fork's sums of needs or what a compaction knows of the pages.
 int64_t workspace_bytes(const gfd_kv_pool& p, int num) {
     const int64_t pages = p.num_pages;
-    return 4 * (ceil_div(pages, kChunk) + std::max<int64_t>(num + 1, pages + 3 * (pages / 2)));
+    return 4 * (chunks_of(p) + std::max<int64_t>(num + 1, pages + 3 * (pages / 2)));
 }
 
 const char* check_workspace(const gfd_kv_pool& p, int num, const void* workspace, size_t bytes) {
@@ -551,9 +570,11 @@ extern "C" int gfd_kv_fork(const gfd_kv_pool* pool, const gfd_kv_fork_call* call
            w.child, w.len, w.capacity, w.copies, w.num, error_flag, (int*)workspace, (int*)workspace + p.chunks};
     const hipStream_t st = (hipStream_t)stream;
     const int turns = turns_of(w.child_stride, w.num);
-    int rc = start(fork_count_kernel, dim3((unsigned)p.chunks + 1), kBlock, st, f);
-    if (!rc) rc = start(fork_kernel, dim3((unsigned)(p.chunks + w.num * turns)), kBlock, st, f, turns);
-    return launched(kName, rc);
+    return launched(kName, with_pages(*pool, [&](auto per) {
+        constexpr int kPer = decltype(per)::value;
+        const int rc = start(fork_count_kernel<kPer>, dim3((unsigned)p.chunks + 1), kBlock, st, f);
+        return rc ? rc : start(fork_kernel<kPer>, dim3((unsigned)(p.chunks + w.num * turns)), kBlock, st, f, turns);
+    }));
 }
 
 extern "C" int gfd_kv_free(const gfd_kv_pool* pool, const int* table, int64_t table_stride, int rows, const int* row,
@@ -595,8 +616,11 @@ extern "C" int gfd_kv_compact(const gfd_kv_pool* pool, const gfd_kv_compact_call
                     w.copies, w.num_copies, error_flag, counts, where, src, src + half, src + 2 * half};
     const hipStream_t st = (hipStream_t)stream;
     const int copy_groups = (int)ceil_div(half, kBlock), turns = turns_of(w.table_stride, w.rows);
-    int rc = start(compact_count_kernel, dim3((unsigned)p.chunks), kBlock, st, f);
-    if (!rc) rc = start(compact_rank_kernel, dim3((unsigned)p.chunks), kBlock, st, f);
+    int rc = with_pages(*pool, [&](auto per) {
+        constexpr int kPer = decltype(per)::value;
+        const int first = start(compact_count_kernel<kPer>, dim3((unsigned)p.chunks), kBlock, st, f);
+        return first ? first : start(compact_rank_kernel<kPer>, dim3((unsigned)p.chunks), kBlock, st, f);
+    });
     const int groups = copy_groups + w.rows * turns;
     if (!rc && groups) rc = start(compact_kernel, dim3((unsigned)groups), kBlock, st, f, copy_groups, turns);
     return launched(kName, rc);

@@ -41,6 +41,17 @@ __device__ __forceinline__ double position_of(const Rows& r, int64_t t, int i) {
     return r.float_positions ? (double)((const float*)r.axes_positions)[at] : (double)((const int*)r.axes_positions)[at];
 }
 
+// Eight values of row t of a kind (0 q, 1 k, 2 v), from value a on.  All of the choice's terms are values: written as a choice
+// between members it becomes a load of the call's arguments in front of each load of a row, and a wait for all
+// that is under way.
+template <typename N>
+__device__ __forceinline__ N pick(int kind, N q, N k, N v) {
+    return kind == 0 ? q : kind == 1 ? k : v;
+}
+__device__ __forceinline__ u32x4 eight_of(const Rows& r, int kind, int64_t t, int a) {
+    return *(const u32x4*)(pick(kind, r.q, r.k, r.v) + t * pick(kind, r.q_stride, r.k_stride, r.v_stride) + a);
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
 #pragma unroll

@@ -223,16 +223,17 @@ __device__ __forceinline__ int head_of(const Call& a, const Block& k, int r, int
     return kv_head * (int)a.group.d + (int)(n - a.group.div(n) * a.group.d);
 }
 
-// Where a key lies, -1 where its page is none of the cache's.
+// Where a key lies; false: nowhere, its page is none of the cache's.
 template <typename S>
-__device__ __forceinline__ int64_t key_place(const Cache& c, const int* table, int n, int64_t head, int* error) {
+__device__ __forceinline__ bool key_place(const Cache& c, const int* table, int n, int64_t head, int* error, Place<S>* to) {
     const uint32_t page = c.page.div((uint32_t)n);
     const int id = table[page];
     if (id < 0 || id >= c.num_pages) {
         if (error) atomicOr(error, GFD_KV_ERR_PAGE);
-        return -1;
+        return false;
     }
-    return place_of<S>(c, id, (uint32_t)n - page * c.page.d, head);
+    *to = place_of<S>(c, id, (uint32_t)n - page * c.page.d, head);
+    return true;
 }
 
 __device__ __forceinline__ int64_t slot_of(const Call& a, int slot, int t, int h) {

@@ -20,9 +20,10 @@ namespace {
 constexpr int kJoinBlock = 256;
 
 // A workgroup joins kPart rows of an own-keys block, a wave per row: a lane
-// weighs one range of 64, then holds D / 64 dims.  Reads what the ranges left once; a
-// launch and a chain of four loads for small batches (3.4 us), 4 to 9 us for 2048 rows of up to 18 ranges.
-template <typename T, int D, int kRows, int kPart>
+// weighs one range of 64, then holds D / 64 dims, of kBatch ranges at once.  Reads what the ranges left once; a
+// launch and a chain of four loads for small batches (3.4 us), 4 to 9 us for 2048 rows of up to 18 ranges.  Few rows of many
+// ranges wait for their batches one after the other: 32 rows of 64 ranges 10.4 us by eights, 6.8 by 32.
+template <typename T, int D, int kRows, int kPart, int kBatch>
 __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage own) {
     constexpr int kDims = D / 64, kWaves = kJoinBlock / 64;
     typedef float Dims __attribute__((ext_vector_type(kDims)));
@@ -56,17 +57,17 @@ __global__ __launch_bounds__(kJoinBlock) void join_kernel(Call a, Cache c, Stage
             const float* from = a.part_o + slot_of(a, s0, t, h) * D + lane * kDims;
             const int64_t step = (int64_t)a.num_tokens * a.q_heads * D;
             const int n = min(64, slots - s0);
-            for (int s = 0; s < n; s += 8) {  // lanes past the last range weigh nothing
-                Dims x[8];
-                float ws[8];
+            for (int s = 0; s < n; s += kBatch) {  // lanes past the last range weigh nothing
+                Dims x[kBatch];
+                float ws[kBatch];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < kBatch; j++) {
                     ws[j] = __shfl(w, s + j);
                     x[j] = 0.f;
                     if (__shfl(l, s + j) != 0.f) x[j] = *(const Dims*)(from + (s + j) * step);
                 }
 #pragma unroll
-                for (int j = 0; j < 8; j++) o += ws[j] * x[j];
+                for (int j = 0; j < kBatch; j++) o += ws[j] * x[j];
             }
         }
         total = across16_sum(total);
@@ -125,7 +126,8 @@ int fit_cu(int dim, bool few, int rows, int dtype) {
 // Past kMostRounds ranges grow instead, walked in pieces: a full card gains nothing from more of them, and what they
 // leave to be joined would grow with the context (512 of 131072 keys: 1.1 GB in ranges of one piece, 17 MB so).
 // 64 of up to 32768: 616 us, in ranges of one piece 634; 512 of up to 4096, whole 515, 520.
-constexpr int kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512;
+// 4 bits: twice the keys for the bytes (64 k keys of one sequence: ranges of 1024 28 us, of 512 32, of 2048 32).
+constexpr int kRounds = 4, kMostRounds = 16, kMinChunk = 128, kGoodChunk = 512, kGoodChunk4 = 1024;
 // From so many workgroups on (two a CU), short contexts get a wave each: of four waves most would
 // find no tile or one, and what takes the time is a workgroup's start (91 times 12 heads of 256 dims and 27 keys:
 // 46 us, with one wave 17; 70 times 8 heads of 128 dims and 128 keys: 15.2, 12.7).
@@ -137,13 +139,13 @@ constexpr int kOneWave = 512;
 // with two workgroups a CU 69; 512 over 2048 84, 98; a prefix of 32768 for 64 requests 160, with two 183.
 constexpr int kTilesMinChunk = 256;
 
-void split(Stage* st, int64_t items, int64_t keys, bool few, int fit) {
+void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, int good) {
     if (few) {
         const int64_t round = (int64_t)fit * kCus;
         const auto chunk_for = [&](int64_t groups) {
             return ceil_div(ceil_div(keys * items, groups), kMinChunk) * kMinChunk;
         };
-        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(kGoodChunk, chunk_for(round)));
+        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(good, chunk_for(round)));
         const int64_t spread = std::min<int64_t>(kRowsPiece, std::max(least, chunk_for(round * kRounds)));
         const int64_t whole = std::max<int64_t>(1, ceil_div(keys, kMinChunk)) * kMinChunk;
         st->chunk = (int)std::min(whole, std::max(spread, chunk_for(round * kMostRounds)));
@@ -157,7 +159,12 @@ void split(Stage* st, int64_t items, int64_t keys, bool few, int fit) {
 
 // Waves of a block of many rows: 8, for half the reads of the cache, where that still gives every CU two blocks
 // (4096 tokens over 16384 keys: 950 us, with 4 waves 1077; 2048 tokens of 32 heads, one block each: 87 us, with 4 73).
-int tile_waves(int64_t rows, int64_t heads, int dim) { return dim != 256 && rows * heads >= 2 * 256 * 256 ? 8 : 4; }
+// 4 bits, which are widened once for each block: also where every CU has one, unless the prompt is most of what it sees and its
+// last block far longer than the first (2048 tokens over 8192 keys: 269 us, with 4 waves 287; 4 times 512 over 2048: 77,
+// 87; 2048 over themselves: 72, 68).
+int tile_waves(int64_t rows, int64_t heads, int dim, bool wide) {
+    return dim != 256 && rows * heads >= (wide ? 1 : 2) * 256 * 256 ? 8 : 4;
+}
 
 Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
     Plan p{};
@@ -173,12 +180,13 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.own.blocks = w.batch;
         p.own.whole = 1;
     } else {
-        p.own_waves = tile_waves(all_rows, heads, cache.head_dim);
+        p.own_waves = tile_waves(all_rows, heads, cache.head_dim, cache.dtype == kE2m1 && w.max_kv_len >= 2 * (int64_t)w.max_q_len);
         p.rows = 32 * p.own_waves;
         p.own.blocks = (int)std::min<int64_t>(w.batch * ceil_div(seq_rows, p.rows), all_rows / p.rows + w.batch);
     }
     const auto fit = [&](bool few) { return fit_cu(cache.head_dim, few, p.rows, cache.dtype); };
-    split(&p.own, p.own.blocks * heads, keys, !p.own_waves, fit(!p.own_waves));
+    const int good = cache.dtype == kE2m1 ? kGoodChunk4 : kGoodChunk;
+    split(&p.own, p.own.blocks * heads, keys, !p.own_waves, fit(!p.own_waves), good);
     p.few_waves = 4;
     if (!p.own_waves && !prefix_len && keys <= kRowsShort && p.own.blocks * heads >= kOneWave) {
         p.few_waves = 1;
@@ -190,21 +198,21 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.prefix.prefix = 1;
         p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : 4;
         p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
-        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves));
+        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves), good);
         p.own.first_slot = p.prefix.splits;
     }
     p.slots = p.own.first_slot + p.own.splits;
-    // Turns of 8 workgroups are filled up.  The join, where there is one, has as many threads at most.
+    // Turns of 8 workgroups are filled up, of 8 ranges' heads with 4 bits.  The join, where there is one, has as many threads at most.
     const int64_t items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
-    p.threads = (items + 16) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
+    p.threads = (items + 16 + (cache.dtype == kE2m1 ? 16 * heads : 0)) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
     if (p.slots > 1)
         p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4 + p.own.blocks * heads * 4;
     return p;
 }
 
-template <typename T, int D, int kRows, int kPart>
+template <typename T, int D, int kRows, int kPart, int kBatch = 8>
 int launch_join(const Call& a, const Cache& c, const Stage& own, hipStream_t st) {
-    return start(join_kernel<T, D, kRows, kPart>, dim3((unsigned)(own.blocks * a.kv_heads), kRows / kPart), kJoinBlock, st,
+    return start(join_kernel<T, D, kRows, kPart, kBatch>, dim3((unsigned)(own.blocks * a.kv_heads), kRows / kPart), kJoinBlock, st,
                  a, c, own);
 }
 template <typename T, int D>
@@ -212,8 +220,10 @@ int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
     // A wave a row takes the least time where few rows leave the card empty (100 tokens over 4196 keys: 33 us in all,
     // with four rows a wave 38); with many it does not matter.
     const bool few = (int64_t)p.own.blocks * p.rows * a.kv_heads <= 16384;
-    if (p.rows == 16) return launch_join<T, D, 16, 4>(a, c, p.own, st);
-    if (p.rows == 32) return launch_join<T, D, 32, 4>(a, c, p.own, st);
+    // With more ranges than two batches of 8.
+    const bool deep = p.slots > 16 && (int64_t)p.own.blocks * a.kv_heads <= 2 * kCus;
+    if (p.rows == 16) return deep ? launch_join<T, D, 16, 4, 32>(a, c, p.own, st) : launch_join<T, D, 16, 4>(a, c, p.own, st);
+    if (p.rows == 32) return deep ? launch_join<T, D, 32, 4, 32>(a, c, p.own, st) : launch_join<T, D, 32, 4>(a, c, p.own, st);
     if (p.rows == 128) return few ? launch_join<T, D, 128, 4>(a, c, p.own, st) : launch_join<T, D, 128, 16>(a, c, p.own, st);
     return few ? launch_join<T, D, 256, 4>(a, c, p.own, st) : launch_join<T, D, 256, 16>(a, c, p.own, st);
 }

@@ -67,6 +67,14 @@ template <typename T>
 __device__ __forceinline__ float scale_of(uint32_t byte) {
     return __uint_as_float((byte > (uint32_t)ScaleRange<T>::kMost ? (uint32_t)kScaleNan : byte) << 23);
 }
+// The same for four scales in a word: bytes above kMost become kScaleNan.
+template <typename T>
+__device__ __forceinline__ uint32_t read_scales(uint32_t w) {
+    constexpr uint32_t kRest = 0x7Fu - (ScaleRange<T>::kMost & 0x7Fu);  // added to 7 bits, sets the eighth above kMost
+    static_assert(ScaleRange<T>::kMost >= 128, "the eighth bit is set too");
+    const uint32_t hot = ((w & 0x7F7F7F7Fu) + kRest * 0x01010101u) & w & 0x80808080u;
+    return w | ((hot << 1) - (hot >> 7));
+}
 // Two numbers, byte `byte` of w, as a pair of T: the first in the low half of the byte and of the pair.
 template <typename T>
 __device__ __forceinline__ uint32_t widen4(uint32_t w, int byte, float scale) {
@@ -125,24 +133,23 @@ struct Cache {
     uint8_t* k_scales;
     uint8_t* v_scales;
     int64_t scale_page_stride;
+    int heads_inner;  // a slot's heads are neighbours
 };
 
-// Where a row (slot and head of a page) of a cache of type S lies, as a number that is not negative: its byte offset, or
-// for 4-bit numbers, whose scales lie elsewhere, the page and the offset within it.
+// Byte offsets of a row (slot and head of a page): of its numbers, and of 4-bit ones' scales.
+struct Place4 {
+    int64_t row, scales;
+};
 template <typename S>
-__device__ __forceinline__ int64_t place_of(const Cache& c, int page, uint32_t slot, int64_t head) {
+using Place = typename std::conditional<S::kBits == 4, Place4, int64_t>::type;
+template <typename S>
+__device__ __forceinline__ Place<S> place_of(const Cache& c, int page, uint32_t slot, int64_t head) {
     const int64_t in = slot * c.slot_stride + head;
-    if constexpr (S::kBits == 4) return (int64_t)page << 32 | in;
+    if constexpr (S::kBits == 4) return Place4{page * c.page_stride + in, page * c.scale_page_stride + (in >> 4)};
     else return page * c.page_stride + in;
 }
-template <typename S>
-__device__ __forceinline__ int64_t row_offset(const Cache& c, int64_t place) {
-    if constexpr (S::kBits == 4) return (int64_t)(int)(place >> 32) * c.page_stride + (uint32_t)place;
-    else return place;
-}
-__device__ __forceinline__ int64_t scales_offset(const Cache& c, int64_t place) {
-    return (int64_t)(int)(place >> 32) * c.scale_page_stride + ((uint32_t)place >> 4);
-}
+__device__ __forceinline__ int64_t numbers_at(int64_t p) { return p; }
+__device__ __forceinline__ int64_t numbers_at(const Place4& p) { return p.row; }
 
 // A launch has fewer threads along a grid than this.
 constexpr int64_t kGridThreads = 1ll << 32;
