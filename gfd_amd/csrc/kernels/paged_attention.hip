@@ -137,20 +137,23 @@ constexpr int kOneWave = 512;
 // tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
 // of the CUs one (64 requests on 32768 shared keys: 91 us, with two 103).  256 dims: 100 tokens over 4196 keys 54 us,
 // with two workgroups a CU 69; 512 over 2048 84, 98; a prefix of 32768 for 64 requests 160, with two 183.
-constexpr int kTilesMinChunk = 256;
+// 4 bits: the rest takes less of the CUs, and a prefix whose ranges stay long has as many as fit (64 requests on 65536
+// shared keys 108 us, with one a CU 126; 200 on 16384 114, 129; but 64 on 32768 79, so 84; on 8192 39, 47).
+constexpr int kTilesMinChunk = 256, kLongPrefix4 = 1536;
 
-void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, int good) {
+void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, bool bits4) {
     if (few) {
         const int64_t round = (int64_t)fit * kCus;
         const auto chunk_for = [&](int64_t groups) {
             return ceil_div(ceil_div(keys * items, groups), kMinChunk) * kMinChunk;
         };
-        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(good, chunk_for(round)));
+        const int64_t least = std::max<int64_t>(kMinChunk, std::min<int64_t>(bits4 ? kGoodChunk4 : kGoodChunk, chunk_for(round)));
         const int64_t spread = std::min<int64_t>(kRowsPiece, std::max(least, chunk_for(round * kRounds)));
         const int64_t whole = std::max<int64_t>(1, ceil_div(keys, kMinChunk)) * kMinChunk;
         st->chunk = (int)std::min(whole, std::max(spread, chunk_for(round * kMostRounds)));
     } else {
-        const int64_t fill = st->prefix ? kCus : fit * kCus;
+        const bool one = st->prefix && !(bits4 && keys * items >= kLongPrefix4 * 2 * kCus);
+        const int64_t fill = one ? kCus : fit * kCus;
         const int64_t parts = items * 2 > kCus ? 1 : fill / std::max<int64_t>(items, 1);
         st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
     }
@@ -185,8 +188,8 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.own.blocks = (int)std::min<int64_t>(w.batch * ceil_div(seq_rows, p.rows), all_rows / p.rows + w.batch);
     }
     const auto fit = [&](bool few) { return fit_cu(cache.head_dim, few, p.rows, cache.dtype); };
-    const int good = cache.dtype == kE2m1 ? kGoodChunk4 : kGoodChunk;
-    split(&p.own, p.own.blocks * heads, keys, !p.own_waves, fit(!p.own_waves), good);
+    const bool bits4 = cache.dtype == kE2m1;
+    split(&p.own, p.own.blocks * heads, keys, !p.own_waves, fit(!p.own_waves), bits4);
     p.few_waves = 4;
     if (!p.own_waves && !prefix_len && keys <= kRowsShort && p.own.blocks * heads >= kOneWave) {
         p.few_waves = 1;
@@ -198,13 +201,13 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
         p.prefix.prefix = 1;
         p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : 4;
         p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
-        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves), good);
+        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves), bits4);
         p.own.first_slot = p.prefix.splits;
     }
     p.slots = p.own.first_slot + p.own.splits;
     // Turns of 8 workgroups are filled up, of 8 ranges' heads with 4 bits.  The join, where there is one, has as many threads at most.
     const int64_t items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
-    p.threads = (items + 16 + (cache.dtype == kE2m1 ? 16 * heads : 0)) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
+    p.threads = (items + 16 + (bits4 ? 16 * heads : 0)) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
     if (p.slots > 1)
         p.bytes = (int64_t)p.slots * w.num_tokens * w.num_q_heads * (cache.head_dim + 2) * 4 + p.own.blocks * heads * 4;
     return p;

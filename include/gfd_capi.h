@@ -701,7 +701,8 @@ typedef struct gfd_kv_read_rows {
 int gfd_kv_read(const gfd_kv_cache* cache, const gfd_kv_read_rows* rows, int* error_flag, void* stream);
 int gfd_kv4_read(const gfd_kv4_cache* cache, const gfd_kv_read_rows* rows, int* error_flag, void* stream);
 
-/* gfd_attention_workspace_bytes, gfd_paged_attention and
+/* gfd_attention_workspace_bytes (a prefix of more than 32 rows of a head: up to
+ * 512 / num_heads ranges), gfd_paged_attention and
  * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type, exactly in
  * bf16 but for magnitudes under 2^-126; in fp16 as that type holds them (steps of 2^-24, infinite
  * from 65520 on): what rows of that type have appended is exact. */
