@@ -205,7 +205,7 @@ def test_children_in_another_table():
     assert p.refs.sum() == 7 + 3 + 12
 
 
-@pytest.mark.parametrize("num,pages", [(700, 3000), (2500, 20000)])
+@pytest.mark.parametrize("num,pages", [(700, 3000), (2500, 20000), (60, 65536), (60, 65537), (3000, 90000), (1025, 400000)])
 def test_many_items_over_many_chunks(num, pages):
     """More items than places in the search's first step, pages of several workgroups."""
     rng = np.random.default_rng(9)
@@ -254,7 +254,8 @@ def test_long_rows_of_few_sequences():
 # ------------------------------------------------------------ compact
 
 @pytest.mark.parametrize("pages,share", [(1, 1.0), (1, 0.0), (2, 0.5), (7, 0.6), (64, 0.4), (1023, 0.3), (1024, 0.5),
-                                         (1025, 0.9), (5000, 0.02), (5000, 0.5), (20000, 0.7)])
+                                         (1025, 0.9), (5000, 0.02), (5000, 0.5), (20000, 0.7),
+                                         (65536, 0.4), (65537, 0.4), (300000, 0.6)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_pages_brought_together(pages, share, in_place):
     rng = np.random.default_rng(pages)
