@@ -688,7 +688,7 @@ int gfd_kv4_append(const gfd_kv4_cache* cache, const gfd_kv_rows* rows, const gf
 
 /* Tokens' keys and values back out of the cache, as rows of num_heads heads of head_dim
  * elements (GFD_BF16 or GFD_FP16; a 16-bit cache's own type): row t is slot
- * slots[t], times the scale in 32 bits, rounded to the type.  A slot that is
+ * slots[t], 8-bit numbers times the scale in 32 bits and rounded to the type, 4-bit ones as attention reads them.  A slot that is
  * negative leaves its row as it is; one outside the cache too, and is reported. */
 typedef struct gfd_kv_read_rows {
     void* k;                   /* NULL: not wanted */
@@ -703,9 +703,9 @@ int gfd_kv4_read(const gfd_kv4_cache* cache, const gfd_kv_read_rows* rows, int* 
 
 /* gfd_attention_workspace_bytes (a prefix of more than 32 rows of a head: up to
  * 512 / num_heads ranges), gfd_paged_attention and
- * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type, exactly in
- * bf16 but for magnitudes under 2^-126; in fp16 as that type holds them (steps of 2^-24, infinite
- * from 65520 on): what rows of that type have appended is exact. */
+ * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type, exactly but for
+ * magnitudes that it has no numbers for (bf16: under 2^-126, fp16: steps of 2^-24): what rows of that type have
+ * appended is exact.  A group whose scale is over 2^125 (bf16) or 2^13 (fp16) reads as NaN. */
 int64_t gfd_kv4_attention_workspace_bytes(const gfd_kv4_cache* cache, const gfd_attention* call, int prefix_len);
 int gfd_kv4_attention(const gfd_kv4_cache* cache, const gfd_attention* call, void* workspace, size_t workspace_bytes,
                       int* error_flag, void* stream);
@@ -747,7 +747,8 @@ typedef struct gfd_kv_pool {
  * The pages that the items need, in their order, are the free pages in theirs, lowest first:
  * the same call gives the same tables.  A child[i] that is negative is skipped.  child_table may
  * be table if no row is both a parent and a child; no row is a child twice.  Entries past a child's pages
- * stay as they are.  A parent's entry that names no page is passed on as -1. */
+ * stay as they are, and what a child's row named before is not let go of.  A parent's entry that names no page is passed
+ * on as -1; one that names a free page breaks the counts. */
 typedef struct gfd_kv_fork_call {
     const int* table;        /* [rows][table_stride] */
     int* child_table;        /* [child_rows][child_stride] */
