@@ -102,6 +102,7 @@ gfd_kv_cache form_of(const gfd_kv_cache& c) { return c; }
 // How a call is cut into row blocks and key ranges.
 struct Plan {
     int prefix_waves, own_waves;  // of a block of 32 rows a wave; 0: few rows (attend_rows.h)
+    bool apart;                   // the prefix's blocks in a launch of their own
     int few_waves;                // of a workgroup of few rows
     int rows;                     // of an own-keys block
     Stage prefix, own;
@@ -137,9 +138,7 @@ constexpr int kOneWave = 512;
 // tokens over 2000 keys, a block each: 65 us whole, 75 in two ranges), but beside few rows that take the other half
 // of the CUs one (64 requests on 32768 shared keys: 91 us, with two 103).  256 dims: 100 tokens over 4196 keys 54 us,
 // with two workgroups a CU 69; 512 over 2048 84, 98; a prefix of 32768 for 64 requests 160, with two 183.
-// 4 bits: the rest takes less of the CUs, and a prefix whose ranges stay long has as many as fit (64 requests on 65536
-// shared keys 108 us, with one a CU 126; 200 on 16384 114, 129; but 64 on 32768 79, so 84; on 8192 39, 47).
-constexpr int kTilesMinChunk = 256, kLongPrefix4 = 1536;
+constexpr int kTilesMinChunk = 256;
 
 void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, bool bits4) {
     if (few) {
@@ -152,8 +151,7 @@ void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, bool bits4
         const int64_t whole = std::max<int64_t>(1, ceil_div(keys, kMinChunk)) * kMinChunk;
         st->chunk = (int)std::min(whole, std::max(spread, chunk_for(round * kMostRounds)));
     } else {
-        const bool one = st->prefix && !(bits4 && keys * items >= kLongPrefix4 * 2 * kCus);
-        const int64_t fill = one ? kCus : fit * kCus;
+        const int64_t fill = fit * kCus;
         const int64_t parts = items * 2 > kCus ? 1 : fill / std::max<int64_t>(items, 1);
         st->chunk = (int)std::max<int64_t>(kTilesMinChunk, ceil_div(ceil_div(keys, parts), 64) * 64);
     }
@@ -167,6 +165,21 @@ void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, bool bits4
 // 87; 2048 over themselves: 72, 68).
 int tile_waves(int64_t rows, int64_t heads, int dim, bool wide) {
     return dim != 256 && rows * heads >= (wide ? 1 : 2) * 256 * 256 ? 8 : 4;
+}
+
+// A shared prefix's blocks, beside sequences of few rows.  4 bits, where ranges stay kLongPrefix4 keys long with two workgroups
+// of four waves a CU: the rest takes less of the CUs, so those two, or, if that fills up the rows by at most a sixth more, one
+// of 8 waves in a launch of its own (64 requests on 65536 shared keys, rows of 4: 102 us, two 109, one 126; 200 on
+// 16384: 111, 120, 129; 300 on 32768: 205, 225; but 80 on 65536, filled up to 512 rows, 147, 134).  Shorter ones as
+// ever (64 on 32768: one 76, 8 waves 77, two 84; on 8192: 33, 43, 47).
+constexpr int kLongPrefix4 = 1536;
+void plan_prefix(Plan* p, int64_t all_rows, int64_t heads, int prefix_len, int dim, bool bits4, int fit) {
+    const int64_t blocks = ceil_div(all_rows, 128);
+    const bool two = bits4 && prefix_len * blocks * heads >= kLongPrefix4 * 2 * kCus;
+    p->apart = two && dim != 256 && 12 * ceil_div(all_rows, 256) <= 7 * blocks;
+    p->prefix_waves = p->apart ? 8 : 4;
+    p->prefix.blocks = (int)ceil_div(all_rows, 32 * p->prefix_waves);
+    split(&p->prefix, p->prefix.blocks * heads, prefix_len, false, two && !p->apart ? fit : 1, bits4);
 }
 
 Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len) {
@@ -199,9 +212,13 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
     p.own.direct = !prefix_len;
     if (prefix_len) {
         p.prefix.prefix = 1;
-        p.prefix_waves = all_rows <= 32 ? 0 : p.own_waves ? p.own_waves : 4;
-        p.prefix.blocks = (int)ceil_div(all_rows, p.prefix_waves ? 32 * p.prefix_waves : p.rows);
-        split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.prefix_waves, fit(!p.prefix_waves), bits4);
+        if (all_rows <= 32 || p.own_waves) {
+            p.prefix_waves = p.own_waves;
+            p.prefix.blocks = (int)ceil_div(all_rows, p.rows);
+            split(&p.prefix, p.prefix.blocks * heads, prefix_len, !p.own_waves, p.own_waves ? 1 : fit(true), bits4);
+        } else {
+            plan_prefix(&p, all_rows, heads, prefix_len, cache.head_dim, bits4, fit(false));
+        }
         p.own.first_slot = p.prefix.splits;
     }
     p.slots = p.own.first_slot + p.own.splits;
@@ -236,7 +253,7 @@ int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st
     int rc;
     if (p.own_waves) {  // both stages have blocks of the same rows
         rc = launch_tiles<T, S>(a, c, p.prefix, p.own, dim, p.own_waves, st);
-    } else if (p.prefix_waves && p.own.chunk > kRowsPiece) {  // a batch that fills the card without the prefix
+    } else if (p.prefix_waves && (p.apart || p.own.chunk > kRowsPiece)) {  // or a batch that fills the card without the prefix
         const Stage none{0, 0, 0, 0, 1, 0, 0};
         rc = launch_tiles<T, S>(a, c, p.prefix, none, dim, p.prefix_waves, st);
         if (!rc) rc = launch_rows<T, S>(a, c, none, p.own, dim, p.rows == 32, p.few_waves, st);
