@@ -5,7 +5,9 @@
 // drafted tokens on 5001 shared 8-bit keys: 30 us, 40).  The prefix goes first: its workgroups are the long ones, and
 // taking the two kinds by turns left one of them a CU (128 us).  Of 256 dims one workgroup fits a CU, and the rest
 // follows the prefix on the CUs that end first: it is as good as two launches (64 requests on 32768: 160 us, 156; 200 on
-// 16384: 345, 368; 17 times 4 tokens on 5001 in 8 bits: 61, 61).
+// 16384: 345, 368; 17 times 4 tokens on 5001 in 8 bits: 61, 61).  64 requests on 32768 shared keys in 4 bits: 72 us,
+// where one wave a SIMD waits for each step of a tile: without the conversions, the exponents, one of the products or the loads it takes
+// no more than 6% less.  Longer 4-bit prefixes are launched apart (plan_prefix).
 #include "attend_rows.h"
 #include "attend_tiles.h"
 
