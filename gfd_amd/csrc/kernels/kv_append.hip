@@ -154,7 +154,10 @@ struct Store<E4m3> {
 // The first values are under way while the turns are computed.  Bound by the rows' and
 // the cache's bytes, which it moves at the rate of a large copy: 16384 tokens of 32 + 8 heads of 128 into an 8-bit cache,
 // 369 MB in 73 us; 4097 tokens of 64 rotated dims, 101 MB in 21.5 us.  Eight tokens take a launch.
-template <typename T, typename S, int kPairs, int kTokensHere>
+// Positions of several axes have kernels of their own (kAxes): where one kernel asks which kind it has, the 4097 tokens
+// take 24.5 us, of 36 rotated dims 6001 take 38.4 for 33.5.  The rows' loads differ too, each the faster one or even: with the other
+// one 4097 tokens of one axis take 23.1 us for 22.0 (side by side), 16384 of three 81.9 for 81.0.
+template <typename T, typename S, int kPairs, int kTokensHere, bool kAxes>
 __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
     __shared__ f32x2 turns[kTokensHere][128];
     __shared__ int64_t places[kTokensHere];
@@ -185,8 +188,16 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
             u.b = u.a + half;
         }
         const int64_t t = t0 + u.t;
-        u.x = eight_of(r, u.kind, t, u.head * r.dim + u.a);
-        u.y = eight_of(r, u.kind, t, u.head * r.dim + u.b);
+        if constexpr (kAxes) {
+            u.x = eight_of(r, u.kind, t, u.head * r.dim + u.a);
+            u.y = eight_of(r, u.kind, t, u.head * r.dim + u.b);
+        } else {
+            const uint16_t* p = (u.kind == 0   ? r.q + t * r.q_stride
+                                 : u.kind == 1 ? r.k + t * r.k_stride
+                                               : r.v + t * r.v_stride) + (int64_t)u.head * r.dim;
+            u.x = *(const u32x4*)(p + u.a);
+            u.y = *(const u32x4*)(p + u.b);
+        }
         return u;
     };
     Unit u;
@@ -194,7 +205,8 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
 
     for (int n = tid; n < tokens * half; n += kBlock) {
         const int t = n / half, i = n - t * half;
-        const double whole = position_of(r, t0 + t, i) * ((double)r.inv_freq[i] * 0.15915494309189533577);
+        const double position = kAxes ? position_of(r, t0 + t, i) : (double)r.positions[t0 + t];
+        const double whole = position * ((double)r.inv_freq[i] * 0.15915494309189533577);
         float s, co;
         sincospif((float)(2.0 * (whole - rint(whole))), &s, &co);
         turns[t][i] = f32x2{co, s};
@@ -282,19 +294,21 @@ __global__ __launch_bounds__(kBlock) void kv_append_kernel(Rows r, Cache c) {
     }
 }
 
-template <typename T, typename S, int kTokensHere>
+template <typename T, typename S, int kTokensHere, bool kAxes>
 int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
     const dim3 grid((unsigned)((r.num_tokens + kTokensHere - 1) / kTokensHere));
     const auto go = [&](auto kernel) { return start(kernel, grid, kBlock, st, r, c); };
-    if (pairs) return go(kv_append_kernel<T, S, kSide, kTokensHere>);
-    if (r.rotary % 16 == 0) return go(kv_append_kernel<T, S, kChunksApart, kTokensHere>);
-    return go(kv_append_kernel<T, S, kApart, kTokensHere>);
+    if (pairs) return go(kv_append_kernel<T, S, kSide, kTokensHere, kAxes>);
+    if (r.rotary % 16 == 0) return go(kv_append_kernel<T, S, kChunksApart, kTokensHere, kAxes>);
+    return go(kv_append_kernel<T, S, kApart, kTokensHere, kAxes>);
 }
 
 // Tokens share a workgroup's start-up where that still fills the card.
 template <typename T, typename S>
 int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
-    return r.num_tokens >= 2048 * kTokens ? launch<T, S, kTokens>(r, c, pairs, st) : launch<T, S, 1>(r, c, pairs, st);
+    const bool many = r.num_tokens >= 2048 * kTokens;
+    if (r.axis) return many ? launch<T, S, kTokens, true>(r, c, pairs, st) : launch<T, S, 1, true>(r, c, pairs, st);
+    return many ? launch<T, S, kTokens, false>(r, c, pairs, st) : launch<T, S, 1, false>(r, c, pairs, st);
 }
 
 int append(const char* name, const gfd_kv_cache* cache, const gfd_kv_rows* rows, const gfd_rotary_axes* axes,
