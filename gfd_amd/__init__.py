@@ -947,17 +947,22 @@ def _bytes(name, *args):
     return n
 
 
+# A KVCache's calls go straight to their functions: small ones are bound by what this side does for them (through _call()
+# 0.2 us more a call, of which the test of a structure's class takes half).
+
 def kv_append(cache, rows, error_flag=None, stream=None, axes=None):
     """Rotate the queries and keys of `rows` (KVRows) to their positions, or to
     those of `axes` (RotaryAxes), and append the keys and values to `cache`
     (KVCache or KV4Cache).  error_flag: device int that takes KV_ERR_* bits.  See gfd_kv_append,
     gfd_kv_append_axes and gfd_kv4_append in include/gfd_capi.h."""
-    if isinstance(cache, KV4Cache):
+    if type(cache) is not KVCache and isinstance(cache, KV4Cache):
         _call("gfd_kv4_append", cache, rows, axes, error_flag, stream)
     elif axes is not None:
         _call("gfd_kv_append_axes", cache, rows, axes, error_flag, stream)
     else:
-        _call("gfd_kv_append", cache, rows, error_flag, stream)
+        rc = lib().gfd_kv_append(cache, rows, error_flag, stream)
+        if rc:
+            _check(rc, "gfd_kv_append")
 
 
 def kv_read(cache, rows, error_flag=None, stream=None):
@@ -970,23 +975,35 @@ def attention_workspace_bytes(cache, call, prefix_len=0):
     shared_prefix_attention() needs for `call` (Attention).  Depends on every
     size of the call and is not the largest for the largest batch: keep the
     largest of those that a program makes, or ask for each."""
-    return _bytes("gfd_kv4_attention_workspace_bytes" if isinstance(cache, KV4Cache) else
-                  "gfd_attention_workspace_bytes", cache, call, prefix_len)
+    if type(cache) is not KVCache and isinstance(cache, KV4Cache):
+        return _bytes("gfd_kv4_attention_workspace_bytes", cache, call, prefix_len)
+    n = lib().gfd_attention_workspace_bytes(cache, call, prefix_len)
+    if n < 0:
+        _check(-1, "gfd_attention_workspace_bytes")
+    return n
 
 
 def paged_attention(cache, call, workspace=None, workspace_bytes=0, error_flag=None, stream=None):
     """Attention of `call` (Attention) over `cache` (KVCache or KV4Cache); see
     gfd_paged_attention and gfd_kv4_attention in include/gfd_capi.h."""
-    _call("gfd_kv4_attention" if isinstance(cache, KV4Cache) else "gfd_paged_attention", cache, call, workspace,
-          workspace_bytes, error_flag, stream)
+    if type(cache) is not KVCache and isinstance(cache, KV4Cache):
+        return _call("gfd_kv4_attention", cache, call, workspace, workspace_bytes, error_flag, stream)
+    rc = lib().gfd_paged_attention(cache, call, workspace, workspace_bytes, error_flag, stream)
+    if rc:
+        _check(rc, "gfd_paged_attention")
 
 
 def shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace=None, workspace_bytes=0, error_flag=None,
                             stream=None):
     """paged_attention() of sequences whose first prefix_len keys are the same
     ones, in the pages of prefix_table; they are read once for all."""
-    _call("gfd_kv4_shared_prefix_attention" if isinstance(cache, KV4Cache) else "gfd_shared_prefix_attention", cache,
-          call, prefix_table, prefix_len, workspace, workspace_bytes, error_flag, stream)
+    if type(cache) is not KVCache and isinstance(cache, KV4Cache):
+        return _call("gfd_kv4_shared_prefix_attention", cache, call, prefix_table, prefix_len, workspace,
+                     workspace_bytes, error_flag, stream)
+    rc = lib().gfd_shared_prefix_attention(cache, call, prefix_table, prefix_len, workspace, workspace_bytes,
+                                           error_flag, stream)
+    if rc:
+        _check(rc, "gfd_shared_prefix_attention")
 
 
 def kv_copy_pages(dst, src, copies, max_copies, count=None, error_flag=None, stream=None):
