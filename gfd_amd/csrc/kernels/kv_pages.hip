@@ -563,6 +563,8 @@ extern "C" int gfd_kv_fork(const gfd_kv_pool* pool, const gfd_kv_fork_call* call
     if (w.num == 0) return 0;
     if (!w.parent || !w.child || !w.len || !w.child_table || (w.rows && !w.table))
         return refused(kName, "parent, child, len or a table is missing");
+    if (w.rows && w.table == w.child_table && w.table_stride != w.child_stride)
+        return refused(kName, "table and child_table are one, with two strides");
     if (!w.copies || (uintptr_t)w.copies % 16 != 0) return refused(kName, "copies is missing or not 16-byte aligned");
     if (const char* why = check_workspace(*pool, w.num, workspace, workspace_size)) return refused(kName, why);
     const Pool p = make_pool(*pool);
@@ -604,6 +606,8 @@ extern "C" int gfd_kv_compact(const gfd_kv_pool* pool, const gfd_kv_compact_call
     if (w.rows > kMostItems) return refused(kName, "more than 2^20 rows");
     if (!w.new_refs || !w.num_copies || (w.rows && (!w.table || !w.new_table || !w.len)))
         return refused(kName, "new_refs, num_copies, a table or len is missing");
+    if (w.rows && w.table == w.new_table && w.table_stride != w.new_stride)
+        return refused(kName, "table and new_table are one, with two strides");
     if ((!w.copies && pool->num_pages > 1) || (uintptr_t)w.copies % 16 != 0)
         return refused(kName, "copies is missing or not 16-byte aligned");
     if (const char* why = check_workspace(*pool, 0, workspace, workspace_size)) return refused(kName, why);

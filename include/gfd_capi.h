@@ -746,7 +746,7 @@ typedef struct gfd_kv_pool {
  * Then it gets free pages up to capacity[i] tokens (NULL, or less than len[i]: len[i]), refs 1.
  * The pages that the items need, in their order, are the free pages in theirs, lowest first:
  * the same call gives the same tables.  A child[i] that is negative is skipped.  child_table may
- * be table if no row is both a parent and a child; no row is a child twice.  Entries past a child's pages
+ * be table (with one stride) if no row is both a parent and a child; no row is a child twice.  Entries past a child's pages
  * stay as they are, and what a child's row named before is not let go of.  A parent's entry that names no page is passed
  * on as -1; one that names a free page breaks the counts. */
 typedef struct gfd_kv_fork_call {
@@ -774,7 +774,7 @@ int gfd_kv_free(const gfd_kv_pool* pool, const int* table, int64_t table_stride,
 
 /* Brings a cache's n used pages to its first n: the used pages from n on, in their order, go to the free
  * ones before n.  copies ([num_pages / 2] at most) and *num_copies say what to copy,
- * new_table and new_refs are the tables and counts after it (they may be table and
+ * new_table and new_refs are the tables and counts after it (they may be table, with one stride, and
  * pool->refs themselves), page_map (NULL: not wanted) where each page is then, -1 for
  * free ones, for what else names pages.  Entries past a row's len stay as new_table has them. */
 typedef struct gfd_kv_compact_call {
