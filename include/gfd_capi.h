@@ -667,7 +667,7 @@ enum {
  * of a head turns by its own axis's position, positions[axis[i] * axis_stride +
  * token * token_stride] * inv_freq[i].  gfd_kv_rows's positions are not read then. */
 typedef struct gfd_rotary_axes {
-    const void* positions;     /* int, or float with float_positions (finite) */
+    const void* positions;     /* int, or float with float_positions (magnitudes up to 2^31) */
     const uint8_t* axis;       /* [rotary_dim / 2] */
     int64_t axis_stride, token_stride;  /* elements */
     int num_axes;              /* 1 to 256 */
@@ -703,8 +703,8 @@ int gfd_kv4_read(const gfd_kv4_cache* cache, const gfd_kv_read_rows* rows, int* 
 
 /* gfd_attention_workspace_bytes (a prefix of more than 32 rows of a head: up to
  * 512 / num_heads ranges), gfd_paged_attention and
- * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type, exactly but for
- * magnitudes that it has no numbers for (bf16: under 2^-126, fp16: steps of 2^-24): what rows of that type have
+ * gfd_shared_prefix_attention over a 4-bit cache.  The numbers are widened to q's type: exactly in bf16, in fp16
+ * below 2^-14 to the nearest multiple of 2^-24 (ties to even); what rows of that type have
  * appended is exact.  A group whose scale is over 2^125 (bf16) or 2^13 (fp16) reads as NaN. */
 int64_t gfd_kv4_attention_workspace_bytes(const gfd_kv4_cache* cache, const gfd_attention* call, int prefix_len);
 int gfd_kv4_attention(const gfd_kv4_cache* cache, const gfd_attention* call, void* workspace, size_t workspace_bytes,
