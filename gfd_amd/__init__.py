@@ -1025,12 +1025,14 @@ def kv_fork(pool, call, workspace, workspace_bytes, error_flag=None, stream=None
 
 
 def kv_free(pool, table, table_stride, rows, row, length, num, error_flag=None, stream=None):
-    """Let go of the pages of length[i] tokens of row[i] of a table (device arrays, num items)."""
+    """Let go of the pages of length[i] tokens of row[i] of a table (device arrays, num items); length: the capacities that
+    the rows' pages were given for."""
     _call("gfd_kv_free", pool, table, table_stride, rows, row, length, num, error_flag, stream)
 
 
 def kv_compact(pool, call, workspace, workspace_bytes, error_flag=None, stream=None):
-    """Bring the used pages of `pool` to its front (`call`: KVCompact); see gfd_kv_compact in include/gfd_capi.h."""
+    """Bring the used pages of `pool` to its front (`call`: KVCompact; its len: the capacities that the rows' pages were given
+    for); see gfd_kv_compact in include/gfd_capi.h."""
     _call("gfd_kv_compact", pool, call, workspace, workspace_bytes, error_flag, stream)
 
 

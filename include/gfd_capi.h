@@ -768,7 +768,9 @@ int gfd_kv_fork(const gfd_kv_pool* pool, const gfd_kv_fork_call* call, void* wor
                 int* error_flag, void* stream);
 
 /* Lets go of the pages of len[i] tokens of row row[i] of table, i < num: each entry's
- * page has one less in refs.  Negative rows and entries are skipped; the table stays as it is. */
+ * page has one less in refs.  len[i] is the capacity that the row's pages were given for (gfd_kv_fork's), not how many
+ * tokens are in them yet: pages past it stay held, by a row that no longer counts them.
+ * Negative rows and entries are skipped; the table stays as it is. */
 int gfd_kv_free(const gfd_kv_pool* pool, const int* table, int64_t table_stride, int rows, const int* row,
                 const int* len, int num, int* error_flag, void* stream);
 
@@ -776,13 +778,15 @@ int gfd_kv_free(const gfd_kv_pool* pool, const int* table, int64_t table_stride,
  * ones before n.  copies ([num_pages / 2] at most) and *num_copies say what to copy,
  * new_table and new_refs are the tables and counts after it (they may be table, with one stride, and
  * pool->refs themselves), page_map (NULL: not wanted) where each page is then, -1 for
- * free ones, for what else names pages.  Entries past a row's len stay as new_table has them. */
+ * free ones, for what else names pages.  A row's len is the capacity that its pages were given for (gfd_kv_fork's), not how
+ * many tokens are in them yet.  Entries past it stay as new_table has them: pages that a row was given but that its len does
+ * not reach move all the same, and its entries then name what is free or another row's, which its next tokens would overwrite. */
 typedef struct gfd_kv_compact_call {
     int* new_refs;           /* [num_pages] */
     const int* table;        /* [rows][table_stride] */
     int* new_table;          /* [rows][new_stride] */
     int64_t table_stride, new_stride;
-    const int* len;          /* [rows], tokens */
+    const int* len;          /* [rows], tokens: the capacities */
     int rows;
     int* page_map;           /* [num_pages] */
     gfd_kv_page_copy* copies;
