@@ -24,7 +24,9 @@
 // 64 x 8192 keys of 8 heads of 128 in bf16: 2.1 GB in 361 us, 5.9 TB/s (a large read: 6.2).
 // 64 ragged contexts of up to 8192: 160 us, 5.2 TB/s.  33 windows of 4096 keys of 256 dims in 8 bits,
 // capped: 60 us, 4.9 TB/s.  4-bit keys of 128 dims: 64 x 8192 of them in 120 us, 4.7 TB/s, 64 ragged contexts of up to 16384 in
-// 97, where the loads alone take 105 of the 120 and the conversions, products and exponents alone 102.
+// 97, where the loads alone take 105 of the 120 and the conversions, products and exponents alone 102.  Several tokens of 4
+// heads a key, 64 ragged contexts of up to 8192 in 4 bits: 1 token 58 us, 2 60, 4 (16 rows) 65, 5 (20 rows) 99, 8 104: of 17 to 32
+// rows a lane holds twice the results, and two waves fit a SIMD in place of four.
 // 700 keys of one token: 7.6 us and 3.9 to join, a chain of loads (lengths, pages, keys) and a launch each.  Many
 // short contexts take a wave each: 128 of 128 keys in 16 us, 4.2 TB/s.
 #include <algorithm>

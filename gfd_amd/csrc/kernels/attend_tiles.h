@@ -22,10 +22,12 @@
 // average neither pipe is full (20% and 31%), a wave waits 36% of its time for results.
 // 7 ragged prompts of 64 dims with a bias: 57 us, the 30 tiles of the longest one by 4 waves, one a SIMD, which waits
 // 47% of its time: a tile's scores, maximum, exponents and values follow one another, and nothing else is there.
-// 4-bit keys, 2048 tokens over 8192, 32 heads of 128: 260 us, 920 TFLOP/s, pipes at 37% at 2.1 GHz with 1.7 waves a SIMD.
+// 4-bit keys, 2048 tokens over 8192, 32 heads of 128: 262 us, 920 TFLOP/s, pipes at 37% at 2.1 GHz with 1.7 waves a SIMD;
+// capped 319, biased 293, 6 packed documents 90, each token with a window of 1024 keys 51; of 64 dims 179, capped 265, biased 217;
+// 1024 tokens of 16 heads of 256 dims 256, capped, biased and in 6 documents 245.
 // Tried and slower: half of the waves a product behind the others (1130 us for 1096), tiles of 32 keys with
 // three under way (2048 tokens 85 us for 74), two groups of 4 waves to a block (packed tokens 263 us for 223).
-// Of 4 bits, the scores of a tile before the weights of the one ahead of it: 2048 over 8192 270 us for 258.
+// Of 4 bits, the scores of a tile before the weights of the one ahead of it: 2048 over 8192 takes 5% more.
 #include <type_traits>
 
 #include "paged_attention.h"

