@@ -15,7 +15,7 @@ namespace gfd {
 namespace kv {
 
 template <typename T, typename S, int D, int R, int kScores>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call a, Cache c, Stage prefix,
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call a, CacheOf<S> c, Stage prefix,
                                                                                   Stage own, int prefix_turns) {
     __shared__ union Lds {
         RowsLds<T, S, D, R, 4> rows;
@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_both_kernel(Call
 }
 
 template <typename T, typename S>
-int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+int launch_both(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, bool wide,
                 hipStream_t st) {
     const Stage none{0, 0, 0, 0, 1, 0, 0};
     const int prefix_turns = (int)(tiles_groups(a, prefix, none) / 8),

@@ -210,7 +210,7 @@ struct RowsKernel<T, E2m1, D, R> : RowsShape<T, E2m1, D, R, D == 64 ? 2 : 4> {
     };
 
     // there: a bit for each key.
-    static __device__ __forceinline__ void load(Tile& t, const Cache& c, const Place4* off, uint32_t there, int lane) {
+    static __device__ __forceinline__ void load(Tile& t, const Cache4& c, const Place4* off, uint32_t there, int lane) {
         const uint32_t w = there >> 4 * (lane >> 4);
         t.valid = (w & 15) | (w >> 12 & 0xF0);
         int64_t o[kKeyLoads];
@@ -305,7 +305,7 @@ struct RowsKernel<T, E2m1, D, R> : RowsShape<T, E2m1, D, R, D == 64 ? 2 : 4> {
             }
         }
     }
-    static __device__ __forceinline__ Value value(const Cache& c, const Place4& place, int n) {
+    static __device__ __forceinline__ Value value(const Cache4& c, const Place4& place, int n) {
         Value x;
         const auto w = load_words<kValBytes>(c.v + place.row + n * kValBytes);
 #pragma unroll
@@ -344,7 +344,7 @@ struct RowsLds {
 
 // kWaves 1: ranges of at most kRowsShort keys.  kPieces: ranges of more than kRowsPiece keys.
 template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
-__device__ __forceinline__ void attend_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int item,
+__device__ __forceinline__ void attend_rows(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int item,
                                             RowsLds<T, S, D, R, kWaves>& lds) {
     using K = RowsKernel<T, S, D, R>;
     constexpr int kRows = 16 * R, kThreads = 64 * kWaves;
@@ -725,7 +725,7 @@ int64_t rows_groups(int64_t ranges, int heads) {
 
 template <typename T, typename S, int D, int R, int kWaves, bool kPieces>
 __global__ __launch_bounds__(64 * kWaves, (rows_waves<S, D, R, kPieces>())) void attend_rows_kernel(
-    Call a, Cache c, Stage prefix, Stage own) {
+    Call a, CacheOf<S> c, Stage prefix, Stage own) {
     __shared__ RowsLds<T, S, D, R, kWaves> lds;
     const int item = rows_item<S>((int)blockIdx.x, a.kv_heads);
     if (S::kBits == 4 && item >= (prefix.blocks * prefix.splits + own.blocks * own.splits) * a.kv_heads) return;
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(64 * kWaves, (rows_waves<S, D, R, kPieces>())) void
 }
 
 template <typename T, typename S>
-int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
+int launch_rows(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st) {
     const dim3 grid((unsigned)rows_groups<S>((int64_t)prefix.blocks * prefix.splits + (int64_t)own.blocks * own.splits, a.kv_heads));
     const auto go = [&](auto kernel) { return start(kernel, grid, 64 * waves, st, a, c, prefix, own); };

@@ -60,7 +60,7 @@ struct TilesKernel {
     static __device__ __forceinline__ int swap_v(int row) { return D == 64 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 
     // kc and vc: the thread's chunk of the cache's first row.
-    static __device__ __forceinline__ void load(Staged& g, const Cache& c, const uint8_t* kc, const uint8_t* vc,
+    static __device__ __forceinline__ void load(Staged& g, const CacheOf<S>& c, const uint8_t* kc, const uint8_t* vc,
                                                 const Place<S>* off, int tid) {
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
@@ -143,7 +143,7 @@ struct TilesLds {
 };
 
 template <typename T, typename S, int D, int W, int kScores>
-__device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int id,
+__device__ __forceinline__ void attend_tiles(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int id,
                                              TilesLds<T, S, D, W>& lds) {
     using K = TilesKernel<T, S, D, W>;
     constexpr int kTile = K::kTile, kRows = K::kRows;
@@ -523,7 +523,7 @@ __device__ __forceinline__ void attend_tiles(const Call& a, const Cache& c, cons
 }
 
 template <typename T, typename S, int D, int W, int kScores>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(Call a, Cache c, Stage prefix, Stage own) {
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attend_tiles_kernel(Call a, CacheOf<S> c, Stage prefix, Stage own) {
     __shared__ TilesLds<T, S, D, W> lds;
     attend_tiles<T, S, D, W, kScores>(a, c, prefix, own, (int)blockIdx.x, lds);
 }
@@ -546,7 +546,7 @@ int with_scores(const Call& a, F f) {
 }
 
 template <typename T, typename S>
-int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
+int launch_tiles(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, int waves,
                  hipStream_t st) {
     const dim3 grid((unsigned)tiles_groups(a, prefix, own));
     const auto go = [&](auto kernel, int w) {

@@ -53,7 +53,7 @@ __device__ __forceinline__ float across4_max(float x) {
 // A thread takes 8 values of a head at a time, so four neighbours have a group, and a head's threads are of one wave: they
 // pass their chunks through LDS for the other halves of their pairs.
 template <typename T, int kPairs, int kTokensHere>
-__global__ __launch_bounds__(kBlock) void kv4_append_kernel(Rows r, Cache c) {
+__global__ __launch_bounds__(kBlock) void kv4_append_kernel(Rows r, Cache4 c) {
     __shared__ f32x2 turns[kTokensHere][128];
     __shared__ Place4 places[kTokensHere];  // row -1: none
     __shared__ u32x4 chunks[kPairs == kSide ? 1 : kBlock];
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kBlock) void kv4_append_kernel(Rows r, Cache c) {
 }
 
 template <typename T, int kTokensHere>
-int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
+int launch(const Rows& r, const Cache4& c, bool pairs, hipStream_t st) {
     const dim3 grid((unsigned)((r.num_tokens + kTokensHere - 1) / kTokensHere));
     const auto go = [&](auto kernel) { return start(kernel, grid, kBlock, st, r, c); };
     if (pairs) return go(kv4_append_kernel<T, kSide, kTokensHere>);
@@ -195,7 +195,7 @@ int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
 
 // Tokens share a workgroup's start-up where that still fills the card.
 template <typename T>
-int launch(const Rows& r, const Cache& c, bool pairs, hipStream_t st) {
+int launch(const Rows& r, const Cache4& c, bool pairs, hipStream_t st) {
     return r.num_tokens >= 2048 * kTokens ? launch<T, kTokens>(r, c, pairs, st) : launch<T, 1>(r, c, pairs, st);
 }
 
@@ -211,7 +211,7 @@ extern "C" int gfd_kv4_append(const gfd_kv4_cache* cache, const gfd_kv_rows* row
     if (const char* why = check_rows(rows, cache->head_dim, axes)) return refused(kName, why);
     if (rows->num_tokens == 0) return 0;
     const Rows r = make_rows(*rows, cache->num_heads, cache->head_dim, axes, 1.f, 1.f, error_flag);
-    const Cache c = make_cache(*cache);
+    const Cache4 c = make_cache(*cache);
     const bool pairs = rows->interleaved != 0;
     return launched(kName, rows->dtype == GFD_BF16 ? launch<Bf16>(r, c, pairs, (hipStream_t)stream)
                                                    : launch<Fp16>(r, c, pairs, (hipStream_t)stream));

@@ -51,18 +51,22 @@ const char* check_cache(const gfd_kv4_cache* c) {
     return nullptr;
 }
 
-Cache make_cache(const gfd_kv4_cache& c) {
-    return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride, c.slot_stride, c.head_stride, c.num_pages,
-                 make_divider((uint32_t)c.page_size), 1.f, 1.f, (uint8_t*)c.k_scales, (uint8_t*)c.v_scales,
-                 c.scale_page_stride, c.head_stride <= c.slot_stride};
+Cache4 make_cache(const gfd_kv4_cache& c) {
+    Cache4 x;
+    (Cache&)x = Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride, c.slot_stride, c.head_stride, c.num_pages,
+                      make_divider((uint32_t)c.page_size), 1.f, 1.f};
+    x.k_scales = (uint8_t*)c.k_scales;
+    x.v_scales = (uint8_t*)c.v_scales;
+    x.scale_page_stride = c.scale_page_stride;
+    x.heads_inner = c.head_stride <= c.slot_stride;
+    return x;
 }
 
 Cache make_cache(const gfd_kv_cache& c) {
     const int64_t size = c.dtype == GFD_E4M3 ? 1 : 2;
     const bool scaled = c.dtype == GFD_E4M3;
     return Cache{(uint8_t*)c.k, (uint8_t*)c.v, c.page_stride * size, c.slot_stride * size, c.head_stride * size,
-                 c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f,
-                 nullptr, nullptr, 0, 0};
+                 c.num_pages, make_divider((uint32_t)c.page_size), scaled ? c.k_scale : 1.f, scaled ? c.v_scale : 1.f};
 }
 
 const char* check_rows(const gfd_kv_rows* rows, int head_dim, const gfd_rotary_axes* axes) {

@@ -387,8 +387,9 @@ __global__ __launch_bounds__(kBlock) void compact_kernel(Compact f, int copy_gro
 
 // ------------------------------------------------------------------ copy
 
+template <typename S>
 struct Copy {
-    Cache dst, src;
+    CacheOf<S> dst, src;
     const gfd_kv_page_copy* copies;
     const int* count;
     int max_copies, heads, row_chunks, parts, heads_inner;  // chunks of 16 bytes a row: 2^row_chunks
@@ -401,7 +402,7 @@ constexpr int kUnits = 4;  // rows' chunks a thread copies at once, of keys and 
 // A workgroup copies kBlock kUnits chunks of 16 bytes of a page's keys and the same of its values, in the order of the
 // destination; with a chunk of 4-bit numbers goes its scale.  Bound by the bytes.
 template <typename S>
-__global__ __launch_bounds__(kBlock) void copy_pages_kernel(Copy f, int64_t groups) {
+__global__ __launch_bounds__(kBlock) void copy_pages_kernel(Copy<S> f, int64_t groups) {
     const int count = f.count ? min(max(*f.count, 0), f.max_copies) : f.max_copies;
     const int rows = f.heads * (int)f.dst.page.d;
     for (int64_t g = blockIdx.x; g < groups; g += gridDim.x) {
@@ -456,7 +457,7 @@ int copy_pages(const char* name, const C* dst, const C* src, const gfd_kv_page_c
     if (max_copies < 0) return refused(name, "negative max_copies");
     if (max_copies == 0) return 0;
     if (!copies || (uintptr_t)copies % 16 != 0) return refused(name, "copies is missing or not 16-byte aligned");
-    Copy f{make_cache(*dst), make_cache(*src), copies, count, max_copies, dst->num_heads, 0, 0, 0, {}, error};
+    Copy<S> f{make_cache(*dst), make_cache(*src), copies, count, max_copies, dst->num_heads, 0, 0, 0, {}, error};
     while (16 * 8 << f.row_chunks < dst->head_dim * S::kBits) f.row_chunks++;
     const int64_t units = ((int64_t)dst->num_heads * dst->page_size) << f.row_chunks;
     if (units >= 1ll << 31) return refused(name, "a page has more than 2^31 chunks of 16 bytes");

@@ -51,8 +51,10 @@ constexpr int kUnits = 2;  // a thread's, at once
 // back over three caches by turns, pages in any order: 16 bits 134 MB in 28.6 us (4.7 TB/s), 8 bits 101 MB in 23.9, 4 bits 21.1; 1000
 // tokens 3.9, 4.2, 4.0, a launch.
 template <typename T, typename S>
-__global__ __launch_bounds__(kBlock) void kv_read_kernel(ReadRows r, Cache c, Divider per_token) {
+__global__ __launch_bounds__(kBlock) void kv_read_kernel(ReadRows r, CacheOf<S> c, Divider per_token) {
     const int shift = r.dim == 64 ? 3 : r.dim == 128 ? 4 : 5;  // units of 8 values a head
+    const uint8_t *k_scales = nullptr, *v_scales = nullptr;
+    if constexpr (S::kBits == 4) k_scales = c.k_scales, v_scales = c.v_scales;
     const int64_t units = (int64_t)r.num_tokens * per_token.d, step = (int64_t)gridDim.x * kBlock * kUnits;
     for (int64_t first = (int64_t)blockIdx.x * kBlock * kUnits; first < units; first += step) {
         u32x4 k[kUnits], v[kUnits];
@@ -75,8 +77,8 @@ __global__ __launch_bounds__(kBlock) void kv_read_kernel(ReadRows r, Cache c, Di
             }
             const int64_t page = slot / c.page.d;
             const auto place = place_of<S>(c, (int)page, (uint32_t)(slot - page * c.page.d), head * c.head_stride);
-            if (r.k) k[i] = eight<T, S>(c.k, c.k_scales, place, a, c.k_scale);
-            if (r.v) v[i] = eight<T, S>(c.v, c.v_scales, place, a, c.v_scale);
+            if (r.k) k[i] = eight<T, S>(c.k, k_scales, place, a, c.k_scale);
+            if (r.v) v[i] = eight<T, S>(c.v, v_scales, place, a, c.v_scale);
         }
 #pragma unroll
         for (int i = 0; i < kUnits; i++) {
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(kBlock) void kv_read_kernel(ReadRows r, Cache c, Di
 }
 
 template <typename T, typename S>
-int launch(const ReadRows& r, const Cache& c, hipStream_t st) {
+int launch(const ReadRows& r, const CacheOf<S>& c, hipStream_t st) {
     const int per_token = r.heads * (r.dim / 8);
     const int64_t groups = ((int64_t)r.num_tokens * per_token + kBlock * kUnits - 1) / (kBlock * kUnits);
     return start(kv_read_kernel<T, S>, dim3((unsigned)std::min<int64_t>(groups, 1 << 20)), kBlock, st, r, c,
@@ -125,7 +127,7 @@ extern "C" int gfd_kv_read(const gfd_kv_cache* cache, const gfd_kv_read_rows* ro
         return refused(kName, "the cache's type is neither the rows' nor GFD_E4M3");
     if (rows->num_tokens == 0 || (!rows->k && !rows->v)) return 0;
     const ReadRows r = make(*rows, *cache, error_flag);
-    const Cache c = make_cache(*cache);
+    const auto c = make_cache(*cache);
     const hipStream_t st = (hipStream_t)stream;
     if (cache->dtype == GFD_E4M3)
         return launched(kName, rows->dtype == GFD_BF16 ? launch<Bf16, E4m3>(r, c, st) : launch<Fp16, E4m3>(r, c, st));
@@ -139,7 +141,7 @@ extern "C" int gfd_kv4_read(const gfd_kv4_cache* cache, const gfd_kv_read_rows* 
     if (const char* why = check(rows)) return refused(kName, why);
     if (rows->num_tokens == 0 || (!rows->k && !rows->v)) return 0;
     const ReadRows r = make(*rows, *cache, error_flag);
-    const Cache c = make_cache(*cache);
+    const auto c = make_cache(*cache);
     const hipStream_t st = (hipStream_t)stream;
     return launched(kName, rows->dtype == GFD_BF16 ? launch<Bf16, E2m1>(r, c, st) : launch<Fp16, E2m1>(r, c, st));
 }

@@ -225,7 +225,7 @@ __device__ __forceinline__ int head_of(const Call& a, const Block& k, int r, int
 
 // Where a key lies; false: nowhere, its page is none of the cache's.
 template <typename S>
-__device__ __forceinline__ bool key_place(const Cache& c, const int* table, int n, int64_t head, int* error, Place<S>* to) {
+__device__ __forceinline__ bool key_place(const CacheOf<S>& c, const int* table, int n, int64_t head, int* error, Place<S>* to) {
     const uint32_t page = c.page.div((uint32_t)n);
     const int id = table[page];
     if (id < 0 || id >= c.num_pages) {
@@ -362,16 +362,16 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
 constexpr int kRowsPiece = 1024;
 constexpr int kRowsShort = 128;  // with one wave
 template <typename T, typename S>
-int launch_rows(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
+int launch_rows(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, bool wide, int waves,
                 hipStream_t st);
 // Many rows (attend_tiles.h).
 template <typename T, typename S>
-int launch_tiles(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, int waves,
+int launch_tiles(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, int waves,
                  hipStream_t st);
 
 // A prefix of many rows and few rows that follow (attend_both.h).
 template <typename T, typename S>
-int launch_both(const Call& a, const Cache& c, const Stage& prefix, const Stage& own, int dim, bool wide,
+int launch_both(const Call& a, const CacheOf<S>& c, const Stage& prefix, const Stage& own, int dim, bool wide,
                 hipStream_t st);
 
 }  // namespace kv

@@ -252,7 +252,7 @@ int launch_join(const Call& a, const Cache& c, const Plan& p, hipStream_t st) {
 }
 
 template <typename T, typename S>
-int launch(const Call& a, const Cache& c, const Plan& p, int dim, hipStream_t st) {
+int launch(const Call& a, const CacheOf<S>& c, const Plan& p, int dim, hipStream_t st) {
     int rc;
     if (p.own_waves) {  // both stages have blocks of the same rows
         rc = launch_tiles<T, S>(a, c, p.prefix, p.own, dim, p.own_waves, st);
@@ -319,7 +319,7 @@ int attention(const char* name, const C* of, const gfd_attention* call, const in
     float* const part_o = p.bytes ? (float*)workspace : nullptr;
     float* const part_ml = p.bytes ? part_o + p.slots * rows * cache->head_dim : nullptr;
     float* const splits = p.bytes ? part_ml + p.slots * rows * 2 : nullptr;
-    const Cache c = make_cache(*of);
+    const auto c = make_cache(*of);
     const float raw = w.scale * c.k_scale;
     // Of a cap past what 32 bits hold of it, the quotients' ends: scores far below it stay as they are, others are +-cap_out.
     const auto held = [](double x) { return (float)std::min(x, 3.4028234e38); };
@@ -333,14 +333,15 @@ int attention(const char* name, const C* of, const gfd_attention* call, const in
                  w.num_q_heads, cache->num_heads, make_divider((uint32_t)(w.num_q_heads / cache->num_heads)), error_flag,
                  (f32x2*)part_ml, part_o, (int*)splits};
     const hipStream_t st = (hipStream_t)stream;
-    if (cache->dtype == kE2m1)
-        return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E2m1>(a, c, p, cache->head_dim, st)
-                                                  : launch<Fp16, E2m1>(a, c, p, cache->head_dim, st));
-    if (cache->dtype == GFD_E4M3)
-        return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, E4m3>(a, c, p, cache->head_dim, st)
-                                                  : launch<Fp16, E4m3>(a, c, p, cache->head_dim, st));
-    return launched(name, w.dtype == GFD_BF16 ? launch<Bf16, Bf16>(a, c, p, cache->head_dim, st)
-                                              : launch<Fp16, Fp16>(a, c, p, cache->head_dim, st));
+    const bool bf16 = w.dtype == GFD_BF16;
+    const int dim = cache->head_dim;
+    if constexpr (std::is_same<C, gfd_kv4_cache>::value) {
+        return launched(name, bf16 ? launch<Bf16, E2m1>(a, c, p, dim, st) : launch<Fp16, E2m1>(a, c, p, dim, st));
+    } else {
+        if (cache->dtype == GFD_E4M3)
+            return launched(name, bf16 ? launch<Bf16, E4m3>(a, c, p, dim, st) : launch<Fp16, E4m3>(a, c, p, dim, st));
+        return launched(name, bf16 ? launch<Bf16, Bf16>(a, c, p, dim, st) : launch<Fp16, Fp16>(a, c, p, dim, st));
+    }
 }
 
 template <typename C>
